@@ -60,6 +60,13 @@ SIGNATURES = {
     "fme_adv_norm": (_i32, [_P, _P, _i32, _P]),
     "fme_replay_add": (_i32, [_P, _P, _P, _i32, _P, _P, _P, _P, _P]),
     "fme_replay_gather": (_i32, [_P, _P, _P, _i32, _i32, _i32, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "fme_decay_attn_bytes": (_i64, [_P, _i32]),
+    "fme_decay_attn_fwd": (_i32, [_P, _P]),
+    "fme_decay_attn_bwd": (_i32, [_P, _P]),
+    "fme_decay_attn_step": (_i32, [_P, _P]),
+    "fme_group_norm_bytes": (_i64, [_P, _i32]),
+    "fme_group_norm_fwd": (_i32, [_P, _P]),
+    "fme_group_norm_bwd": (_i32, [_P, _P]),
     "fme_palette": (None, [_P]),
     "fme_resize": (_i32, [_P, _P, _i32, _P]),
     "fme_state_bytes": (_i64, []),
@@ -88,6 +95,29 @@ class FmeReplayBufs(ctypes.Structure):
 
 class FmeBuffers(ctypes.Structure):
     _fields_ = [(f, _P) for f in ("obs", "final_obs", "rew", "term", "trunc", "info", "ep_ret", "ep_len")]
+
+
+FME_F32, FME_BF16 = 0, 1
+FME_ACT_NONE, FME_ACT_RELU, FME_ACT_SILU = 0, 1, 2
+
+
+class FmeAttnTensor(ctypes.Structure):
+    _fields_ = [("p", _P), ("sn", _i64), ("st", _i64), ("sh", _i64)]
+
+
+class FmeDecayAttn(ctypes.Structure):
+    _fields_ = [(f, _i32) for f in ("n", "t", "h", "d", "dtype")] + [("scale", ctypes.c_float)] + \
+               [(f, FmeAttnTensor) for f in ("q", "k", "v", "o")] + \
+               [("log_decay", _P), ("reset", _P), ("reset_sn", _i64), ("reset_st", _i64), ("s_in", _P), ("s_out", _P)] + \
+               [(f, FmeAttnTensor) for f in ("d_o", "dq", "dk", "dv")] + \
+               [("ds_out", _P), ("ds_in", _P), ("saved", _P), ("ws", _P), ("ws_bytes", _i64)]
+
+
+class FmeGroupNorm(ctypes.Structure):
+    _fields_ = [(f, _i32) for f in ("n", "p", "c", "g", "dtype", "act")] + [("eps", ctypes.c_float)] + \
+               [("x", _P), ("x_sn", _i64), ("dy_sn", _i64)] + \
+               [(f, _P) for f in ("y", "w", "b", "mean", "rstd", "codes", "lo", "hi", "dy", "dx", "dw", "db", "ws")] + \
+               [("ws_bytes", _i64)]
 
 
 class FmeError(RuntimeError):

@@ -33,6 +33,7 @@
 #include "fme_ppo.cuh"
 #include "fme_replay.cuh"
 #include "../../include/fme.h"
+#include "fme_host.h"
 #include "fme_tables.h"
 
 using namespace fme;
@@ -621,6 +622,13 @@ namespace {
 
 thread_local std::string g_err;
 int fail(int code, const std::string& msg) { g_err = msg; return code; }
+}  // namespace
+// fme_host.h: the message of the other translation units' failures
+int fme::host_fail(int code, const char* msg) noexcept {
+    try { g_err = msg; } catch (...) { g_err.clear(); }
+    return code;
+}
+namespace {
 #define CK(call)                                                                              \
     do {                                                                                      \
         cudaError_t _e = (call);                                                              \

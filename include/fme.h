@@ -229,6 +229,82 @@ int fme_replay_gather(const FmeReplayBufs* rb, const int64_t* d_env, const int64
                       int64_t* d_act, float* d_reward, float* d_discount, float* d_terminal, int64_t* d_steps,
                       void* stream);
 
+/* ---- operators of a policy with memory (no counterpart in the reference, whose policy has none) ---- */
+#define FME_F32 0
+#define FME_BF16 1
+/* One (n, t, h, d) operand: strides in elements, the last axis contiguous, rows 16-byte aligned. A stride may be 0
+ * for an input that is shared along an axis. */
+typedef struct FmeAttnTensor {
+    void* p;
+    int64_t sn, st, sh;
+} FmeAttnTensor;
+/* Decayed linear attention over n sequences of t tokens and h heads of d features (32, 64 or 128):
+ *   S_t = (reset_t ? 0 : exp(log_decay[h]) * S_{t-1}) + k_t v_t^T,   o_t = scale * q_t S_t,
+ * S the (d, d) matrix of one sequence and head, fp32 (row: feature of k, column: feature of v). Restarts (an episode
+ * that begins at token t) leave nothing of earlier tokens, whatever their values were. log_decay is expected to be
+ * <= 0 (-inf: only the token itself counts). */
+typedef struct FmeDecayAttn {
+    int32_t n, t, h, d;
+    int32_t dtype;              /* FME_F32 or FME_BF16: q, k, v, o and their gradients */
+    float scale;
+    FmeAttnTensor q, k, v, o;
+    const float* log_decay;     /* (h,) fp32 */
+    const uint8_t* reset;       /* (n, t), 0 or 1, strides below; NULL: none */
+    int64_t reset_sn, reset_st;
+    const float* s_in;          /* (n, h, d, d) fp32 state before token 0; NULL: zeros */
+    float* s_out;               /* (n, h, d, d) fp32 state after the last token; NULL: not wanted */
+    FmeAttnTensor d_o, dq, dk, dv;   /* backward: gradient of o in, gradients of q, k, v out */
+    const float* ds_out;        /* gradient of s_out; NULL: zeros */
+    float* ds_in;               /* gradient of s_in; NULL: not wanted */
+    float* saved;               /* forward writes, backward reads; see fme_decay_attn_bytes. NULL in a forward pass
+                                   that no backward pass follows */
+    void* ws;                   /* workspace, 256-byte aligned */
+    int64_t ws_bytes;
+} FmeDecayAttn;
+/* Bytes that a call with these sizes needs: which = 0 forward workspace, 1 backward workspace, 2 `saved`.
+ * Negative on bad sizes. Nothing of it has to be initialised. */
+int64_t fme_decay_attn_bytes(const FmeDecayAttn* a, int32_t which);
+/* o and s_out from q, k, v, s_in. Async; allocates nothing. */
+int fme_decay_attn_fwd(const FmeDecayAttn* a, void* stream);
+/* dq, dk, dv and ds_in from q, k, v, s_in, saved, d_o and ds_out. Async; allocates nothing. Sums are taken in a fixed
+ * order: the same inputs give the same bits. */
+int fme_decay_attn_bwd(const FmeDecayAttn* a, void* stream);
+/* One token for each of n envs: t must be 1; s_in is the state to update and s_out where the new one goes (the same
+ * pointer updates it in place). Async. */
+int fme_decay_attn_step(const FmeDecayAttn* a, void* stream);
+
+#define FME_ACT_NONE 0
+#define FME_ACT_RELU 1
+#define FME_ACT_SILU 2
+/* Group norm with an activation, channels last: n samples of p pixels of c channels in g groups,
+ *   y = act((x - mean) * rstd * w + b),  mean and rstd = 1 / sqrt(var + eps) over p * (c / g) values.
+ * With `codes` the forward pass also stores x in 8 bits, code = rint((x - lo) * (255 * (1 / (hi - lo)))), each operation
+ * rounded to fp32, with lo and hi the least and largest x of the (sample, group), and 0 where they are equal; the backward
+ * pass takes lo + code * ((hi - lo) / 255) for x. */
+typedef struct FmeGroupNorm {
+    int32_t n, p, c, g;
+    int32_t dtype;              /* FME_F32 or FME_BF16: x, y, dy, dx */
+    int32_t act;
+    float eps;
+    const void* x;              /* backward: NULL where codes are given */
+    int64_t x_sn, dy_sn;        /* elements between samples of x and of dy; y, dx and codes are dense */
+    void* y;
+    const float *w, *b;         /* (c,) fp32; NULL: 1 and 0 */
+    float *mean, *rstd;         /* (n, g): forward writes, backward reads; may be NULL in a forward pass alone */
+    uint8_t* codes;             /* (n, p, c) or NULL */
+    float *lo, *hi;             /* (n, g), with codes */
+    const void* dy;
+    void* dx;
+    float *dw, *db;             /* (c,) fp32, both or neither */
+    void* ws;                   /* backward workspace, 256-byte aligned */
+    int64_t ws_bytes;
+} FmeGroupNorm;
+/* Workspace bytes of a call: which = 0 forward, 1 backward. Negative on bad sizes. */
+int64_t fme_group_norm_bytes(const FmeGroupNorm* a, int32_t which);
+int fme_group_norm_fwd(const FmeGroupNorm* a, void* stream);
+/* dx, dw and db; sums in a fixed order. Async; allocates nothing. */
+int fme_group_norm_bwd(const FmeGroupNorm* a, void* stream);
+
 /* Console state size in bytes of the reset-cache image (cf. fm_state_bytes, csrc/fastmario.cpp:631). */
 int64_t fme_state_bytes(void);
 const char* fme_last_error(void);

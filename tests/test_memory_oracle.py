@@ -1,0 +1,112 @@
+"""The float64 oracle of the memory policy's operators against differences, and the refusals that need no GPU."""
+import ctypes
+
+import pytest
+import torch
+from conftest import fme  # noqa: F401  (loads the package)
+
+import memory_oracle as mo
+from fast_mario_env_b200 import _native as N
+from fast_mario_env_b200 import ops
+
+
+def _case(seed=0, n=2, t=7, h=2, d=4):
+    r = torch.Generator().manual_seed(seed)
+    z = lambda *s: torch.randn(s, generator=r, dtype=torch.float64)  # noqa: E731
+    reset = torch.rand((n, t), generator=r) < 0.3
+    return dict(q=z(n, t, h, d), k=z(n, t, h, d), v=z(n, t, h, d), state=z(n, h, d, d)), -torch.rand(h, generator=r, dtype=torch.float64), \
+        reset, z(n, t, h, d), z(n, h, d, d)
+
+
+@pytest.mark.parametrize("seed", [0, 1])
+def test_attention_gradients_match_differences(seed):
+    """o and the last state are linear in each of q, k, v and the first state, so a difference is exact."""
+    x, g, reset, do, dl = _case(seed)
+    dq, dk, dv, ds = mo.attn_backward(x["q"], x["k"], x["v"], g, do, reset, x["state"], dl, 0.7)
+
+    def loss(**y):
+        z = {**x, **y}
+        o, last, _ = mo.attn_forward(z["q"], z["k"], z["v"], g, reset, z["state"], 0.7)
+        return (o * do).sum() + (last * dl).sum()
+
+    for name, grad in (("q", dq), ("k", dk), ("v", dv), ("state", ds)):
+        u = torch.randn(x[name].shape, generator=torch.Generator().manual_seed(9), dtype=torch.float64)
+        got = loss(**{name: x[name] + u}) - loss(**{name: x[name] - u})
+        assert torch.allclose(got, 2 * (grad * u).sum(), rtol=1e-11, atol=1e-11), name
+
+
+@pytest.mark.parametrize("name", ["none", "relu", "silu"])
+def test_norm_gradients_match_differences(name):
+    r = torch.Generator().manual_seed(3)
+    z = lambda *s: torch.randn(s, generator=r, dtype=torch.float64)  # noqa: E731
+    x, w, b, dy = z(3, 6, 5), z(6), z(6), z(3, 6, 5)
+    dx, dw, db = mo.norm_backward(x, 2, w, b, 1e-5, name, dy)
+    loss = lambda x, w, b: (mo.norm_forward(x, 2, w, b, 1e-5, name) * dy).sum()  # noqa: E731
+    e = 1e-6
+    for i, (t, grad) in enumerate(((x, dx), (w, dw), (b, db))):
+        u = z(*t.shape)
+        a, c = [x, w, b], [x, w, b]
+        a[i], c[i] = t + e * u, t - e * u
+        assert torch.allclose((loss(*a) - loss(*c)) / (2 * e), (grad * u).sum(), rtol=1e-7, atol=1e-7)
+
+
+def test_operators_refuse_cpu_tensors():
+    q = torch.zeros(1, 2, 1, 32)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.decay_attention(q, q, q, torch.zeros(1))
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.decay_attention_step(q[:, 0], q[:, 0], q[:, 0], torch.zeros(1), torch.zeros(1, 1, 32, 32))
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.group_norm_act(torch.zeros(2, 8), 2)
+
+
+def _attn(**kw):
+    a = N.FmeDecayAttn(n=1, t=1, h=1, d=64, dtype=N.FME_F32, scale=1.0, log_decay=256)
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+@pytest.mark.parametrize("kw, said", [
+    (dict(n=-1), ">= 0"), (dict(t=-1), ">= 0"), (dict(h=0), "h >= 1"), (dict(d=48), "32, 64 or 128"), (dict(dtype=7), "dtype"),
+    (dict(n=1 << 20, h=1 << 12), "pairs"), (dict(log_decay=None), "log_decay"), (dict(s_in=264), "16-byte"),
+    (dict(), "q, k, v"), (dict(q=(260, 64, 64, 64), k=(256, 64, 64, 64), v=(256, 64, 64, 64)), "16-byte"),
+    (dict(q=(256, 64, 64, 63), k=(256, 64, 64, 64), v=(256, 64, 64, 64)), "16-byte")])
+def test_library_refuses_bad_attention_arguments(kw, said):
+    """Refused on the host, before anything is launched."""
+    kw = {k: N.FmeAttnTensor(*v) if isinstance(v, tuple) else v for k, v in kw.items()}
+    a = _attn(**kw)
+    for f in (N.lib().fme_decay_attn_fwd, N.lib().fme_decay_attn_bwd, N.lib().fme_decay_attn_step):
+        assert f(ctypes.byref(a), None) == -1
+        assert said in N.last_error()
+
+
+def test_library_refuses_bad_step_and_missing_outputs():
+    rows = N.FmeAttnTensor(256, 64, 64, 64)
+    L = N.lib()
+    assert L.fme_decay_attn_step(ctypes.byref(_attn(t=2, q=rows, k=rows, v=rows)), None) == -1 and "t must be 1" in N.last_error()
+    assert L.fme_decay_attn_step(ctypes.byref(_attn(q=rows, k=rows, v=rows)), None) == -1 and "s_in and s_out" in N.last_error()
+    assert L.fme_decay_attn_fwd(ctypes.byref(_attn(q=rows, k=rows, v=rows)), None) == -1 and "o must be given" in N.last_error()
+    assert L.fme_decay_attn_bwd(ctypes.byref(_attn(q=rows, k=rows, v=rows)), None) == -1 and "gradients" in N.last_error()
+    assert L.fme_decay_attn_fwd(None, None) == -1
+    assert L.fme_decay_attn_bytes(None, 0) == -1 and L.fme_decay_attn_bytes(ctypes.byref(_attn()), 3) == -1
+
+
+@pytest.mark.parametrize("kw, said", [
+    (dict(n=-1), "sizes"), (dict(p=-1), "sizes"), (dict(g=3), "divide"), (dict(g=0), "divide"), (dict(c=8192, g=2), "4096"), (dict(dtype=5), "dtype"),
+    (dict(act=3), "activation"), (dict(), "required")])
+def test_library_refuses_bad_norm_arguments(kw, said):
+    a = N.FmeGroupNorm(n=1, p=1, c=8, g=2, dtype=N.FME_F32, act=0, eps=1e-5)
+    for k, v in kw.items():
+        setattr(a, k, v)
+    for f in (N.lib().fme_group_norm_fwd, N.lib().fme_group_norm_bwd):
+        assert f(ctypes.byref(a), None) == -1
+        assert said in N.last_error()
+    a = N.FmeGroupNorm(n=1, p=1, c=8, g=2, dtype=N.FME_F32, act=0, eps=1e-5, dw=256)
+    assert N.lib().fme_group_norm_bwd(ctypes.byref(a), None) == -1 and "together" in N.last_error()
+
+
+def test_empty_calls_need_no_buffers():
+    assert N.lib().fme_decay_attn_fwd(ctypes.byref(_attn(n=0)), None) == 0
+    a = N.FmeGroupNorm(n=0, p=1, c=8, g=2, dtype=N.FME_F32, act=0, eps=1e-5)
+    assert N.lib().fme_group_norm_fwd(ctypes.byref(a), None) == 0
