@@ -249,11 +249,12 @@ class _GroupNormAct(torch.autograd.Function):
         else:
             a.x, a.x_sn = kept.data_ptr(), kept.stride(0)
         a.dy, a.dy_sn, a.dx = dy.data_ptr(), dy.stride(0), dx.data_ptr()
-        dw = db = ws = None
+        dw = db = None
         if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
             dw, db = torch.empty((2, a.c), dtype=torch.float32, device=dev).unbind()
-            ws = _scratch(_bytes("fme_group_norm_bytes", a, 1), dev)
-            a.dw, a.db, a.ws, a.ws_bytes = dw.data_ptr(), db.data_ptr(), _p(ws), 0 if ws is None else ws.numel()
+            a.dw, a.db = dw.data_ptr(), db.data_ptr()
+        ws = _scratch(_bytes("fme_group_norm_bytes", a, 1), dev)
+        a.ws, a.ws_bytes = _p(ws), 0 if ws is None else ws.numel()
         _call("fme_group_norm_bwd", a, dev)
         return dx, dw if ctx.needs_input_grad[1] else None, db if ctx.needs_input_grad[2] else None, None, None, None, None
 
