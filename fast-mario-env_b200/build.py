@@ -19,7 +19,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libfme_cuda.so")
 SOURCES = {"fme.cu": ["--fmad=false"], "fme_attn.cu": [], "fme_norm.cu": []}   # source: flags of its own
 DEPS = ["fme.cu", "fme_kernels.cuh", "fme_core.h", "fme_agent.h", "fme_render.h", "fme_defs.h", "fme_tables.h", "fme_fast.h", "fme_dp.h", "fme_ppo.cuh", "fme_replay.cuh",
-        "fme_host.h", "fme_attn.cu", "fme_norm.cu"]
+        "fme_host.h", "fme_mma.cuh", "fme_attn.cu", "fme_norm.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

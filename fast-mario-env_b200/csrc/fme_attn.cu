@@ -1,129 +1,630 @@
 // fme_attn.cu - decayed linear attention with restarts: over whole sequences, forward and backward, and one token at
 // a time. Sizes, layouts and the recurrence are those of include/fme.h (FmeDecayAttn).
-#include <cuda_bf16.h>
-#include <cuda_runtime.h>
+//
+// Sequences are taken in chunks of C tokens. With S the state before a chunk, L_ij = lambda^(i-j) where j <= i and no restart
+// lies in (j, i], a_i = lambda^(i+1) where none lies in [0, i], z_j = lambda^(last-j) where none lies in (j, last], all else 0:
+//   o    = scale ( (q k^T . L) v + a (q S) )                      S'  = thru S + (z k)^T v
+//   dq   = scale ( (do v^T . L) k + a (do S^T) )                  U   = thru U' + scale (a q)^T do
+//   dk   = scale (do v^T . L)^T q + z (v U'^T)                    dv  = scale (q k^T . L)^T do + z (k U')
+// with U' the gradient of the state after the chunk and U that before it. A CTA walks the chunks of one sequence and head and
+// keeps S (or U) in registers, fp32, so that q, k, v (and do) are read once and o (dq, dk, dv) written once; the forward pass of a
+// training step also stores S before every chunk but the first, in the operands' type, as the products read it.
+// Where there are too few sequences and heads to fill the GPU, the chunks are split into segments: first every segment's own
+// part of the state, then these joined in order, then all segments at once with the state that they begin with.
 #include <math.h>
-#include <stdint.h>
 
 #include "fme_host.h"
+#include "fme_mma.cuh"
 
 namespace fme {
 namespace {
-
-__device__ __forceinline__ float to_f(float x) { return x; }
-__device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
-template <typename T> __device__ __forceinline__ T from_f(float x);
-template <> __device__ __forceinline__ float from_f<float>(float x) { return x; }
-template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x) { return __float2bfloat16(x); }
-
-// ---------------------------------------------------------------- token by token
-// All four products of the operator are one recurrence over a (D, D) matrix M, with an index b that is summed over and
-// an index a that the output keeps:   M[b][a] += x_b y_a;   out_a = sum_b z_b M[b][a]
-//   o  : forward,  M = S,   x = k, y = v,  z = q       dq : forward,  M = S^T, x = v,  y = k, z = do
-//   dv : backward, M = U,   x = q, y = do, z = k       dk : backward, M = U^T, x = do, y = q, z = v
-// with U_t = scale q_t do_t^T + (reset_{t+1} ? 0 : lambda U_{t+1}) the gradient of S_t. Going forward the decay comes
-// before the token's own product, going backward after it.
-template <typename T> struct Sweep {
-    const T *x, *y, *z;
-    T* out;
-    int64_t xt, yt, zt, ot;
-    const uint8_t* reset;
-    int64_t rt;
-    const float* m_in;   // element (b, a) at b * mb + a * ma
-    float* m_out;
-    int mb, ma;
-    float lam, xs, os;
-    int t;
-    bool back;
-};
-
-constexpr int SEQ_THREADS = 256;
-
-// One CTA; thread (r, a) holds D / R rows b of column a in registers. One token costs two barriers.
-template <typename T, int D> __device__ void sweep(const Sweep<T>& s, float* sm) {
-    constexpr int R = SEQ_THREADS / D, PER = D / R;
-    const int a = threadIdx.x % D, r = threadIdx.x / D;
-    float* in = sm;                 // x, y, z
-    float* part = sm + 3 * D;       // R x D
-    float m[PER];
-#pragma unroll
-    for (int i = 0; i < PER; i++) m[i] = s.m_in ? s.m_in[(r * PER + i) * s.mb + a * s.ma] : 0.f;
-    for (int u = 0; u < s.t; u++) {
-        const int64_t t = s.back ? s.t - 1 - u : u;
-        for (int i = threadIdx.x; i < 3 * D; i += SEQ_THREADS) {
-            const int w = i / D, e = i % D;
-            in[i] = w == 0 ? to_f(s.x[t * s.xt + e]) * s.xs : w == 1 ? to_f(s.y[t * s.yt + e]) : to_f(s.z[t * s.zt + e]);
-        }
-        const bool cut = s.reset && s.reset[t * s.rt];
-        __syncthreads();
-        const float y = in[D + a];
-        float acc = 0.f;
-#pragma unroll
-        for (int i = 0; i < PER; i++) {
-            if (!s.back) m[i] = cut ? 0.f : m[i] * s.lam;
-            m[i] = fmaf(in[r * PER + i], y, m[i]);
-            acc = fmaf(in[2 * D + r * PER + i], m[i], acc);
-            if (s.back) m[i] = cut ? 0.f : m[i] * s.lam;
-        }
-        part[r * D + a] = acc;
-        __syncthreads();
-        if (r == 0) {
-            float o = 0.f;
-#pragma unroll
-            for (int i = 0; i < R; i++) o += part[i * D + a];
-            s.out[t * s.ot + a] = from_f<T>(o * s.os);
-        }
-    }
-    if (s.m_out) {
-#pragma unroll
-        for (int i = 0; i < PER; i++) s.m_out[(r * PER + i) * s.mb + a * s.ma] = m[i];
-    }
-}
 
 template <typename T> __device__ __forceinline__ T* at(const FmeAttnTensor& x, int64_t n, int64_t h) {
     return reinterpret_cast<T*>(x.p) + n * x.sn + h * x.sh;
 }
 
-// blockIdx.x: sequence and head; blockIdx.y: which of the sweeps (forward: o; backward: dq, dv, dk)
-template <typename T, int D, bool BWD>
-__global__ void __launch_bounds__(SEQ_THREADS) k_sweep(const FmeDecayAttn A) {
-    __shared__ float sm[3 * D + SEQ_THREADS];
-    const int64_t n = blockIdx.x / A.h, h = blockIdx.x % A.h, mat = (int64_t)blockIdx.x * D * D;
-    Sweep<T> s{};
-    s.reset = A.reset ? A.reset + n * A.reset_sn : nullptr;
-    s.rt = A.reset_st;
-    s.lam = expf(A.log_decay[h]);
-    s.xs = s.os = 1.f;
-    s.t = A.t;
-    T *q = at<T>(A.q, n, h), *k = at<T>(A.k, n, h), *v = at<T>(A.v, n, h);
-    if (!BWD) {
-        s.x = k; s.xt = A.k.st; s.y = v; s.yt = A.v.st; s.z = q; s.zt = A.q.st;
-        s.out = at<T>(A.o, n, h); s.ot = A.o.st; s.os = A.scale;
-        s.m_in = A.s_in ? A.s_in + mat : nullptr; s.m_out = A.s_out ? A.s_out + mat : nullptr; s.mb = D; s.ma = 1;
-    } else {
-        T* g = at<T>(A.d_o, n, h);
-        if (blockIdx.y == 0) {
-            s.x = v; s.xt = A.v.st; s.y = k; s.yt = A.k.st; s.z = g; s.zt = A.d_o.st;
-            s.out = at<T>(A.dq, n, h); s.ot = A.dq.st; s.os = A.scale;
-            s.m_in = A.s_in ? A.s_in + mat : nullptr; s.mb = 1; s.ma = D;
-        } else {
-            s.back = true; s.xs = A.scale;
-            s.m_in = A.ds_out ? A.ds_out + mat : nullptr;
-            if (blockIdx.y == 1) {
-                s.x = q; s.xt = A.q.st; s.y = g; s.yt = A.d_o.st; s.z = k; s.zt = A.k.st;
-                s.out = at<T>(A.dv, n, h); s.ot = A.dv.st;
-                s.m_out = A.ds_in ? A.ds_in + mat : nullptr; s.mb = D; s.ma = 1;
-            } else {
-                s.x = g; s.xt = A.d_o.st; s.y = q; s.yt = A.q.st; s.z = v; s.zt = A.v.st;
-                s.out = at<T>(A.dk, n, h); s.ot = A.dk.st;
-                s.mb = 1; s.ma = D;
-            }
+// Sizes of a CTA: D / 16 warps; warp w owns rows 16 w of the state and, of a chunk's outputs, rows 16 (w % RB) and columns
+// NC (w / RB). C is 64 but for D = 32 (two warps) and D = 128 in fp32 (shared memory), 32.
+template <typename T, int D> struct Shape {
+    static constexpr int C = D == 32 || (D == 128 && sizeof(T) == 4) ? 32 : 64;
+    static constexpr int NW = D / 16, NT = 32 * NW, RB = C / 16, CG = NW / RB, NC = D / CG;
+    static constexpr int TILE = C * D * (int)sizeof(T), MAT = D * D * (int)sizeof(T);
+    static constexpr int STAGE = 16 * NC * (int)sizeof(T);   // a warp's outputs on their way out
+    static constexpr int FLOATS = 2 * 72;                    // powers and weights
+};
+
+// Where a chunk restarts. Bit i: token i does; valid tokens only.
+struct Cuts {
+    uint64_t m;
+    int n;   // tokens in the chunk
+    __device__ __forceinline__ int last_up_to(int i) const {   // latest restart at or before i, -1: none
+        const uint64_t x = m & (~0ull >> (63 - i));
+        return 63 - __clzll((long long)x);
+    }
+    __device__ __forceinline__ int next_after(int j) const {   // earliest restart after j, 64: none
+        const uint64_t x = j >= 63 ? 0ull : m & (~0ull << (j + 1));
+        return x ? __ffsll((long long)x) - 1 : 64;
+    }
+};
+
+struct ResetBytes {
+    uint32_t a = 0, b = 0;
+    __device__ __forceinline__ void load(const uint8_t* r, int64_t rt, int t0, int n) {
+        const int l = threadIdx.x & 31;
+        a = r && l < n ? r[(t0 + l) * rt] : 0u;
+        b = r && l + 32 < n ? r[(t0 + l + 32) * rt] : 0u;
+    }
+    __device__ __forceinline__ uint64_t bits() const {
+        const uint32_t lo = __ballot_sync(0xffffffffu, a != 0u), hi = __ballot_sync(0xffffffffu, b != 0u);
+        return ((uint64_t)hi << 32) | lo;
+    }
+};
+
+// rows of one operand's chunk to shared memory; rows past the sequence's end become zeros
+template <typename T, int D, int C, int NT>
+__device__ __forceinline__ void load_tile(const Tile<T, D>& dst, const T* src, int64_t st, int t0, int n) {
+    constexpr int PIECES = D / Tile<T, D>::PER;
+#pragma unroll
+    for (int i = 0; i < C * PIECES / NT; i++) {
+        const int e = i * NT + threadIdx.x, row = e / PIECES, col = (e % PIECES) * Tile<T, D>::PER;
+        const bool in = row < n;
+        cp16(dst.addr(row, col), src + (in ? (t0 + row) * st + col : 0), in);
+    }
+}
+
+// A warp's 16 x NC accumulators to rows row0.. and columns col0.. of a (t, h, d) output: through shared memory, so that a row's
+// pieces leave as 16 bytes each
+template <typename T, int NC>
+__device__ __forceinline__ void store_rows(char* stage, const float (&acc)[NC / 8][4], T* dst, int64_t st, int row0, int col0, int t0, int n) {
+    constexpr int PW = NC < 32 ? 32 : NC;
+    static_assert(NC >= 32, "");
+    const Tile<T, PW> s(stage);
+    const int l = threadIdx.x & 31, g = l >> 2, c = l & 3;
+#pragma unroll
+    for (int i = 0; i < NC / 8; i++) {
+        s.put2(g, 8 * i + 2 * c, acc[i][0], acc[i][1]);
+        s.put2(g + 8, 8 * i + 2 * c, acc[i][2], acc[i][3]);
+    }
+    __syncwarp();
+    constexpr int PIECES = NC / Tile<T, PW>::PER;
+#pragma unroll
+    for (int i = 0; i < 16 * PIECES / 32; i++) {
+        const int e = i * 32 + l, row = e / PIECES, col = (e % PIECES) * Tile<T, PW>::PER;
+        if (row0 + row < n)
+            *reinterpret_cast<uint4*>(dst + (t0 + row0 + row) * st + col0 + col) = *reinterpret_cast<const uint4*>(s.gen + s.off(row, col));
+    }
+    __syncwarp();
+}
+
+template <int N> __device__ __forceinline__ bool not_finite(const float (&a)[N][4]) {
+    float z = 0.f;   // x * 0 is NaN unless x is finite
+#pragma unroll
+    for (int i = 0; i < N; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) z = fmaf(a[i][j], 0.f, z);
+    return z != 0.f;
+}
+
+template <int N> __device__ __forceinline__ void zero(float (&a)[N][4]) {
+#pragma unroll
+    for (int i = 0; i < N; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) a[i][j] = 0.f;
+}
+
+// acc (16 x 8 NB) += A (16 x K) B: A rows of one tile; B rows of another as columns, or, TR, its columns as columns
+template <typename T, int NB, int K, bool TR, typename TA, typename TB>
+__device__ __forceinline__ void product(float (&acc)[NB][4], const TA& a, int m, const TB& b, int n) {
+    using F = Frag<T>;
+#pragma unroll
+    for (int k = 0; k < K; k += F::KS) {
+        const typename F::A fa = F::ldA(a, m, k);
+#pragma unroll
+        for (int i = 0; i < NB; i += 2) {
+            typename F::B b0, b1;
+            if (TR) F::template ldBt<true>(b, k, n + 8 * i, b0, b1);
+            else F::ldB(b, n + 8 * i, k, b0, b1);
+            F::mma(acc[i], fa, b0);
+            F::mma(acc[i + 1], fa, b1);
         }
     }
-    sweep<T, D>(s, sm);
+}
+
+// One chunk's scores: p[row][col] = (a_row . b_col) L scale for rows row0.. against all C columns. UP: rows are i, columns j
+// (a = q or do, b = k or v); otherwise rows are j and columns i. Blocks that L empties are skipped.
+template <typename T, int D, int C, bool UP>
+__device__ __forceinline__ void scores(float (&p)[C / 8][4], const Tile<T, D>& a, const Tile<T, D>& b, int row0, const Cuts& cuts, const float* pw, float scale) {
+    using F = Frag<T>;
+    zero(p);
+#pragma unroll
+    for (int k = 0; k < D; k += F::KS) {
+        const typename F::A fa = F::ldA(a, row0, k);
+#pragma unroll
+        for (int i = 0; i < C / 8; i += 2) {
+            if (UP ? 8 * i > row0 : 8 * i < row0) continue;   // 16 columns against 16 rows
+            typename F::B b0, b1;
+            F::ldB(b, 8 * i, k, b0, b1);
+            F::mma(p[i], fa, b0);
+            F::mma(p[i + 1], fa, b1);
+        }
+    }
+    const int l = threadIdx.x & 31, g = l >> 2, c = l & 3;
+#pragma unroll
+    for (int half = 0; half < 2; half++) {
+        const int row = row0 + g + 8 * half;
+        const int lim = UP ? cuts.last_up_to(row) : cuts.next_after(row);
+#pragma unroll
+        for (int i = 0; i < C / 8; i++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const int col = 8 * i + 2 * c + e;
+                float& x = p[i][2 * half + e];
+                const bool in = UP ? col <= row && col >= lim : col >= row && col < lim;
+                const int far = UP ? row - col : col - row;
+                x = in ? x * (pw[far < 0 ? 0 : far] * scale) : 0.f;
+            }
+    }
+}
+
+// acc += p (16 x C) times rows of a tile, blocks that the scores left empty skipped
+template <typename T, int D, int C, int NB, bool UP>
+__device__ __forceinline__ void apply_scores(float (&acc)[NB][4], const float (&p)[C / 8][4], const Tile<T, D>& b, int row0, int n) {
+    using F = Frag<T>;
+#pragma unroll
+    for (int ks = 0; ks < C / F::KS; ks++) {
+        if (UP ? ks * F::KS > row0 + 15 : (ks + 1) * F::KS <= row0) continue;
+        const typename F::A fa = F::chain(p, ks);
+#pragma unroll
+        for (int i = 0; i < NB; i += 2) {
+            typename F::B b0, b1;
+            F::template ldBt<false>(b, ks * F::KS, n + 8 * i, b0, b1);
+            F::mma(acc[i], fa, b0);
+            F::mma(acc[i + 1], fa, b1);
+        }
+    }
+}
+
+// state (rows m0..m0+15 of the D x D matrix) += (w a)^T b over the chunk's tokens; TWO: the scaled rows in 16 bits at least
+template <typename T, int D, int C, bool TWO>
+__device__ __forceinline__ void outer(float (&s)[D / 8][4], const Tile<T, D>& a, int m0, const float* w, const Tile<T, D>& b) {
+    using F = Frag<T>;
+#pragma unroll
+    for (int k = 0; k < C; k += F::KS) {
+        const typename F::A2 fa = F::template ldAt<TWO>(a, k, m0, w);
+#pragma unroll
+        for (int i = 0; i < D / 8; i += 2) {
+            typename F::B b0, b1;
+            F::template ldBt<false>(b, k, 8 * i, b0, b1);
+            F::template mma2<TWO>(s[i], fa, b0);
+            F::template mma2<TWO>(s[i + 1], fa, b1);
+        }
+    }
+}
+
+template <int D> __device__ __forceinline__ void keep_state(float (&s)[D / 8][4], const Cuts& cuts, const float* pw) {
+    const float thru = pw[cuts.n];
+    const bool cut = cuts.m != 0ull;
+#pragma unroll
+    for (int i = 0; i < D / 8; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) s[i][j] = cut ? 0.f : s[i][j] * thru;
+}
+
+// A warp's rows of the state in a tile of the operands' type
+template <typename T, int D> __device__ __forceinline__ void put_state(const Tile<T, D>& m, const float (&s)[D / 8][4], int row0) {
+    const int l = threadIdx.x & 31, g = l >> 2, c = l & 3;
+#pragma unroll
+    for (int i = 0; i < D / 8; i++) {
+        m.put2(row0 + g, 8 * i + 2 * c, s[i][0], s[i][1]);
+        m.put2(row0 + g + 8, 8 * i + 2 * c, s[i][2], s[i][3]);
+    }
+}
+// ... and to or from a (d, d) fp32 matrix. FLIP: the warp's rows are the matrix's columns.
+template <int D, bool FLIP, bool STORE, typename P> __device__ __forceinline__ void move_state(float (&s)[D / 8][4], P* mat, int row0) {
+    const int l = threadIdx.x & 31, g = l >> 2, c = l & 3;
+#pragma unroll
+    for (int i = 0; i < D / 8; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int row = row0 + g + 8 * (j >> 1), col = 8 * i + 2 * c + (j & 1);
+            P* e = mat + (FLIP ? col * D + row : row * D + col);
+            if constexpr (STORE) *e = s[i][j];
+            else s[i][j] = *e;
+        }
+}
+// Between the segments' kernels the state stays in the order of the registers
+template <int D, int NT, bool STORE> __device__ __forceinline__ void move_part(float (&s)[D / 8][4], float* ws, int64_t item) {
+    float4* p = reinterpret_cast<float4*>(ws) + item * (D / 8) * NT + threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < D / 8; i++) {
+        if (STORE) p[i * NT] = make_float4(s[i][0], s[i][1], s[i][2], s[i][3]);
+        else { const float4 f = p[i * NT]; s[i][0] = f.x; s[i][1] = f.y; s[i][2] = f.z; s[i][3] = f.w; }
+    }
+}
+
+// ---------------------------------------------------------------- token by token
+// A product with 0 keeps the NaN of a masked token, so a chunk whose result is not finite is done again by the recurrence
+// itself, in which a restart drops what was before. A warp holds 16 rows r of a matrix M and walks the tokens:
+//   M[r][c] += x_r y_c (after the decay going forward, before it going backward),   out_r = f sum_c M[r][c] z_c
+template <typename T, int D, bool BACK>
+__device__ __forceinline__ void walk(float (&m)[D / 8][4], const Tile<T, D>& x, const Tile<T, D>& y, const Tile<T, D>& z, float xf, float f,
+                                     int row0, const Cuts& cuts, float lam, T* out, int64_t st, int t0) {
+    const int l = threadIdx.x & 31, g = l >> 2, c = l & 3;
+    for (int u = 0; u < cuts.n; u++) {
+        const int t = BACK ? cuts.n - 1 - u : u;
+        const bool cut = (cuts.m >> t) & 1;
+        const float x0 = to_f(x.at(t, row0 + g)) * xf, x1 = to_f(x.at(t, row0 + g + 8)) * xf;
+        float o0 = 0.f, o1 = 0.f;
+#pragma unroll
+        for (int i = 0; i < D / 8; i++) {
+            const float2 yy = y.two(t, 8 * i + 2 * c), zz = z.two(t, 8 * i + 2 * c);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                float& s = m[i][j];
+                if (!BACK) s = cut ? 0.f : s * lam;
+                s = fmaf(j < 2 ? x0 : x1, j & 1 ? yy.y : yy.x, s);
+                float& o = j < 2 ? o0 : o1;
+                o = fmaf(s, j & 1 ? zz.y : zz.x, o);
+                if (BACK) s = cut ? 0.f : s * lam;
+            }
+        }
+#pragma unroll
+        for (int d = 1; d < 4; d <<= 1) { o0 += __shfl_xor_sync(0xffffffffu, o0, d); o1 += __shfl_xor_sync(0xffffffffu, o1, d); }
+        if (out && c == 0) {
+            out[(t0 + t) * st + row0 + g] = from_f<T>(o0 * f);
+            out[(t0 + t) * st + row0 + g + 8] = from_f<T>(o1 * f);
+        }
+    }
+}
+
+struct Walkers {   // the grid's layout: CTA = (sequence and head) * segs + segment
+    int chunks, segs, per;   // chunks of the sequence, segments, chunks of a segment
+    float* parts;            // state of the segments: D * D floats each, then one float each: what a segment passes on
+};
+
+__device__ __forceinline__ void powers(float* pw, int n, float log2_lam) {
+    for (int i = threadIdx.x; i < n; i += blockDim.x) pw[i] = i ? exp2f(log2_lam * (float)i) : 1.f;
+}
+
+constexpr float LOG2E = 1.44269504088896340736f;
+
+// The forward pass of a segment (state rows: features of v). LOCAL: only its part of the state, from zero (the first: from s_in).
+template <typename T, int D, bool LOCAL, int MINB>
+__global__ void __launch_bounds__(Shape<T, D>::NT, MINB) k_attn_fwd(const FmeDecayAttn A, const Walkers W) {
+    using Z = Shape<T, D>;
+    using Ti = Tile<T, D>;
+    constexpr int C = Z::C, NT = Z::NT, NC = Z::NC;
+    extern __shared__ __align__(1024) char sm[];
+    const Ti tk(sm), tv(sm + Z::TILE), tq(sm + 2 * Z::TILE), ts(sm + 3 * Z::TILE);
+    float* pw = reinterpret_cast<float*>(sm + (LOCAL ? 2 * Z::TILE : 3 * Z::TILE + Z::MAT));   // C + 1
+    float* z = pw + 72;                                                                       // C
+    const int warp = threadIdx.x >> 5, l = threadIdx.x & 31, g = l >> 2;
+    const int64_t pair = LOCAL ? blockIdx.x / (W.segs - 1) : blockIdx.x / W.segs;
+    const int seg = LOCAL ? blockIdx.x % (W.segs - 1) : blockIdx.x % W.segs;
+    const int64_t n = pair / A.h, h = pair % A.h;
+    const T *q = at<T>(A.q, n, h), *k = at<T>(A.k, n, h), *v = at<T>(A.v, n, h);
+    T* o = at<T>(A.o, n, h);
+    const uint8_t* reset = A.reset ? A.reset + n * A.reset_sn : nullptr;
+    const int c0 = seg * W.per, c1 = min(c0 + W.per, W.chunks);
+    const int row0 = 16 * (warp % Z::RB), col0 = NC * (warp / Z::RB), m0 = 16 * warp;
+    const float g2 = A.log_decay[h] * LOG2E;
+    float s[D / 8][4];
+    bool some = true;   // whether the state before the chunk may be other than zero
+    ResetBytes rb;
+    auto fetch = [&](int c) {
+        const int t0 = c * C, nv = min(C, A.t - t0);
+        load_tile<T, D, C, NT>(tk, k, A.k.st, t0, nv);
+        load_tile<T, D, C, NT>(tv, v, A.v.st, t0, nv);
+        if (!LOCAL) load_tile<T, D, C, NT>(tq, q, A.q.st, t0, nv);
+        cp_commit();
+        rb.load(reset, A.reset_st, t0, nv);
+    };
+    if (c0 < c1) fetch(c0);
+    powers(pw, C + 1, g2);
+    if (seg > 0 && !LOCAL) move_part<D, NT, false>(s, W.parts, pair * (W.segs - 1) + seg - 1);
+    else if (seg == 0 && A.s_in) move_state<D, true, false>(s, A.s_in + pair * D * D, m0);
+    else { zero(s); some = false; }
+    if (!LOCAL && some) put_state(ts, s, m0);
+    uint64_t any_cut = 0;
+    for (int c = c0; c < c1; c++) {
+        const int t0 = c * C;
+        cp_wait<0>();
+        __syncthreads();
+        const Cuts cuts{rb.bits(), min(C, A.t - t0)};
+        any_cut |= cuts.m;
+        const int last = cuts.last_up_to(63);
+        bool again = false;
+        if constexpr (!LOCAL) {
+            float acc[NC / 8][4], p[C / 8][4];
+            zero(acc);
+            if (some) {
+                product<T, NC / 8, D, false>(acc, tq, row0, ts, col0);
+                const bool in0 = cuts.last_up_to(row0 + g) < 0, in1 = cuts.last_up_to(row0 + g + 8) < 0;
+                const float a0 = pw[row0 + g + 1] * A.scale, a1 = pw[row0 + g + 9] * A.scale;
+#pragma unroll
+                for (int i = 0; i < NC / 8; i++) {
+                    acc[i][0] = in0 ? acc[i][0] * a0 : 0.f; acc[i][1] = in0 ? acc[i][1] * a0 : 0.f;
+                    acc[i][2] = in1 ? acc[i][2] * a1 : 0.f; acc[i][3] = in1 ? acc[i][3] * a1 : 0.f;
+                }
+            }
+            scores<T, D, C, true>(p, tq, tk, row0, cuts, pw, A.scale);
+            apply_scores<T, D, C, NC / 8, true>(acc, p, tv, row0, col0);
+            again = __syncthreads_or(not_finite(acc));
+            // q and the old state have been read by all: the q tile takes the outputs
+            if (!again) store_rows<T, NC>(sm + 2 * Z::TILE + warp * Z::STAGE, acc, o, A.o.st, row0, col0, t0, cuts.n);
+        }
+        const bool more = c + 1 < c1;
+        if (more || LOCAL || A.s_out || A.saved) {
+            const int j = threadIdx.x;
+            if (j < C) z[j] = j < cuts.n && j >= last ? pw[cuts.n - 1 - j] : 0.f;
+            __syncthreads();
+            if (LOCAL) {
+                float add[D / 8][4];
+                zero(add);
+                outer<T, D, C, true>(add, tv, m0, z, tk);
+                again = __any_sync(0xffffffffu, not_finite(add));
+                if (!again) {
+                    keep_state<D>(s, cuts, pw);
+#pragma unroll
+                    for (int i = 0; i < D / 8; i++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) s[i][j] += add[i][j];
+                }
+            } else if (!again) {
+                keep_state<D>(s, cuts, pw);
+                outer<T, D, C, true>(s, tv, m0, z, tk);
+            }
+        }
+        if (again) walk<T, D, false>(s, tv, tk, LOCAL ? tk : tq, 1.f, A.scale, m0, cuts, pw[1], LOCAL ? (T*)nullptr : o, A.o.st, t0);
+        some = true;
+        if constexpr (!LOCAL) {
+            if (more || A.saved) put_state(ts, s, m0);
+            if (A.saved && c + 1 < W.chunks) {
+                __syncwarp();
+                T* dst = reinterpret_cast<T*>(A.saved) + ((pair * (W.chunks - 1) + c) * D + m0) * D;
+                constexpr int PIECES = D / Ti::PER;
+#pragma unroll
+                for (int i = 0; i < 16 * PIECES / 32; i++) {
+                    const int e = i * 32 + l, row = e / PIECES, col = (e % PIECES) * Ti::PER;
+                    *reinterpret_cast<uint4*>(dst + row * D + col) = *reinterpret_cast<const uint4*>(ts.gen + ts.off(m0 + row, col));
+                }
+            }
+        }
+        __syncthreads();   // the tiles have been read by all
+        if (more) fetch(c + 1);
+    }
+    if (LOCAL) {
+        move_part<D, NT, true>(s, W.parts, blockIdx.x);
+        if (threadIdx.x == 0) {
+            const int len = min(c1 * C, A.t) - c0 * C;
+            W.parts[(int64_t)gridDim.x * D * D + blockIdx.x] = any_cut ? -1.f : exp2f(g2 * (float)len);
+        }
+    } else if (A.s_out && seg == W.segs - 1) {
+        move_state<D, true, true>(s, A.s_out + pair * D * D, m0);
+    }
+}
+
+// The backward pass of a segment, from its last chunk to its first (state rows: features of k). LOCAL: only its part of the
+// state's gradient, from zero (the last: from ds_out); segments then count from the end. TWO: ds_in is wanted.
+template <typename T, int D, bool LOCAL, bool TWO, int MINB>
+__global__ void __launch_bounds__(Shape<T, D>::NT, MINB) k_attn_bwd(const FmeDecayAttn A, const Walkers W) {
+    using Z = Shape<T, D>;
+    using Ti = Tile<T, D>;
+    constexpr int C = Z::C, NT = Z::NT, NC = Z::NC;
+    extern __shared__ __align__(1024) char sm[];
+    const Ti tq(sm), tg(sm + Z::TILE), tk(sm + 2 * Z::TILE), tv(sm + 3 * Z::TILE), ts(sm + 4 * Z::TILE), tu(sm + 4 * Z::TILE + Z::MAT);
+    char* stage = sm + 4 * Z::TILE + 2 * Z::MAT + (threadIdx.x >> 5) * Z::STAGE;
+    float* pw = reinterpret_cast<float*>(sm + (LOCAL ? 2 * Z::TILE : 4 * Z::TILE + 2 * Z::MAT + Z::NW * Z::STAGE));
+    float* a = pw + 72;
+    const int warp = threadIdx.x >> 5, l = threadIdx.x & 31, g = l >> 2;
+    const int64_t pair = LOCAL ? blockIdx.x / (W.segs - 1) : blockIdx.x / W.segs;
+    const int rseg = LOCAL ? blockIdx.x % (W.segs - 1) : blockIdx.x % W.segs;   // 0: the last in time
+    const int seg = W.segs - 1 - rseg;
+    const int64_t n = pair / A.h, h = pair % A.h;
+    const T *q = at<T>(A.q, n, h), *k = at<T>(A.k, n, h), *v = at<T>(A.v, n, h), *go = at<T>(A.d_o, n, h);
+    T *dq = at<T>(A.dq, n, h), *dk = at<T>(A.dk, n, h), *dv = at<T>(A.dv, n, h);
+    const uint8_t* reset = A.reset ? A.reset + n * A.reset_sn : nullptr;
+    const int c0 = seg * W.per, c1 = min(c0 + W.per, W.chunks);
+    const int row0 = 16 * (warp % Z::RB), col0 = NC * (warp / Z::RB), m0 = 16 * warp;
+    const float g2 = A.log_decay[h] * LOG2E;
+    float u[D / 8][4];
+    bool some = true;   // whether the gradient of the state after the chunk may be other than zero
+    ResetBytes rb;
+    auto fetch = [&](int c) {
+        const int t0 = c * C, nv = min(C, A.t - t0);
+        load_tile<T, D, C, NT>(tq, q, A.q.st, t0, nv);
+        load_tile<T, D, C, NT>(tg, go, A.d_o.st, t0, nv);
+        if (!LOCAL) {
+            load_tile<T, D, C, NT>(tk, k, A.k.st, t0, nv);
+            load_tile<T, D, C, NT>(tv, v, A.v.st, t0, nv);
+            if (c > 0) load_tile<T, D, D, NT>(ts, reinterpret_cast<const T*>(A.saved) + (pair * (W.chunks - 1) + c - 1) * D * D, D, 0, D);
+            else if (A.s_in) {
+                for (int i = threadIdx.x; i < D * D; i += NT) ts.at(i % D, i / D) = from_f<T>(A.s_in[pair * D * D + i]);
+            }
+        }
+        cp_commit();
+        rb.load(reset, A.reset_st, t0, nv);
+    };
+    if (c0 < c1) fetch(c1 - 1);
+    powers(pw, C + 1, g2);
+    if (rseg > 0 && !LOCAL) move_part<D, NT, false>(u, W.parts, pair * (W.segs - 1) + rseg - 1);
+    else if (rseg == 0 && A.ds_out) move_state<D, false, false>(u, A.ds_out + pair * D * D, m0);
+    else { zero(u); some = false; }
+    uint64_t any_cut = 0;
+    for (int c = c1 - 1; c >= c0; c--) {
+        const int t0 = c * C;
+        if (!LOCAL && some) put_state(tu, u, m0);
+        cp_wait<0>();
+        __syncthreads();
+        const Cuts cuts{rb.bits(), min(C, A.t - t0)};
+        any_cut |= cuts.m;
+        const int last = cuts.last_up_to(63);
+        const bool before = c > 0 || A.s_in;   // whether the state before the chunk may be other than zero
+        bool again = false;
+        if constexpr (!LOCAL) {
+            float acc[NC / 8][4], p[C / 8][4];
+            const int r0 = row0 + g, r1 = r0 + 8;
+            const bool z0 = r0 >= last && r0 < cuts.n, z1 = r1 >= last && r1 < cuts.n;
+            const float w0 = pw[z0 ? cuts.n - 1 - r0 : 0], w1 = pw[z1 ? cuts.n - 1 - r1 : 0];
+            auto weigh = [&](bool in0, bool in1, float f0, float f1) {
+#pragma unroll
+                for (int i = 0; i < NC / 8; i++) {
+                    acc[i][0] = in0 ? acc[i][0] * f0 : 0.f; acc[i][1] = in0 ? acc[i][1] * f0 : 0.f;
+                    acc[i][2] = in1 ? acc[i][2] * f1 : 0.f; acc[i][3] = in1 ? acc[i][3] * f1 : 0.f;
+                }
+            };
+            zero(acc);
+            if (some) { product<T, NC / 8, D, true>(acc, tk, row0, tu, col0); weigh(z0, z1, w0, w1); }
+            scores<T, D, C, false>(p, tk, tq, row0, cuts, pw, A.scale);
+            apply_scores<T, D, C, NC / 8, false>(acc, p, tg, row0, col0);
+            again |= not_finite(acc);
+            store_rows<T, NC>(stage, acc, dv, A.dv.st, row0, col0, t0, cuts.n);
+            zero(acc);
+            if (some) { product<T, NC / 8, D, false>(acc, tv, row0, tu, col0); weigh(z0, z1, w0, w1); }
+            scores<T, D, C, false>(p, tv, tg, row0, cuts, pw, A.scale);
+            apply_scores<T, D, C, NC / 8, false>(acc, p, tq, row0, col0);
+            again |= not_finite(acc);
+            store_rows<T, NC>(stage, acc, dk, A.dk.st, row0, col0, t0, cuts.n);
+            zero(acc);
+            if (before) {
+                product<T, NC / 8, D, true>(acc, tg, row0, ts, col0);
+                weigh(cuts.last_up_to(r0) < 0, cuts.last_up_to(r1) < 0, pw[r0 + 1] * A.scale, pw[r1 + 1] * A.scale);
+            }
+            scores<T, D, C, true>(p, tg, tv, row0, cuts, pw, A.scale);
+            apply_scores<T, D, C, NC / 8, true>(acc, p, tk, row0, col0);
+            again |= not_finite(acc);
+            store_rows<T, NC>(stage, acc, dq, A.dq.st, row0, col0, t0, cuts.n);
+        }
+        const bool more = c > c0;
+        const int j = threadIdx.x;
+        if (j < C) a[j] = j < cuts.n && cuts.last_up_to(j) < 0 ? pw[j + 1] * A.scale : 0.f;
+        again = __syncthreads_or(again);
+        if (LOCAL || again || more || TWO) {
+            if (LOCAL) {
+                float add[D / 8][4];
+                zero(add);
+                outer<T, D, C, true>(add, tq, m0, a, tg);
+                again = __any_sync(0xffffffffu, not_finite(add));
+                if (!again) {
+                    keep_state<D>(u, cuts, pw);
+#pragma unroll
+                    for (int i = 0; i < D / 8; i++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) u[i][j] += add[i][j];
+                } else {
+                    walk<T, D, true>(u, tq, tg, tg, A.scale, 1.f, m0, cuts, pw[1], (T*)nullptr, 0, t0);
+                }
+            } else if (!again) {
+                keep_state<D>(u, cuts, pw);
+                outer<T, D, C, TWO>(u, tq, m0, a, tg);
+            } else {
+                float s[D / 8][4];
+                const int cc = l & 3;
+                // dq: forward from the state before the chunk (rows: features of k)
+#pragma unroll
+                for (int i = 0; i < D / 8; i++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) s[i][j] = before ? to_f(ts.at(8 * i + 2 * cc + (j & 1), m0 + g + 8 * (j >> 1))) : 0.f;
+                walk<T, D, false>(s, tk, tv, tg, 1.f, A.scale, m0, cuts, pw[1], dq, A.dq.st, t0);
+                // dv: backward, the transposed gradient (rows: features of v)
+#pragma unroll
+                for (int i = 0; i < D / 8; i++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) s[i][j] = some ? to_f(tu.at(8 * i + 2 * cc + (j & 1), m0 + g + 8 * (j >> 1))) : 0.f;
+                walk<T, D, true>(s, tg, tq, tk, A.scale, 1.f, m0, cuts, pw[1], dv, A.dv.st, t0);
+                // dk, and the gradient itself
+                walk<T, D, true>(u, tq, tg, tv, A.scale, 1.f, m0, cuts, pw[1], dk, A.dk.st, t0);
+            }
+        }
+        some = true;
+        __syncthreads();   // the tiles and the gradient have been read by all
+        if (more) fetch(c - 1);
+    }
+    if (LOCAL) {
+        move_part<D, NT, true>(u, W.parts, blockIdx.x);
+        if (threadIdx.x == 0) {
+            const int len = min(c1 * C, A.t) - c0 * C;
+            W.parts[(int64_t)gridDim.x * D * D + blockIdx.x] = any_cut ? -1.f : exp2f(g2 * (float)len);
+        }
+    } else if (TWO && rseg == W.segs - 1) {
+        move_state<D, false, true>(u, A.ds_in + pair * D * D, m0);
+    }
+}
+
+// The segments' parts joined: parts[s] becomes the state after segments 0..s. One thread for four values of one pair.
+__global__ void __launch_bounds__(256) k_attn_join(float* parts, int64_t pairs, int segs, int dd) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, per = dd / 4;
+    if (i >= pairs * per) return;
+    const int64_t pair = i / per;
+    float4* p = reinterpret_cast<float4*>(parts) + pair * segs * per + i % per;
+    const float* keep = parts + pairs * segs * dd + pair * segs;
+    float4 s = p[0];
+    for (int b = 1; b < segs; b += 8) {
+        float4 x[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            if (b + j < segs) x[j] = p[(b + j) * per];
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            if (b + j < segs) {
+                const float f = keep[b + j];   // negative: a restart
+                s = f < 0.f ? x[j] : make_float4(fmaf(s.x, f, x[j].x), fmaf(s.y, f, x[j].y), fmaf(s.z, f, x[j].z), fmaf(s.w, f, x[j].w));
+                p[(b + j) * per] = s;
+            }
+    }
+}
+
+// An empty sequence hands its state on.
+__global__ void k_attn_pass(const float* from, float* to, int64_t n) {
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) to[i] = from ? from[i] : 0.f;
+}
+
+// ---------------------------------------------------------------- one token
+// One CTA a (sequence, head): a thread holds D * D / 256 values of the state in pieces of four columns, all loaded before the
+// first is used. Bound by HBM: the state is read and written once, 8 D * D bytes, against 4 D values of q, k, v and o.
+constexpr int STEP_THREADS = 256;
+template <typename T, int D> __global__ void __launch_bounds__(STEP_THREADS) k_attn_step(const FmeDecayAttn A) {
+    constexpr int LANES = D / 4, R = STEP_THREADS / LANES, PER = D / R;
+    __shared__ float qk[2][D];
+    __shared__ float4 part[R][LANES];
+    const int64_t pair = blockIdx.x, n = pair / A.h, h = pair % A.h;
+    const int lane = threadIdx.x % LANES, r = threadIdx.x / LANES;
+    const bool cut = A.reset && A.reset[n * A.reset_sn];
+    const float4* in = reinterpret_cast<const float4*>(A.s_in + pair * D * D) + lane;
+    float4* out = reinterpret_cast<float4*>(A.s_out + pair * D * D) + lane;
+    float4 s[PER];
+#pragma unroll
+    for (int i = 0; i < PER; i++) s[i] = in[(i * R + r) * LANES];
+    if (threadIdx.x < 2 * D) qk[threadIdx.x / D][threadIdx.x % D] = to_f((threadIdx.x < D ? at<T>(A.q, n, h) : at<T>(A.k, n, h))[threadIdx.x % D]);
+    const T* vp = at<T>(A.v, n, h) + 4 * lane;
+    const float4 v = make_float4(to_f(vp[0]), to_f(vp[1]), to_f(vp[2]), to_f(vp[3]));
+    const float lam = expf(A.log_decay[h]);
+    __syncthreads();
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        const float q = qk[0][i * R + r], k = qk[1][i * R + r];
+        float4 x = s[i];
+        if (cut) x = make_float4(0.f, 0.f, 0.f, 0.f);   // not a product: what was there may not be a number
+        x = make_float4(fmaf(k, v.x, x.x * lam), fmaf(k, v.y, x.y * lam), fmaf(k, v.z, x.z * lam), fmaf(k, v.w, x.w * lam));
+        out[(i * R + r) * LANES] = x;
+        o = make_float4(fmaf(q, x.x, o.x), fmaf(q, x.y, o.y), fmaf(q, x.z, o.z), fmaf(q, x.w, o.w));
+    }
+    part[r][lane] = o;
+    __syncthreads();
+    if (threadIdx.x < D) {
+        const float* p = reinterpret_cast<const float*>(part) + threadIdx.x;
+        float t = 0.f;
+#pragma unroll
+        for (int i = 0; i < R; i++) t += p[i * D];
+        at<T>(A.o, n, h)[threadIdx.x] = from_f<T>(t * A.scale);
+    }
 }
 
 // ---------------------------------------------------------------- host side
+constexpr int FEW_PAIRS = 592;   // four CTAs for each of 148 SMs: with fewer sequences and heads, segments
+constexpr int SEG_CHUNKS = 4;    // chunks of a segment at least
+
 int bad(const char* msg) { return host_fail(FME_E_ARG, msg); }
 
 int check_sizes(const FmeDecayAttn* a) {
@@ -151,24 +652,87 @@ int check_common(const FmeDecayAttn* a) {
     return FME_OK;
 }
 
-template <typename T, int D> void launch_fwd(const FmeDecayAttn& a, cudaStream_t st) {
-    k_sweep<T, D, false><<<dim3(a.n * a.h, 1), SEQ_THREADS, 0, st>>>(a);
+template <typename T, int D> struct Plan {
+    using Z = Shape<T, D>;
+    Walkers W;
+    int64_t pairs;
+    explicit Plan(const FmeDecayAttn& a) {
+        pairs = (int64_t)a.n * a.h;
+        W.chunks = (a.t + Z::C - 1) / Z::C;
+        W.segs = 1;
+        W.per = W.chunks;
+        W.parts = (float*)a.ws;
+        if (pairs > 0 && pairs < FEW_PAIRS && W.chunks >= 2 * SEG_CHUNKS) {
+            int64_t want = (FEW_PAIRS + pairs - 1) / pairs;
+            if (want > W.chunks / SEG_CHUNKS) want = W.chunks / SEG_CHUNKS;
+            W.per = (int)((W.chunks + want - 1) / want);
+            W.segs = (W.chunks + W.per - 1) / W.per;
+        }
+    }
+    int64_t ws_bytes() const { return W.segs > 1 ? pairs * (W.segs - 1) * (4 * D * D + 4) : 0; }
+    int64_t saved_bytes() const { return W.chunks > 1 ? pairs * (W.chunks - 1) * D * D * (int64_t)sizeof(T) : 0; }
+    static constexpr int FLOAT_BYTES = Z::FLOATS * 4;
+    static constexpr int FWD = 3 * Z::TILE + Z::MAT + FLOAT_BYTES, BWD = 4 * Z::TILE + 2 * Z::MAT + Z::NW * Z::STAGE + FLOAT_BYTES, LOCAL = 2 * Z::TILE + FLOAT_BYTES;
+};
+// CTAs an SM that the registers are bounded for: what shared memory allows, and no more than keeps the accumulators in registers
+template <typename T, int D> constexpr int fwd_ctas() { return D == 128 ? 1 : sizeof(T) == 4 ? 3 : D == 64 ? 4 : 8; }
+template <typename T, int D> constexpr int bwd_ctas() { return D == 128 ? 1 : sizeof(T) == 4 ? 2 : D == 64 ? 3 : 6; }
+
+template <typename K> int go(const char* what, K kernel, int64_t grid, int threads, int smem, cudaStream_t st, const FmeDecayAttn& a, const Walkers& W) {
+    if (smem > 48 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    kernel<<<(unsigned)grid, threads, smem, st>>>(a, W);
+    return launch_status(what);
 }
-template <typename T, int D> void launch_bwd(const FmeDecayAttn& a, cudaStream_t st) {
-    k_sweep<T, D, true><<<dim3(a.n * a.h, 3), SEQ_THREADS, 0, st>>>(a);
+int join(const char* what, const Walkers& W, int64_t pairs, int dd, cudaStream_t st) {
+    if (W.segs == 2) return FME_OK;   // one part: nothing to add
+    k_attn_join<<<(unsigned)((pairs * (dd / 4) + 255) / 256), 256, 0, st>>>(W.parts, pairs, W.segs - 1, dd);
+    return launch_status(what);
 }
-#define FME_BY_TYPE(a, FN, st)                                                           \
-    do {                                                                                 \
-        if ((a).dtype == FME_F32) {                                                      \
-            if ((a).d == 32) FN<float, 32>(a, st);                                       \
-            else if ((a).d == 64) FN<float, 64>(a, st);                                  \
-            else FN<float, 128>(a, st);                                                  \
-        } else {                                                                         \
-            if ((a).d == 32) FN<__nv_bfloat16, 32>(a, st);                               \
-            else if ((a).d == 64) FN<__nv_bfloat16, 64>(a, st);                          \
-            else FN<__nv_bfloat16, 128>(a, st);                                          \
-        }                                                                                \
-    } while (0)
+bool has_ws(const FmeDecayAttn& a, int64_t need) { return need == 0 || (a.ws && !((uintptr_t)a.ws & 255) && a.ws_bytes >= need); }
+int pass_on(const char* what, const FmeDecayAttn& a, const float* from, float* to, cudaStream_t st) {
+    if (to && to != from) k_attn_pass<<<592, 256, 0, st>>>(from, to, (int64_t)a.n * a.h * a.d * a.d);
+    return launch_status(what);
+}
+
+template <typename T, int D> int launch_fwd(const FmeDecayAttn& a, cudaStream_t st) {
+    const char* what = "fme_decay_attn_fwd";
+    const Plan<T, D> P(a);
+    if (a.t == 0) return pass_on(what, a, a.s_in, a.s_out, st);
+    if (!has_ws(a, P.ws_bytes())) return bad("decay attention: workspace too small or not aligned");
+    if (P.pairs * P.W.segs > 0x7fffffff) return bad("decay attention: too many sequences");
+    constexpr int NT = Shape<T, D>::NT;
+    if (P.W.segs > 1) {
+        int rc = go(what, k_attn_fwd<T, D, true, 1>, P.pairs * (P.W.segs - 1), NT, Plan<T, D>::LOCAL, st, a, P.W);
+        if (rc || (rc = join(what, P.W, P.pairs, D * D, st))) return rc;
+    }
+    return go(what, k_attn_fwd<T, D, false, fwd_ctas<T, D>()>, P.pairs * P.W.segs, NT, Plan<T, D>::FWD, st, a, P.W);
+}
+template <typename T, int D> int launch_bwd(const FmeDecayAttn& a, cudaStream_t st) {
+    const char* what = "fme_decay_attn_bwd";
+    const Plan<T, D> P(a);
+    if (a.t == 0) return pass_on(what, a, a.ds_out, a.ds_in, st);
+    if (!has_ws(a, P.ws_bytes())) return bad("decay attention: workspace too small or not aligned");
+    if (P.saved_bytes() && !a.saved) return bad("decay attention: the backward pass needs what the forward pass saved");
+    if (P.pairs * P.W.segs > 0x7fffffff) return bad("decay attention: too many sequences");
+    constexpr int NT = Shape<T, D>::NT;
+    if (P.W.segs > 1) {
+        int rc = go(what, k_attn_bwd<T, D, true, true, 1>, P.pairs * (P.W.segs - 1), NT, Plan<T, D>::LOCAL, st, a, P.W);
+        if (rc || (rc = join(what, P.W, P.pairs, D * D, st))) return rc;
+    }
+    if (a.ds_in) return go(what, k_attn_bwd<T, D, false, true, bwd_ctas<T, D>()>, P.pairs * P.W.segs, NT, Plan<T, D>::BWD, st, a, P.W);
+    return go(what, k_attn_bwd<T, D, false, false, bwd_ctas<T, D>()>, P.pairs * P.W.segs, NT, Plan<T, D>::BWD, st, a, P.W);
+}
+template <typename T, int D> int launch_step(const FmeDecayAttn& a, cudaStream_t st) {
+    k_attn_step<T, D><<<a.n * a.h, STEP_THREADS, 0, st>>>(a);
+    return launch_status("fme_decay_attn_step");
+}
+template <typename T, int D> int64_t sizes(const FmeDecayAttn& a, int which) {
+    const Plan<T, D> P(a);
+    return which == 2 ? P.saved_bytes() : P.ws_bytes();
+}
+#define FME_BY_TYPE(a, FN, arg)                                                                                              \
+    ((a).dtype == FME_F32 ? ((a).d == 32 ? FN<float, 32>(a, arg) : (a).d == 64 ? FN<float, 64>(a, arg) : FN<float, 128>(a, arg)) \
+                          : ((a).d == 32 ? FN<bf16, 32>(a, arg) : (a).d == 64 ? FN<bf16, 64>(a, arg) : FN<bf16, 128>(a, arg)))
 
 }  // namespace
 }  // namespace fme
@@ -181,7 +745,7 @@ int64_t fme_decay_attn_bytes(const FmeDecayAttn* a, int32_t which) {
     const int rc = check_sizes(a);
     if (rc) return rc;
     if (which < 0 || which > 2) return bad("decay attention: which must be 0, 1 or 2");
-    return 0;
+    return FME_BY_TYPE(*a, sizes, which);
 }
 
 int fme_decay_attn_fwd(const FmeDecayAttn* a, void* stream) {
@@ -189,8 +753,7 @@ int fme_decay_attn_fwd(const FmeDecayAttn* a, void* stream) {
     if (rc) return rc;
     if (a->n == 0) return FME_OK;
     if (a->t && !rows_aligned(a->o, a->dtype)) return bad("decay attention: o must be given, with 16-byte aligned rows");
-    FME_BY_TYPE(*a, launch_fwd, (cudaStream_t)stream);
-    return launch_status("fme_decay_attn_fwd");
+    return FME_BY_TYPE(*a, launch_fwd, (cudaStream_t)stream);
 }
 
 int fme_decay_attn_bwd(const FmeDecayAttn* a, void* stream) {
@@ -200,8 +763,7 @@ int fme_decay_attn_bwd(const FmeDecayAttn* a, void* stream) {
     if (a->t && (!rows_aligned(a->d_o, a->dtype) || !rows_aligned(a->dq, a->dtype) || !rows_aligned(a->dk, a->dtype) ||
                  !rows_aligned(a->dv, a->dtype)))
         return bad("decay attention: the gradients must be given, with 16-byte aligned rows");
-    FME_BY_TYPE(*a, launch_bwd, (cudaStream_t)stream);
-    return launch_status("fme_decay_attn_bwd");
+    return FME_BY_TYPE(*a, launch_bwd, (cudaStream_t)stream);
 }
 
 int fme_decay_attn_step(const FmeDecayAttn* a, void* stream) {
@@ -211,8 +773,7 @@ int fme_decay_attn_step(const FmeDecayAttn* a, void* stream) {
     if (a->n == 0) return FME_OK;
     if (!a->s_in || !a->s_out) return bad("decay attention step: s_in and s_out are required");
     if (!rows_aligned(a->o, a->dtype)) return bad("decay attention: o must be given, with 16-byte aligned rows");
-    FME_BY_TYPE(*a, launch_fwd, (cudaStream_t)stream);
-    return launch_status("fme_decay_attn_step");
+    return FME_BY_TYPE(*a, launch_step, (cudaStream_t)stream);
 }
 
 }  // extern "C"

@@ -1,0 +1,210 @@
+// fme_mma.cuh - shared-memory tiles and matrix products of one warp, for bfloat16 and for float32.
+//
+// bfloat16: mma m16n8k16. float32: mma m16n8k8 in tf32 with every operand split in two tf32 numbers, x = hi + lo, and the
+// products hi hi + hi lo + lo hi: 22 bits of each operand count, the dropped lo lo is 2^-22 of a term. Accumulators are
+// float32, in the layout that both shapes share: acc[0..1] = (row g, columns 2c, 2c+1), acc[2..3] = (row g + 8, the same)
+// with g = lane / 4 and c = lane % 4.
+//
+// A tile is a row-major matrix of COLS values; its 16-byte pieces are permuted within 128 bytes by the row, so that
+// neither eight rows of one piece (ldmatrix) nor columns of rows 2c and 2c + 1 (transposed reads of float32) share a bank.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace fme {
+
+using bf16 = __nv_bfloat16;
+
+__device__ __forceinline__ float to_f(float x) { return x; }
+__device__ __forceinline__ float to_f(bf16 x) { return __bfloat162float(x); }
+template <typename T> __device__ __forceinline__ T from_f(float x);
+template <> __device__ __forceinline__ float from_f<float>(float x) { return x; }
+template <> __device__ __forceinline__ bf16 from_f<bf16>(float x) { return __float2bfloat16(x); }
+
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    __nv_bfloat162 p = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&p);
+}
+__device__ __forceinline__ float2 unpack2(uint32_t p) {
+    return make_float2(__uint_as_float(p << 16), __uint_as_float(p & 0xffff0000u));
+}
+
+template <typename T, int COLS> struct Tile {
+    static constexpr int ROW = COLS * (int)sizeof(T);   // bytes
+    static constexpr int PER = 16 / (int)sizeof(T);     // values of a 16-byte piece
+    uint32_t base;                                      // shared-space address
+    char* gen;                                          // generic address
+    __device__ __forceinline__ Tile(void* p) : base((uint32_t)__cvta_generic_to_shared(p)), gen((char*)p) {}
+    static __device__ __forceinline__ uint32_t off(int row, int col) {
+        const uint32_t piece = (uint32_t)col / PER, in = ((uint32_t)col % PER) * sizeof(T);
+        const uint32_t sw = ROW >= 128 ? (uint32_t)(row & 7) : (uint32_t)((row >> 1) & 3);
+        return (uint32_t)row * ROW + ((piece ^ sw) << 4) + in;
+    }
+    __device__ __forceinline__ uint32_t addr(int row, int col) const { return base + off(row, col); }
+    __device__ __forceinline__ T& at(int row, int col) const { return *reinterpret_cast<T*>(gen + off(row, col)); }
+    __device__ __forceinline__ float2 two(int row, int col) const {   // col even
+        if constexpr (sizeof(T) == 2) return unpack2(*reinterpret_cast<const uint32_t*>(gen + off(row, col)));
+        else return *reinterpret_cast<const float2*>(gen + off(row, col));
+    }
+    __device__ __forceinline__ void put2(int row, int col, float a, float b) const {
+        if constexpr (sizeof(T) == 2) *reinterpret_cast<uint32_t*>(gen + off(row, col)) = pack2(a, b);
+        else *reinterpret_cast<float2*>(gen + off(row, col)) = make_float2(a, b);
+    }
+};
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ uint32_t tf32(float x) {
+    uint32_t r;
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
+    hi = tf32(x);
+    lo = tf32(x - __uint_as_float(hi));
+}
+
+template <typename T> struct Frag;
+
+template <> struct Frag<bf16> {
+    static constexpr int KS = 16;
+    struct A { uint32_t r[4]; };
+    struct B { uint32_t r[2]; };
+    struct A2 { A hi, lo; };    // a scaled operand in two bfloat16 numbers: 16 bits of it count
+    static __device__ __forceinline__ void mma(float (&d)[4], const A& a, const B& b) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a.r[0]), "r"(a.r[1]), "r"(a.r[2]), "r"(a.r[3]), "r"(b.r[0]), "r"(b.r[1]));
+    }
+    // A[m][k] = tile[m][k]
+    template <int COLS> static __device__ __forceinline__ A ldA(const Tile<bf16, COLS>& s, int m, int k) {
+        const int l = threadIdx.x & 31;
+        A a;
+        ldsm4(a.r, s.addr(m + (l & 15), k + ((l >> 4) << 3)));
+        return a;
+    }
+    // B[k][n] = tile[n][k], 16 columns n
+    template <int COLS> static __device__ __forceinline__ void ldB(const Tile<bf16, COLS>& s, int n, int k, B& b0, B& b1) {
+        const int l = threadIdx.x & 31;
+        uint32_t r[4];
+        ldsm4(r, s.addr(n + (l & 7) + ((l >> 4) << 3), k + (l & 8)));
+        b0.r[0] = r[0]; b0.r[1] = r[1]; b1.r[0] = r[2]; b1.r[1] = r[3];
+    }
+    // B[k][n] = tile[k][n], 16 columns n
+    template <bool NAT, int COLS> static __device__ __forceinline__ void ldBt(const Tile<bf16, COLS>& s, int k, int n, B& b0, B& b1) {
+        const int l = threadIdx.x & 31;
+        uint32_t r[4];
+        ldsm4t(r, s.addr(k + (l & 15), n + ((l >> 4) << 3)));
+        b0.r[0] = r[0]; b0.r[1] = r[1]; b1.r[0] = r[2]; b1.r[1] = r[3];
+    }
+    // A[m][k] = weight[k] * tile[k][m], weights in shared memory
+    template <bool TWO, int COLS> static __device__ __forceinline__ A2 ldAt(const Tile<bf16, COLS>& s, int k, int m, const float* w) {
+        const int l = threadIdx.x & 31;
+        A2 a;
+        ldsm4t(a.hi.r, s.addr(k + (l & 7) + ((l >> 4) << 3), m + (l & 8)));
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int at = k + ((i >> 1) << 3) + 2 * (l & 3);
+            const float2 v = unpack2(a.hi.r[i]);
+            const float x = v.x * w[at], y = v.y * w[at + 1];
+            a.hi.r[i] = pack2(x, y);
+            if (TWO) {
+                const float2 h = unpack2(a.hi.r[i]);
+                a.lo.r[i] = pack2(x - h.x, y - h.y);
+            }
+        }
+        return a;
+    }
+    template <bool TWO> static __device__ __forceinline__ void mma2(float (&d)[4], const A2& a, const B& b) {
+        mma(d, a.hi, b);
+        if (TWO) mma(d, a.lo, b);
+    }
+    // The accumulators of 16 columns as an operand whose k runs over them
+    static __device__ __forceinline__ A chain(const float (*acc)[4], int ks) {
+        const float *u = acc[2 * ks], *v = acc[2 * ks + 1];
+        return A{{pack2(u[0], u[1]), pack2(u[2], u[3]), pack2(v[0], v[1]), pack2(v[2], v[3])}};
+    }
+};
+
+template <> struct Frag<float> {
+    static constexpr int KS = 8;
+    struct A { uint32_t hi[4], lo[4]; };
+    struct B { uint32_t hi[2], lo[2]; };
+    using A2 = A;
+    static __device__ __forceinline__ void one(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+        asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+    }
+    static __device__ __forceinline__ void mma(float (&d)[4], const A& a, const B& b) {
+        one(d, a.lo, b.hi);
+        one(d, a.hi, b.lo);
+        one(d, a.hi, b.hi);
+    }
+    template <int COLS> static __device__ __forceinline__ A ldA(const Tile<float, COLS>& s, int m, int k) {
+        const int l = threadIdx.x & 31;
+        uint32_t r[4];
+        ldsm4(r, s.addr(m + (l & 15), k + ((l >> 4) << 2)));
+        A a;
+#pragma unroll
+        for (int i = 0; i < 4; i++) split_tf32(__uint_as_float(r[i]), a.hi[i], a.lo[i]);
+        return a;
+    }
+    template <int COLS> static __device__ __forceinline__ void ldB(const Tile<float, COLS>& s, int n, int k, B& b0, B& b1) {
+        const int l = threadIdx.x & 31;
+        uint32_t r[4];
+        ldsm4(r, s.addr(n + (l & 7) + ((l >> 4) << 3), k + ((l & 8) >> 1)));
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            split_tf32(__uint_as_float(r[i]), b0.hi[i], b0.lo[i]);
+            split_tf32(__uint_as_float(r[2 + i]), b1.hi[i], b1.lo[i]);
+        }
+    }
+    // Which row of eight the two halves of a transposed operand take: rows c and c + 4 (NAT, to go with ldA), or rows 2c and
+    // 2c + 1, to go with chain() and ldAt(), without bank conflicts
+    template <bool NAT> static __device__ __forceinline__ int row_of(int i) {
+        const int c = threadIdx.x & 3;
+        return NAT ? c + 4 * i : 2 * c + i;
+    }
+    template <bool NAT, int COLS> static __device__ __forceinline__ void ldBt(const Tile<float, COLS>& s, int k, int n, B& b0, B& b1) {
+        const int g = (threadIdx.x & 31) >> 2;
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            split_tf32(s.at(k + row_of<NAT>(i), n + g), b0.hi[i], b0.lo[i]);
+            split_tf32(s.at(k + row_of<NAT>(i), n + 8 + g), b1.hi[i], b1.lo[i]);
+        }
+    }
+    template <bool TWO, int COLS> static __device__ __forceinline__ A2 ldAt(const Tile<float, COLS>& s, int k, int m, const float* w) {
+        const int g = (threadIdx.x & 31) >> 2;
+        A a;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int row = k + row_of<false>(i >> 1);
+            split_tf32(s.at(row, m + g + 8 * (i & 1)) * w[row], a.hi[i], a.lo[i]);
+        }
+        return a;
+    }
+    template <bool TWO> static __device__ __forceinline__ void mma2(float (&d)[4], const A2& a, const B& b) { mma(d, a, b); }
+    static __device__ __forceinline__ A chain(const float (*acc)[4], int ks) {
+        const float* u = acc[ks];
+        A a;
+        split_tf32(u[0], a.hi[0], a.lo[0]);
+        split_tf32(u[2], a.hi[1], a.lo[1]);
+        split_tf32(u[1], a.hi[2], a.lo[2]);
+        split_tf32(u[3], a.hi[3], a.lo[3]);
+        return a;
+    }
+};
+
+// 16 bytes from global to shared memory, zeros where !in
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool in) {
+    const int n = in ? 16 : 0;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+}  // namespace fme
