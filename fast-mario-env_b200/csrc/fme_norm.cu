@@ -31,76 +31,116 @@ __device__ __forceinline__ float act_bwd(int act, float z, float dy) {
     return act == FME_ACT_RELU ? (z <= 0.f ? 0.f : dy) : dy;
 }
 
-template <int V> struct cuda_int { static constexpr int value = V; };
 constexpr int NT = 256;
 constexpr int MAX_C = 4096;
 
 template <typename T, int VEC> struct alignas(sizeof(T) * VEC) Pack { T v[VEC]; };
 
-// ---------------------------------------------------------------- samples held in registers
-// A sample is p * c values in a row. Threads take vectors of VEC of them; R threads form a team and R * VEC is a multiple
-// of c, so that a thread meets the same channels in each of its K vectors and keeps their weights in registers. A team
-// holds R * K vectors. Small samples: M teams in a CTA, a sample each. Large ones: the CTAs of a cluster share a sample and
-// add up their sums through distributed shared memory. So x (and dy) are read once, which is the bound: HBM bytes.
-// Where no cluster can hold a sample (or so few samples would leave most SMs idle) its pieces are separate CTAs, and the
-// kernel runs twice, for the sums (STATS) and, after k_norm_join*, for the values (APPLY), with a second read of the inputs.
-// GR: all values of a vector belong to one group (VEC divides c / g).
+// ---------------------------------------------------------------- samples held in shared memory
+// A sample is p * c values in a row. Threads take vectors of VEC of them, R threads form a team and R * VEC is a multiple of
+// c, so that a thread meets the same channels in each of its vectors and keeps their weights (and, backward, their dw and db)
+// in registers. Each thread copies its own vectors to shared memory (asynchronously, without registers) and reads them from
+// there in every pass, so that x (and dy) come from HBM once, which is the bound: some 50 KB a CTA, four CTAs an SM, of which
+// some load while others compute. Small samples: M teams in a CTA, a sample each. Large ones: the CTAs of a cluster share a
+// sample and add up their sums through distributed shared memory. Where no cluster can hold a sample its pieces are separate
+// CTAs, and the kernel runs twice, for the sums (STATS) and, after k_norm_join*, for the values (APPLY), with a second read.
+// How a group's sums are found: EACH: a vector's values may belong to several groups (VEC does not divide c / g); ONE: to one
+// group; WARP: to one, and the c / VEC vectors of a pixel are a power of two up to 32, so that shuffles do most of it.
 enum Phase { WHOLE, STATS, APPLY };
+enum How { EACH, ONE, WARP };
+
+struct Div {   // x / d for x < 2^16, d <= 2^12
+    uint32_t d, m;
+    __device__ __forceinline__ int operator()(int x) const { return d == 1 ? x : (int)__umulhi((uint32_t)x, m); }
+    __device__ __forceinline__ int mod(int x) const { return x - (*this)(x) * (int)d; }
+};
 
 struct Plan {
-    int R, M, K, vec, parts;   // parts: CTAs that share a sample
-    bool gr, cluster;
-    int threads, grid;         // grid: CTAs
+    int R, M, vec, parts;      // parts: CTAs that share a sample
+    int chunk, nvec;           // vectors of a part at most, of a sample
+    int how;
+    bool cluster;
+    int L, gl, rows;           // what is summed over a group stands at row * L + g * gl + 0..gl-1
+    Div by_r, by_c, by_cg, by_gl, by_g;
+    int threads, grid;
+    int tile;                  // bytes of a team's vectors
     size_t smem;
 };
 
-template <int NS> struct Slots {   // where the values to be summed over a group stand in shared memory
-    int R, M, L, gl, rows, G, n;
-    __device__ Slots(const FmeGroupNorm& A, int R_, int M_, int vec)
-        : R(R_), M(M_), L(NS == 1 ? A.c / vec : A.c), gl(L / A.g), rows(R_ * NS / L), G(A.g), n(R_ * M_ * NS) {}
-};
-
-// Sum (or, for the second and third value with MM, minimum and maximum) of NV values of each (team, group), in a fixed order;
-// out[v * M * G + pair]. All threads of the CTA call it.
-template <int NV, int NS, bool MM>
-__device__ __forceinline__ void group_reduce(const Slots<NS>& S, const float (&v)[NV][NS], bool mine, float* red, float* out) {
-    if (mine) {
+// Sums (MM: the second and third value's minimum and maximum) over each (team, group), in a fixed order. red: room for NV *
+// threads * NS values, twice that for WARP, which alternates between halves (buf) and so needs one barrier. The result of the
+// thread's own group(s) in v; in out[i * pairs + pair] as well, for EACH and ONE, and for WARP from the team's first warp
+// (without a barrier after it).
+template <int NV, int NS, int HOW, bool MM>
+__device__ __forceinline__ void group_sums(const Plan& P, int G, float (&v)[NV][NS], const int (&grp)[NS], int team, int t, float* red, float* out, int buf) {
+    auto join = [](int i, float x, float y) { return !MM || i == 0 ? x + y : i == 1 ? fminf(x, y) : fmaxf(x, y); };
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, pairs = P.M * G;
+    if (HOW == WARP) {
+        for (int o = 16; o >= P.L; o >>= 1)
+#pragma unroll
+            for (int i = 0; i < NV; i++) v[i][0] = join(i, v[i][0], __shfl_xor_sync(0xffffffffu, v[i][0], o));
+        for (int o = P.gl >> 1; o > 0; o >>= 1)
+#pragma unroll
+            for (int i = 0; i < NV; i++) v[i][0] = join(i, v[i][0], __shfl_xor_sync(0xffffffffu, v[i][0], o));
+        const int warps = blockDim.x >> 5, g = P.by_gl(lane & (P.L - 1));
+        float* mine = red + buf * NV * warps * G;
+        if (lane < P.L && (lane & (P.gl - 1)) == 0) {
+#pragma unroll
+            for (int i = 0; i < NV; i++) mine[(i * warps + warp) * G + g] = v[i][0];
+        }
+        __syncthreads();
+        const int per = P.M == 1 ? warps : P.R >> 5, w0 = P.M == 1 ? 0 : team * per;   // M > 1: a team is whole warps
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const float* src = mine + (i * warps + min(w0, warps - per)) * G + g;
+            float x = src[0];
+            for (int w = 1; w < per; w++) x = join(i, x, src[w * G]);
+            v[i][0] = x;
+        }
+        if (t < P.L && (t & (P.gl - 1)) == 0 && team < P.M) {
+#pragma unroll
+            for (int i = 0; i < NV; i++) out[i * pairs + team * G + g] = v[i][0];
+        }
+        return;
+    }
+    const int n = P.R * P.M * NS, members = P.rows * P.gl;
+    __syncthreads();
+    if (team < P.M) {
 #pragma unroll
         for (int i = 0; i < NV; i++)
 #pragma unroll
-            for (int j = 0; j < NS; j++) red[i * S.n + threadIdx.x * NS + j] = v[i][j];
+            for (int j = 0; j < NS; j++) red[i * n + threadIdx.x * NS + j] = v[i][j];
     }
     __syncthreads();
-    const int lane = threadIdx.x & 31, members = S.rows * S.gl, pairs = S.M * S.G;
-    for (int pair = threadIdx.x >> 5; pair < pairs; pair += blockDim.x >> 5) {
-        const int base = (pair / S.G) * S.R * NS + (pair % S.G) * S.gl;
+    for (int pair = warp; pair < pairs; pair += blockDim.x >> 5) {
+        const int tm = P.by_g(pair), base = tm * P.R * NS + (pair - tm * G) * P.gl;
         float a[NV];
 #pragma unroll
         for (int i = 0; i < NV; i++) a[i] = !MM || i == 0 ? 0.f : i == 1 ? INFINITY : -INFINITY;
         for (int m = lane; m < members; m += 32) {
-            const int at = base + (m / S.gl) * S.L + m % S.gl;
+            const int row = P.by_gl(m), at = base + row * P.L + (m - row * P.gl);
 #pragma unroll
-            for (int i = 0; i < NV; i++) {
-                const float x = red[i * S.n + at];
-                a[i] = !MM || i == 0 ? a[i] + x : i == 1 ? fminf(a[i], x) : fmaxf(a[i], x);
-            }
+            for (int i = 0; i < NV; i++) a[i] = join(i, a[i], red[i * n + at]);
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1)
 #pragma unroll
-            for (int i = 0; i < NV; i++) {
-                const float x = __shfl_xor_sync(0xffffffffu, a[i], o);
-                a[i] = !MM || i == 0 ? a[i] + x : i == 1 ? fminf(a[i], x) : fmaxf(a[i], x);
-            }
+            for (int i = 0; i < NV; i++) a[i] = join(i, a[i], __shfl_xor_sync(0xffffffffu, a[i], o));
         if (lane == 0) {
 #pragma unroll
             for (int i = 0; i < NV; i++) out[i * pairs + pair] = a[i];
         }
     }
     __syncthreads();
+    if (team < P.M) {
+#pragma unroll
+        for (int i = 0; i < NV; i++)
+#pragma unroll
+            for (int j = 0; j < NS; j++) v[i][j] = out[i * pairs + team * G + grp[j]];
+    }
 }
 
-// mean and rstd from the parts' means and squared distances (count of values each)
+// mean and squared distances of several parts
 struct Moments {
     float n = 0.f, mean = 0.f, m2 = 0.f;
     __device__ __forceinline__ void add(float cnt, float mu, float q) {
@@ -116,160 +156,185 @@ __device__ __forceinline__ float rstd_of(float m2, float m, float eps) { return 
 __device__ __forceinline__ float code_inv(float lo, float hi) { return hi > lo ? __fmul_rn(__frcp_rn(__fsub_rn(hi, lo)), 255.f) : 0.f; }
 __device__ __forceinline__ float code_step(float lo, float hi) { return __fdiv_rn(__fsub_rn(hi, lo), 255.f); }
 
-template <typename T, int VEC, int K, bool GR, int PH>
-__global__ void __launch_bounds__(512) k_norm_fwd(const FmeGroupNorm A, const int R, const int M, const int parts) {
-    constexpr int NS = GR ? 1 : VEC;
-    extern __shared__ float sm[];
-    const Slots<NS> S(A, R, M, VEC);
-    const int pairs = M * A.g, team = threadIdx.x / R, t = threadIdx.x - team * R;
-    float* red = sm;                       // 3 * S.n, or 1 * S.n
-    float* out = sm + 3 * S.n;             // 3 * pairs: sum, lo, hi; then mean, rstd in the first two
-    float* out2 = out + 3 * pairs;         // pairs
-    float* part = out2 + pairs;            // 4 * pairs: what the cluster's other CTAs read
-    const int rank = blockIdx.x % parts;
-    const int64_t n = (int64_t)(blockIdx.x / parts) * M + team;
-    const bool mine = team < M, ok = mine && n < A.n;
-    const int nvec = (int)((int64_t)A.p * A.c / VEC), v0 = rank * R * K;
-    const int count = max(0, min(nvec - v0, R * K));
-    const float cnt = (float)((int64_t)count * VEC / A.g);   // of each group in this CTA: whole pixels
-    const T* x = (const T*)A.x + n * A.x_sn;
-    Pack<T, VEC> raw[K];
-#pragma unroll
-    for (int k = 0; k < K; k++)
-        if (ok && k * R + t < count) raw[k] = reinterpret_cast<const Pack<T, VEC>*>(x)[v0 + k * R + t];
-    const int c0 = (int)((int64_t)t * VEC % A.c), cgr = A.c / A.g;
-    int ch[VEC];                           // channel of each value of the vector
+// a thread's vector to its place in shared memory; BYTES 16, 8 or 4 asynchronously
+template <typename V> __device__ __forceinline__ void fetch(V* dst, const V* src) {
+    constexpr int B = sizeof(V);
+    if constexpr (B == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
+    else if constexpr (B == 8 || B == 4) asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src), "n"(B) : "memory");
+    else *dst = *src;
+}
+__device__ __forceinline__ void fetched() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+// values of each group in part r: parts begin and end with whole pixels
+__device__ __forceinline__ int part_vecs(const Plan& P, int r) { return max(0, min(P.nvec - r * P.chunk, P.chunk)); }
+
+template <int ACT> struct act_is { static constexpr int value = ACT; };
+template <typename F> __device__ __forceinline__ void by_act(int act, F f) {
+    if (act == FME_ACT_SILU) f(act_is<FME_ACT_SILU>{});
+    else if (act == FME_ACT_RELU) f(act_is<FME_ACT_RELU>{});
+    else f(act_is<FME_ACT_NONE>{});
+}
+
+constexpr int MAX_THREADS = 512;
+
+template <typename T, int VEC, int HOW, int PH>
+__global__ void __launch_bounds__(MAX_THREADS, 2) k_norm_fwd(const FmeGroupNorm A, const __grid_constant__ Plan P) {
+    constexpr int NS = HOW == EACH ? VEC : 1;
+    using V = Pack<T, VEC>;
+    extern __shared__ __align__(16) char sm[];
+    const int pairs = P.M * A.g, team = P.M == 1 ? (threadIdx.x < P.R ? 0 : 1) : P.by_r(threadIdx.x), t = threadIdx.x - team * P.R;
+    V* tile = reinterpret_cast<V*>(sm + team * P.tile);                // only for team < M
+    float* out = reinterpret_cast<float*>(sm + (size_t)P.M * P.tile);  // sum, lo, hi: 3 * pairs; squared distances: pairs
+    float* part = out + 4 * pairs;                                     // 4 * pairs
+    float* red = part + 4 * pairs;
+    const int rank = P.parts == 1 ? 0 : blockIdx.x % P.parts, block = P.parts == 1 ? blockIdx.x : blockIdx.x / P.parts;
+    const int64_t n = (int64_t)block * P.M + team;
+    const bool ok = team < P.M && n < A.n;
+    const int v0 = rank * P.chunk, count = ok ? part_vecs(P, rank) : 0;
+    const V* x = reinterpret_cast<const V*>((const T*)A.x + n * A.x_sn) + v0;
+    for (int i = t; i < count; i += P.R) fetch(tile + i, x + i);
+    int ch[VEC], grp[NS];
     float w[VEC], b[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; j++) {
-        ch[j] = c0 + j;
-        if (!GR) ch[j] %= A.c;
+        ch[j] = P.by_c.mod(t * VEC + j);
         w[j] = PH != STATS && A.w ? __ldg(A.w + ch[j]) : 1.f;
         b[j] = PH != STATS && A.b ? __ldg(A.b + ch[j]) : 0.f;
     }
-    int grp[NS];
 #pragma unroll
-    for (int j = 0; j < NS; j++) grp[j] = team * A.g + ch[j] / cgr;
+    for (int j = 0; j < NS; j++) grp[j] = P.by_cg(ch[j]);
     const bool u8 = A.codes != nullptr;
+    const float per_vec = (float)VEC / (float)A.g, cnt = (float)part_vecs(P, rank) * per_vec, m = (float)P.nvec * per_vec;
+    float mean[NS], rstd[NS], lo[NS], hi[NS];
+    fetched();
     if (PH != APPLY) {
-        float v[3][NS];
+        float v[3][NS], q[1][NS];
 #pragma unroll
-        for (int j = 0; j < NS; j++) { v[0][j] = 0.f; v[1][j] = INFINITY; v[2][j] = -INFINITY; }
-#pragma unroll
-        for (int k = 0; k < K; k++)
-            if (ok && k * R + t < count) {
+        for (int j = 0; j < NS; j++) { v[0][j] = 0.f; v[1][j] = INFINITY; v[2][j] = -INFINITY; q[0][j] = 0.f; }
+        if (u8) {
+#pragma unroll 4
+            for (int i = t; i < count; i += P.R) {
+                const V r = tile[i];
 #pragma unroll
                 for (int j = 0; j < VEC; j++) {
-                    const float f = to_f(raw[k].v[j]);
-                    const int s = GR ? 0 : j;
-                    v[0][s] += f;
-                    if (u8) { v[1][s] = fminf(v[1][s], f); v[2][s] = fmaxf(v[2][s], f); }
+                    const float f = to_f(r.v[j]);
+                    const int s = NS == 1 ? 0 : j;
+                    v[0][s] += f; v[1][s] = fminf(v[1][s], f); v[2][s] = fmaxf(v[2][s], f);
                 }
             }
-        if (u8) group_reduce<3, NS, true>(S, v, mine, red, out);
-        else { float s1[1][NS];
+            group_sums<3, NS, HOW, true>(P, A.g, v, grp, team, t, red, out, 0);
+        } else {
+            float s1[1][NS];
 #pragma unroll
-            for (int j = 0; j < NS; j++) s1[0][j] = v[0][j];
-            group_reduce<1, NS, false>(S, s1, mine, red, out); }
-        float mu[NS], q[1][NS];
+            for (int j = 0; j < NS; j++) s1[0][j] = 0.f;
+#pragma unroll 4
+            for (int i = t; i < count; i += P.R) {
+                const V r = tile[i];
 #pragma unroll
-        for (int j = 0; j < NS; j++) { mu[j] = mine && cnt > 0.f ? out[grp[j]] / cnt : 0.f; q[0][j] = 0.f; }
-#pragma unroll
-        for (int k = 0; k < K; k++)
-            if (ok && k * R + t < count) {
-#pragma unroll
-                for (int j = 0; j < VEC; j++) { const int s = GR ? 0 : j; const float d = to_f(raw[k].v[j]) - mu[s]; q[0][s] = fmaf(d, d, q[0][s]); }
+                for (int j = 0; j < VEC; j++) s1[0][NS == 1 ? 0 : j] += to_f(r.v[j]);
             }
-        group_reduce<1, NS, false>(S, q, mine, red, out2);
+            group_sums<1, NS, HOW, false>(P, A.g, s1, grp, team, t, red, out, 0);
+#pragma unroll
+            for (int j = 0; j < NS; j++) v[0][j] = s1[0][j];
+        }
+#pragma unroll
+        for (int j = 0; j < NS; j++) { mean[j] = cnt > 0.f ? v[0][j] / cnt : 0.f; lo[j] = v[1][j]; hi[j] = v[2][j]; }
+#pragma unroll 4
+        for (int i = t; i < count; i += P.R) {
+            const V r = tile[i];
+#pragma unroll
+            for (int j = 0; j < VEC; j++) { const int s = NS == 1 ? 0 : j; const float d = to_f(r.v[j]) - mean[s]; q[0][s] = fmaf(d, d, q[0][s]); }
+        }
+        // 3 * warps * g floats on: past what the first sums used
+        group_sums<1, NS, HOW, false>(P, A.g, q, grp, team, t, HOW == WARP ? red + 3 * (blockDim.x >> 5) * A.g : red, out + 3 * pairs, 0);
+#pragma unroll
+        for (int j = 0; j < NS; j++) rstd[j] = rstd_of(q[0][j], m, A.eps);
+        if (PH == STATS || P.parts > 1) __syncthreads();   // out, for other threads
     }
-    const float m = (float)((int64_t)A.p * cgr);
-    if (PH == STATS) {                     // (sample, part, group): mean, squared distances, lo, hi
+    if (PH == STATS) {                     // (sample, part, group): mean, squared distances, lo, hi; M is 1
         for (int i = threadIdx.x; i < pairs; i += blockDim.x) {
-            float4* dst = reinterpret_cast<float4*>(A.ws) + ((blockIdx.x / parts) * (int64_t)parts + rank) * A.g + i;   // M is 1 here
-            *dst = make_float4(cnt > 0.f ? out[i] / cnt : 0.f, out2[i], u8 ? out[pairs + i] : 0.f, u8 ? out[2 * pairs + i] : 0.f);
+            float4* dst = reinterpret_cast<float4*>(A.ws) + ((int64_t)block * P.parts + rank) * A.g + i;
+            *dst = make_float4(cnt > 0.f ? out[i] / cnt : 0.f, out[3 * pairs + i], u8 ? out[pairs + i] : 0.f, u8 ? out[2 * pairs + i] : 0.f);
         }
         return;
     }
-    if (PH == WHOLE) {
-        if (parts == 1) {
-            for (int i = threadIdx.x; i < pairs; i += blockDim.x) { out[i] = out[i] / m; out2[i] = rstd_of(out2[i], m, A.eps); }
-        } else {
-            cg::cluster_group cl = cg::this_cluster();
-            for (int i = threadIdx.x; i < pairs; i += blockDim.x) {
-                part[i] = cnt > 0.f ? out[i] / cnt : 0.f; part[pairs + i] = out2[i];
-                if (u8) { part[2 * pairs + i] = out[pairs + i]; part[3 * pairs + i] = out[2 * pairs + i]; }
-            }
-            cl.sync();
-            for (int i = threadIdx.x; i < pairs; i += blockDim.x) {
-                Moments mo;
-                float lo = INFINITY, hi = -INFINITY;
-                for (int r = 0; r < parts; r++) {
-                    const float* o = cl.map_shared_rank(part, r);
-                    const int rc = max(0, min(nvec - r * R * K, R * K));
-                    mo.add((float)((int64_t)rc * VEC / A.g), o[i], o[pairs + i]);
-                    if (u8) { lo = fminf(lo, o[2 * pairs + i]); hi = fmaxf(hi, o[3 * pairs + i]); }
-                }
-                out[i] = mo.mean; out2[i] = rstd_of(mo.m2, m, A.eps);
-                if (u8) { out[pairs + i] = lo; out[2 * pairs + i] = hi; }
-            }
-            cg::this_cluster().barrier_arrive();   // this CTA has read the others; it ends only when they have read it
-        }
-    } else {
+    if (PH == WHOLE && P.parts > 1) {
+        cg::cluster_group cl = cg::this_cluster();
         for (int i = threadIdx.x; i < pairs; i += blockDim.x) {
-            const float4 f = reinterpret_cast<const float4*>(A.ws)[(int64_t)A.n * parts * A.g + (blockIdx.x / parts) * (int64_t)A.g + i];
-            out[i] = f.x; out2[i] = f.y;
-            if (u8) { out[pairs + i] = f.z; out[2 * pairs + i] = f.w; }
+            part[i] = cnt > 0.f ? out[i] / cnt : 0.f; part[pairs + i] = out[3 * pairs + i];
+            if (u8) { part[2 * pairs + i] = out[pairs + i]; part[3 * pairs + i] = out[2 * pairs + i]; }
         }
+        cl.sync();
+        for (int i = threadIdx.x; i < pairs; i += blockDim.x) {
+            Moments mo;
+            float l = INFINITY, h = -INFINITY;
+            for (int r = 0; r < P.parts; r++) {
+                const float* o = cl.map_shared_rank(part, r);
+                mo.add((float)part_vecs(P, r) * per_vec, o[i], o[pairs + i]);
+                if (u8) { l = fminf(l, o[2 * pairs + i]); h = fmaxf(h, o[3 * pairs + i]); }
+            }
+            out[i] = mo.mean; out[3 * pairs + i] = rstd_of(mo.m2, m, A.eps);
+            out[pairs + i] = l; out[2 * pairs + i] = h;
+        }
+        cl.barrier_arrive();   // this CTA has read the others; it ends only when they have read it
+        __syncthreads();
     }
-    __syncthreads();
-    if (rank == 0) {
+    if (PH == APPLY) {
         for (int i = threadIdx.x; i < pairs; i += blockDim.x) {
-            const int64_t ng = (int64_t)(blockIdx.x / parts) * pairs + i;
-            if (ng < (int64_t)A.n * A.g) {
-                if (A.mean) { A.mean[ng] = out[i]; A.rstd[ng] = out2[i]; }
-                if (u8) { A.lo[ng] = out[pairs + i]; A.hi[ng] = out[2 * pairs + i]; }
-            }
+            const float4 f = reinterpret_cast<const float4*>(A.ws)[(int64_t)A.n * P.parts * A.g + (int64_t)block * A.g + i];
+            out[i] = f.x; out[3 * pairs + i] = f.y; out[pairs + i] = f.z; out[2 * pairs + i] = f.w;
         }
+        __syncthreads();
     }
     if (ok) {
-        float mean[NS], rstd[NS], lo[NS], inv[NS];
+        if (PH == APPLY || P.parts > 1) {
 #pragma unroll
-        for (int j = 0; j < NS; j++) {
-            mean[j] = out[grp[j]]; rstd[j] = out2[grp[j]];
-            if (u8) { lo[j] = out[pairs + grp[j]]; inv[j] = code_inv(lo[j], out[2 * pairs + grp[j]]); }
+            for (int j = 0; j < NS; j++) { mean[j] = out[grp[j]]; rstd[j] = out[3 * pairs + grp[j]]; lo[j] = out[pairs + grp[j]]; hi[j] = out[2 * pairs + grp[j]]; }
         }
-        const int64_t base = n * nvec + v0;
-        auto apply = [&](auto act) {
+        if (rank == 0 && A.mean && t < P.L * (NS == 1 ? 1 : A.g)) {   // a group's first thread; EACH: every value of the first pixels
 #pragma unroll
-            for (int k = 0; k < K; k++)
-                if (k * R + t < count) {
-                    Pack<T, VEC> y;
-#pragma unroll
-                    for (int j = 0; j < VEC; j++) {
-                        const int s = GR ? 0 : j;
-                        y.v[j] = from_f<T>(act_fwd(decltype(act)::value, fmaf((to_f(raw[k].v[j]) - mean[s]) * rstd[s], w[j], b[j])));
-                    }
-                    reinterpret_cast<Pack<T, VEC>*>(A.y)[base + k * R + t] = y;
+            for (int j = 0; j < NS; j++) {
+                const int64_t ng = n * A.g + grp[j];
+                const bool first = NS == 1 ? t == grp[j] * P.gl : t * VEC + j == grp[j] * P.gl;
+                if (first) {
+                    A.mean[ng] = mean[j]; A.rstd[ng] = rstd[j];
+                    if (u8) { A.lo[ng] = lo[j]; A.hi[ng] = hi[j]; }
                 }
-        };
+            }
+        }
+        V* y = reinterpret_cast<V*>(A.y) + n * P.nvec + v0;
+        by_act(A.act, [&](auto act) {
+#pragma unroll 4
+            for (int i = t; i < count; i += P.R) {
+                const V r = tile[i];
+                V o;
+#pragma unroll
+                for (int j = 0; j < VEC; j++) {
+                    const int s = NS == 1 ? 0 : j;
+                    o.v[j] = from_f<T>(act_fwd(decltype(act)::value, fmaf((to_f(r.v[j]) - mean[s]) * rstd[s], w[j], b[j])));
+                }
+                y[i] = o;
+            }
+        });
         if (u8) {
+            float inv[NS];
 #pragma unroll
-            for (int k = 0; k < K; k++)
-                if (k * R + t < count) {
-                    Pack<uint8_t, VEC> q;
+            for (int j = 0; j < NS; j++) inv[j] = code_inv(lo[j], hi[j]);
+            Pack<uint8_t, VEC>* codes = reinterpret_cast<Pack<uint8_t, VEC>*>(A.codes) + n * P.nvec + v0;
+#pragma unroll 4
+            for (int i = t; i < count; i += P.R) {
+                const V r = tile[i];
+                Pack<uint8_t, VEC> o;
 #pragma unroll
-                    for (int j = 0; j < VEC; j++) {
-                        const int s = GR ? 0 : j;   // in 0..255 by construction; a group with NaN gets some code
-                        q.v[j] = (uint8_t)__float2uint_rn(__fmul_rn(__fsub_rn(to_f(raw[k].v[j]), lo[s]), inv[s]));
-                    }
-                    reinterpret_cast<Pack<uint8_t, VEC>*>(A.codes)[base + k * R + t] = q;
+                for (int j = 0; j < VEC; j++) {
+                    const int s = NS == 1 ? 0 : j;   // in 0..255 by construction; a group with NaN gets some code
+                    o.v[j] = (uint8_t)__float2uint_rn(__fmul_rn(__fsub_rn(to_f(r.v[j]), lo[s]), inv[s]));
                 }
+                codes[i] = o;
+            }
         }
-        if (A.act == FME_ACT_SILU) apply(cuda_int<FME_ACT_SILU>{});
-        else if (A.act == FME_ACT_RELU) apply(cuda_int<FME_ACT_RELU>{});
-        else apply(cuda_int<FME_ACT_NONE>{});
     }
-    if (PH == WHOLE && parts > 1) cg::this_cluster().barrier_wait();
+    if (PH == WHOLE && P.parts > 1) cg::this_cluster().barrier_wait();
 }
 
 // One warp a (sample, group): its parts' moments in order, to the end of the workspace.
@@ -300,49 +365,45 @@ template <typename T, int VEC> __global__ void __launch_bounds__(NT) k_norm_join
 
 // x^ = (x - mean) rstd, z = w x^ + b, dz = dy act'(z); dw = sum dz x^, db = sum dz;
 // dx = rstd (w dz - mean(w dz) - x^ mean(w dz x^)), the means over the (sample, group).
-// A CTA (or cluster) walks samples and keeps its channels' dw and db in registers until the end.
-template <typename T, int VEC, int K, bool GR, int PH, bool U8>
-__global__ void __launch_bounds__(512) k_norm_bwd(const FmeGroupNorm A, const int R, const int M, const int parts) {
-    constexpr int NS = GR ? 1 : VEC;
-    extern __shared__ float sm[];
-    const Slots<NS> S(A, R, M, VEC);
-    const int pairs = M * A.g, team = threadIdx.x / R, t = threadIdx.x - team * R;
-    float* red = sm;                       // 2 * S.n (at the end 2 * threads * VEC)
-    float* out = sm + 2 * R * M * VEC;     // 2 * pairs
-    float* part = out + 2 * pairs;         // 2 * pairs
-    const int rank = blockIdx.x % parts, nvec = (int)((int64_t)A.p * A.c / VEC), v0 = rank * R * K;
-    const int count = max(0, min(nvec - v0, R * K));
-    const int c0 = (int)((int64_t)t * VEC % A.c), cgr = A.c / A.g;
-    const float m = (float)((int64_t)A.p * cgr);
-    const bool mine = team < M;
-    int ch[VEC];
+// A CTA (or cluster) walks samples and keeps its channels' dw and db in registers until the end. fp32 keeps dz in dy's place in
+// shared memory; bf16 would round it and computes it twice.
+template <typename T, int VEC, int HOW, int PH, bool U8>
+__global__ void __launch_bounds__(MAX_THREADS, 2) k_norm_bwd(const FmeGroupNorm A, const __grid_constant__ Plan P) {
+    constexpr int NS = HOW == EACH ? VEC : 1;
+    constexpr bool KEEP = sizeof(T) == 4 && PH != APPLY;
+    using V = Pack<T, VEC>;
+    using X = typename std::conditional<U8, Pack<uint8_t, VEC>, V>::type;
+    extern __shared__ __align__(16) char sm[];
+    const int pairs = P.M * A.g, team = P.M == 1 ? (threadIdx.x < P.R ? 0 : 1) : P.by_r(threadIdx.x), t = threadIdx.x - team * P.R;
+    V* td = reinterpret_cast<V*>(sm + team * P.tile);      // only for team < M
+    X* tx = reinterpret_cast<X*>(td + P.chunk);
+    float* out = reinterpret_cast<float*>(sm + (size_t)P.M * P.tile);   // 2 * pairs
+    float* part = out + 2 * pairs;                                       // 2 * pairs
+    float* red = part + 2 * pairs;
+    const int rank = P.parts == 1 ? 0 : blockIdx.x % P.parts, block = P.parts == 1 ? blockIdx.x : blockIdx.x / P.parts;
+    const int blocks = P.parts == 1 ? gridDim.x : gridDim.x / P.parts;
+    const int v0 = rank * P.chunk, mine = team < P.M ? part_vecs(P, rank) : 0;
+    const float inv_m = 1.f / ((float)P.nvec * ((float)VEC / (float)A.g));
+    int ch[VEC], grp[NS];
     float w[VEC], b[VEC], dw[VEC], db[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; j++) {
-        ch[j] = c0 + j;
-        if (!GR) ch[j] %= A.c;
+        ch[j] = P.by_c.mod(t * VEC + j);
         w[j] = A.w ? __ldg(A.w + ch[j]) : 1.f;
         b[j] = A.b ? __ldg(A.b + ch[j]) : 0.f;
         dw[j] = db[j] = 0.f;
     }
-    int grp[NS];
 #pragma unroll
-    for (int j = 0; j < NS; j++) grp[j] = ch[j] / cgr;
-    for (int64_t n0 = (int64_t)(blockIdx.x / parts) * M; n0 < A.n; n0 += (int64_t)(gridDim.x / parts) * M) {
+    for (int j = 0; j < NS; j++) grp[j] = P.by_cg(ch[j]);
+    int buf = 0;
+    for (int64_t n0 = (int64_t)block * P.M; n0 < A.n; n0 += (int64_t)blocks * P.M) {
         const int64_t n = n0 + team;
-        const bool ok = mine && n < A.n;
-        Pack<T, VEC> rx[U8 ? 1 : K], rd[K];
-        Pack<uint8_t, VEC> rc[U8 ? K : 1];
-        const T* dy = (const T*)A.dy + n * A.dy_sn;
-#pragma unroll
-        for (int k = 0; k < K; k++)
-            if (ok && k * R + t < count) {
-                const int i = v0 + k * R + t;
-                if (U8) rc[k] = reinterpret_cast<const Pack<uint8_t, VEC>*>(A.codes)[n * nvec + i];
-                else rx[k] = reinterpret_cast<const Pack<T, VEC>*>((const T*)A.x + n * A.x_sn)[i];
-                rd[k] = reinterpret_cast<const Pack<T, VEC>*>(dy)[i];
-            }
-        // x^ = x * xa + xb (of codes: code * xa + xb)
+        const bool ok = team < P.M && n < A.n;
+        const int count = ok ? mine : 0;
+        const V* dy = reinterpret_cast<const V*>((const T*)A.dy + n * A.dy_sn) + v0;
+        const X* x = U8 ? reinterpret_cast<const X*>(A.codes) + n * P.nvec + v0 : reinterpret_cast<const X*>((const T*)A.x + n * A.x_sn) + v0;
+        for (int i = t; i < count; i += P.R) { fetch(tx + i, x + i); fetch(td + i, dy + i); }
+        // x^ = (x - xb) xa; of codes: code * xa + xb
         float xa[NS], xb[NS], rstd[NS];
 #pragma unroll
         for (int j = 0; j < NS; j++) {
@@ -354,94 +415,331 @@ __global__ void __launch_bounds__(512) k_norm_bwd(const FmeGroupNorm A, const in
                 xa[j] = code_step(lo, hi) * rstd[j]; xb[j] = (lo - mean) * rstd[j];
             } else { xa[j] = rstd[j]; xb[j] = mean; }
         }
-        auto hat = [&](int k, int j) {
-            const int s = GR ? 0 : j;
-            return U8 ? fmaf((float)rc[U8 ? k : 0].v[j], xa[s], xb[s]) : (to_f(rx[U8 ? 0 : k].v[j]) - xb[s]) * xa[s];
+        auto hat = [&](const X& r, int j) {
+            const int s = NS == 1 ? 0 : j;
+            if constexpr (U8) return fmaf((float)r.v[j], xa[s], xb[s]);
+            else return (to_f(r.v[j]) - xb[s]) * xa[s];
         };
-        auto value = [&](auto act) {
-            if (PH != APPLY) {
-                float v[2][NS];
+        fetched();
+        float v[2][NS];
+        if (PH != APPLY) {
 #pragma unroll
-                for (int j = 0; j < NS; j++) v[0][j] = v[1][j] = 0.f;
+            for (int j = 0; j < NS; j++) v[0][j] = v[1][j] = 0.f;
+            by_act(A.act, [&](auto act) {
+#pragma unroll 2
+                for (int i = t; i < count; i += P.R) {
+                    const X r = tx[i];
+                    V g = td[i];
 #pragma unroll
-                for (int k = 0; k < K; k++)
-                    if (ok && k * R + t < count) {
-#pragma unroll
-                        for (int j = 0; j < VEC; j++) {
-                            const int s = GR ? 0 : j;
-                            const float xh = hat(k, j), dz = act_bwd(decltype(act)::value, fmaf(xh, w[j], b[j]), to_f(rd[k].v[j]));
-                            if (sizeof(T) == 4) rd[k].v[j] = from_f<T>(dz);   // fp32 keeps dz; bf16 would round it
-                            const float wd = w[j] * dz;
-                            v[0][s] += wd; v[1][s] = fmaf(wd, xh, v[1][s]);
-                            db[j] += dz; dw[j] = fmaf(dz, xh, dw[j]);
-                        }
+                    for (int j = 0; j < VEC; j++) {
+                        const int s = NS == 1 ? 0 : j;
+                        const float xh = hat(r, j), dz = act_bwd(decltype(act)::value, fmaf(xh, w[j], b[j]), to_f(g.v[j]));
+                        if (KEEP) g.v[j] = from_f<T>(dz);
+                        const float wd = w[j] * dz;
+                        v[0][s] += wd; v[1][s] = fmaf(wd, xh, v[1][s]);
+                        db[j] += dz; dw[j] = fmaf(dz, xh, dw[j]);
                     }
-                group_reduce<2, NS, false>(S, v, mine, red, out);
-            }
-            if (PH == STATS) {
-                for (int i = threadIdx.x; i < pairs; i += blockDim.x)
-                    reinterpret_cast<float2*>(A.ws)[(n0 * parts + rank) * A.g + i] = make_float2(out[i], out[pairs + i]);
-                return;
-            }
-            if (PH == WHOLE && parts > 1) {
-                cg::cluster_group cl = cg::this_cluster();
-                for (int i = threadIdx.x; i < 2 * pairs; i += blockDim.x) part[i] = out[i];
-                cl.sync();
-                for (int i = threadIdx.x; i < 2 * pairs; i += blockDim.x) {
-                    float s = 0.f;
-                    for (int r = 0; r < parts; r++) s += cl.map_shared_rank(part, r)[i];
-                    out[i] = s;
+                    if (KEEP && decltype(act)::value != FME_ACT_NONE) td[i] = g;
                 }
-                cl.barrier_arrive();
-                __syncthreads();
+            });
+            group_sums<2, NS, HOW, false>(P, A.g, v, grp, team, t, red, out, buf);
+            buf ^= 1;
+            if (PH == STATS || P.parts > 1) __syncthreads();
+        }
+        if (PH == STATS) {
+            for (int i = threadIdx.x; i < pairs; i += blockDim.x)
+                reinterpret_cast<float2*>(A.ws)[(n0 * P.parts + rank) * A.g + i] = make_float2(out[i], out[pairs + i]);
+            break;   // one sample a CTA
+        }
+        if (PH == WHOLE && P.parts > 1) {
+            cg::cluster_group cl = cg::this_cluster();
+            for (int i = threadIdx.x; i < 2 * pairs; i += blockDim.x) part[i] = out[i];
+            cl.sync();
+            for (int i = threadIdx.x; i < 2 * pairs; i += blockDim.x) {
+                float s = 0.f;
+                for (int r = 0; r < P.parts; r++) s += cl.map_shared_rank(part, r)[i];
+                out[i] = s;
             }
-            if (PH == APPLY) {
-                for (int i = threadIdx.x; i < pairs; i += blockDim.x) {
-                    const float2 f = reinterpret_cast<const float2*>(A.ws)[(int64_t)A.n * parts * A.g + n0 * A.g + i];
-                    out[i] = f.x; out[pairs + i] = f.y;
-                }
-                __syncthreads();
+            cl.barrier_arrive();
+            __syncthreads();
+        }
+        if (PH == APPLY) {
+            for (int i = threadIdx.x; i < pairs; i += blockDim.x) {
+                const float2 f = reinterpret_cast<const float2*>(A.ws)[(int64_t)A.n * P.parts * A.g + n0 * A.g + i];
+                out[i] = f.x; out[pairs + i] = f.y;
             }
-            if (ok) {
-                float a1[NS], a2[NS];
+            __syncthreads();
+        }
+        if (ok) {
+            float a1[NS], a2[NS];
 #pragma unroll
-                for (int j = 0; j < NS; j++) { a1[j] = out[team * A.g + grp[j]] / m; a2[j] = out[pairs + team * A.g + grp[j]] / m; }
+            for (int j = 0; j < NS; j++) {
+                a1[j] = inv_m * (PH == APPLY || P.parts > 1 ? out[team * A.g + grp[j]] : v[0][j]);
+                a2[j] = inv_m * (PH == APPLY || P.parts > 1 ? out[pairs + team * A.g + grp[j]] : v[1][j]);
+            }
+            V* dx = reinterpret_cast<V*>(A.dx) + n * P.nvec + v0;
+            by_act(A.act, [&](auto act) {
+#pragma unroll 2
+                for (int i = t; i < count; i += P.R) {
+                    const X r = tx[i];
+                    const V g = td[i];
+                    V o;
 #pragma unroll
-                for (int k = 0; k < K; k++)
-                    if (k * R + t < count) {
-                        Pack<T, VEC> dx;
-#pragma unroll
-                        for (int j = 0; j < VEC; j++) {
-                            const int s = GR ? 0 : j;
-                            const float xh = hat(k, j);
-                            const float dz = sizeof(T) == 4 && PH != APPLY ? to_f(rd[k].v[j])
-                                                                           : act_bwd(decltype(act)::value, fmaf(xh, w[j], b[j]), to_f(rd[k].v[j]));
-                            dx.v[j] = from_f<T>(rstd[s] * (fmaf(dz, w[j], -a1[s]) - xh * a2[s]));
-                        }
-                        reinterpret_cast<Pack<T, VEC>*>(A.dx)[n * nvec + v0 + k * R + t] = dx;
+                    for (int j = 0; j < VEC; j++) {
+                        const int s = NS == 1 ? 0 : j;
+                        const float xh = hat(r, j);
+                        const float dz = KEEP ? to_f(g.v[j]) : act_bwd(decltype(act)::value, fmaf(xh, w[j], b[j]), to_f(g.v[j]));
+                        o.v[j] = from_f<T>(rstd[s] * (fmaf(dz, w[j], -a1[s]) - xh * a2[s]));
                     }
-            }
-            if (PH == WHOLE && parts > 1) cg::this_cluster().barrier_wait();   // before part is written again
-        };
-        if (A.act == FME_ACT_SILU) value(cuda_int<FME_ACT_SILU>{});
-        else if (A.act == FME_ACT_RELU) value(cuda_int<FME_ACT_RELU>{});
-        else value(cuda_int<FME_ACT_NONE>{});
-        __syncthreads();   // out and red are written again
+                    dx[i] = o;
+                }
+            });
+        }
+        if (PH == WHOLE && P.parts > 1) cg::this_cluster().barrier_wait();   // before part is written again
+        if (PH == APPLY) break;
     }
     if (PH == APPLY || !A.dw) return;
     // dw and db of this CTA: slots c, c + C, ... hold channel c
-    float* rw = sm;
-    const int slots = R * M * VEC;
-    if (mine) {
+    __syncthreads();
+    float* rw = reinterpret_cast<float*>(sm);
+    const int slots = P.R * P.M * VEC;
+    if (team < P.M) {
 #pragma unroll
         for (int j = 0; j < VEC; j++) { rw[threadIdx.x * VEC + j] = dw[j]; rw[slots + threadIdx.x * VEC + j] = db[j]; }
     }
     __syncthreads();
-    float* row = (float*)A.ws + (PH == STATS ? 2 * ((int64_t)A.n * parts * A.g + (int64_t)A.n * A.g) : 0) + (int64_t)blockIdx.x * 2 * A.c;
+    float* row = (float*)A.ws + (PH == STATS ? 2 * ((int64_t)A.n * P.parts * A.g + (int64_t)A.n * A.g) : 0) + (int64_t)blockIdx.x * 2 * A.c;
     for (int i = threadIdx.x; i < 2 * A.c; i += blockDim.x) {
         const float* src = rw + (i < A.c ? i : slots + i - A.c);
         float s = 0.f;
         for (int k = 0; k < slots; k += A.c) s += src[k];
+        row[i] = s;
+    }
+}
+
+// ---------------------------------------------------------------- groups in a row
+// p = 1 (tokens, heads): a (sample, group) is c / g values in a row, KV vectors for each of LG lanes of a warp. No shared
+// memory and no barrier: shuffles. A lane keeps its channels over the samples that it walks, U of them loaded at a time.
+struct Rows {
+    int LG, segs, tall;   // lanes of a group; groups of a CTA at once; samples of a CTA at once (0: the groups take grid.y)
+    Div by_lg, by_g;
+    int cgv, grid, gy;
+    size_t smem;
+};
+constexpr int ROW_U = 4;
+
+template <int KV> struct RowSpot {
+    int lane, g, first, step;   // lane within the group, group, first sample, samples between
+    bool on;
+    __device__ RowSpot(const Rows& W, int G) {
+        const int seg = W.by_lg(threadIdx.x);
+        lane = threadIdx.x - seg * W.LG;
+        if (W.tall) {
+            const int k = W.by_g(seg);
+            g = seg - k * G;
+            on = k < W.tall;
+            first = blockIdx.x * W.tall + k;
+            step = gridDim.x * W.tall;
+        } else {
+            g = blockIdx.y * W.segs + seg;
+            on = g < G;
+            first = blockIdx.x;
+            step = gridDim.x;
+        }
+    }
+};
+__device__ __forceinline__ float lanes_sum(float x, int LG) {
+    for (int o = LG >> 1; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    return x;
+}
+
+template <typename T, int VEC, int KV>
+__global__ void __launch_bounds__(NT) k_norm_rows_fwd(const FmeGroupNorm A, const __grid_constant__ Rows W) {
+    using V = Pack<T, VEC>;
+    const RowSpot<KV> S(W, A.g);
+    const int cgr = W.cgv * VEC;
+    const bool u8 = A.codes != nullptr;
+    const float inv_m = 1.f / (float)cgr;
+    bool has[KV];
+    float w[KV][VEC], b[KV][VEC];
+#pragma unroll
+    for (int k = 0; k < KV; k++) {
+        has[k] = S.on && S.lane + k * W.LG < W.cgv;
+#pragma unroll
+        for (int j = 0; j < VEC; j++) {
+            const int c = S.g * cgr + (S.lane + k * W.LG) * VEC + j;
+            w[k][j] = has[k] && A.w ? __ldg(A.w + c) : 1.f;
+            b[k][j] = has[k] && A.b ? __ldg(A.b + c) : 0.f;
+        }
+    }
+    for (int64_t base = 0; base < A.n; base += (int64_t)ROW_U * S.step) {   // the same trips for all lanes: shuffles
+        V x[ROW_U][KV];
+#pragma unroll
+        for (int u = 0; u < ROW_U; u++) {
+            const int64_t n = base + (int64_t)u * S.step + S.first;
+#pragma unroll
+            for (int k = 0; k < KV; k++)
+                if (has[k] && n < A.n) x[u][k] = reinterpret_cast<const V*>((const T*)A.x + n * A.x_sn + S.g * cgr)[S.lane + k * W.LG];
+        }
+#pragma unroll
+        for (int u = 0; u < ROW_U; u++) {
+            const int64_t n = base + (int64_t)u * S.step + S.first;
+            const bool ok = n < A.n;
+            float s = 0.f, lo = INFINITY, hi = -INFINITY, q = 0.f;
+#pragma unroll
+            for (int k = 0; k < KV; k++)
+                if (has[k] && ok) {
+#pragma unroll
+                    for (int j = 0; j < VEC; j++) { const float f = to_f(x[u][k].v[j]); s += f; if (u8) { lo = fminf(lo, f); hi = fmaxf(hi, f); } }
+                }
+            s = lanes_sum(s, W.LG);
+            if (u8) for (int o = W.LG >> 1; o > 0; o >>= 1) { lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o)); hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o)); }
+            const float mean = s * inv_m;
+#pragma unroll
+            for (int k = 0; k < KV; k++)
+                if (has[k] && ok) {
+#pragma unroll
+                    for (int j = 0; j < VEC; j++) { const float d = to_f(x[u][k].v[j]) - mean; q = fmaf(d, d, q); }
+                }
+            q = lanes_sum(q, W.LG);
+            const float rstd = __frsqrt_rn(fmaf(q, inv_m, A.eps));
+            if (!ok || !S.on) continue;
+            if (A.mean && S.lane == 0) {
+                const int64_t ng = n * A.g + S.g;
+                A.mean[ng] = mean; A.rstd[ng] = rstd;
+                if (u8) { A.lo[ng] = lo; A.hi[ng] = hi; }
+            }
+            const float inv = u8 ? code_inv(lo, hi) : 0.f;
+            const int64_t at = (n * A.c + S.g * cgr) / VEC + S.lane;
+            by_act(A.act, [&](auto act) {
+#pragma unroll
+                for (int k = 0; k < KV; k++)
+                    if (has[k]) {
+                        V y;
+#pragma unroll
+                        for (int j = 0; j < VEC; j++) y.v[j] = from_f<T>(act_fwd(decltype(act)::value, fmaf((to_f(x[u][k].v[j]) - mean) * rstd, w[k][j], b[k][j])));
+                        reinterpret_cast<V*>(A.y)[at + k * W.LG] = y;
+                    }
+            });
+            if (u8) {
+#pragma unroll
+                for (int k = 0; k < KV; k++)
+                    if (has[k]) {
+                        Pack<uint8_t, VEC> y;
+#pragma unroll
+                        for (int j = 0; j < VEC; j++) y.v[j] = (uint8_t)__float2uint_rn(__fmul_rn(__fsub_rn(to_f(x[u][k].v[j]), lo), inv));
+                        reinterpret_cast<Pack<uint8_t, VEC>*>(A.codes)[at + k * W.LG] = y;
+                    }
+            }
+        }
+    }
+}
+
+template <typename T, int VEC, int KV, bool U8>
+__global__ void __launch_bounds__(NT) k_norm_rows_bwd(const FmeGroupNorm A, const __grid_constant__ Rows W) {
+    using V = Pack<T, VEC>;
+    using X = typename std::conditional<U8, Pack<uint8_t, VEC>, V>::type;
+    constexpr int U = KV == 1 ? ROW_U : KV == 2 ? 2 : 1;
+    extern __shared__ float rw[];
+    const RowSpot<KV> S(W, A.g);
+    const int cgr = W.cgv * VEC;
+    const float inv_m = 1.f / (float)cgr;
+    bool has[KV];
+    float w[KV][VEC], b[KV][VEC], dw[KV][VEC], db[KV][VEC];
+#pragma unroll
+    for (int k = 0; k < KV; k++) {
+        has[k] = S.on && S.lane + k * W.LG < W.cgv;
+#pragma unroll
+        for (int j = 0; j < VEC; j++) {
+            const int c = S.g * cgr + (S.lane + k * W.LG) * VEC + j;
+            w[k][j] = has[k] && A.w ? __ldg(A.w + c) : 1.f;
+            b[k][j] = has[k] && A.b ? __ldg(A.b + c) : 0.f;
+            dw[k][j] = db[k][j] = 0.f;
+        }
+    }
+    for (int64_t base = 0; base < A.n; base += (int64_t)U * S.step) {
+        V g[U][KV];
+        X x[U][KV];
+        float mean[U], rstd[U], lo[U], hi[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int64_t n = base + (int64_t)u * S.step + S.first, at = (n * A.c + S.g * cgr) / VEC + S.lane, ng = n * A.g + S.g;
+            const bool ok = S.on && n < A.n;
+#pragma unroll
+            for (int k = 0; k < KV; k++)
+                if (has[k] && ok) {
+                    if constexpr (U8) x[u][k] = reinterpret_cast<const X*>(A.codes)[at + k * W.LG];
+                    else x[u][k] = reinterpret_cast<const X*>((const T*)A.x + n * A.x_sn + S.g * cgr)[S.lane + k * W.LG];
+                    g[u][k] = reinterpret_cast<const V*>((const T*)A.dy + n * A.dy_sn + S.g * cgr)[S.lane + k * W.LG];
+                }
+            mean[u] = ok ? __ldg(A.mean + ng) : 0.f;
+            rstd[u] = ok ? __ldg(A.rstd + ng) : 0.f;
+            lo[u] = U8 && ok ? __ldg(A.lo + ng) : 0.f;
+            hi[u] = U8 && ok ? __ldg(A.hi + ng) : 0.f;
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int64_t n = base + (int64_t)u * S.step + S.first;
+            const bool ok = n < A.n;
+            const float step = U8 ? code_step(lo[u], hi[u]) : 0.f;
+            auto hat = [&](int k, int j) {
+                if constexpr (U8) return fmaf((float)x[u][k].v[j], step * rstd[u], (lo[u] - mean[u]) * rstd[u]);
+                else return (to_f(x[u][k].v[j]) - mean[u]) * rstd[u];
+            };
+            by_act(A.act, [&](auto act) {
+                float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+                for (int k = 0; k < KV; k++)
+                    if (has[k] && ok) {
+#pragma unroll
+                        for (int j = 0; j < VEC; j++) {
+                            const float xh = hat(k, j), dz = act_bwd(decltype(act)::value, fmaf(xh, w[k][j], b[k][j]), to_f(g[u][k].v[j]));
+                            if (sizeof(T) == 4) g[u][k].v[j] = from_f<T>(dz);
+                            const float wd = w[k][j] * dz;
+                            s1 += wd; s2 = fmaf(wd, xh, s2);
+                            db[k][j] += dz; dw[k][j] = fmaf(dz, xh, dw[k][j]);
+                        }
+                    }
+                const float a1 = lanes_sum(s1, W.LG) * inv_m, a2 = lanes_sum(s2, W.LG) * inv_m;
+                if (!ok) return;
+                const int64_t at = (n * A.c + S.g * cgr) / VEC + S.lane;
+#pragma unroll
+                for (int k = 0; k < KV; k++)
+                    if (has[k]) {
+                        V dx;
+#pragma unroll
+                        for (int j = 0; j < VEC; j++) {
+                            const float xh = hat(k, j);
+                            const float dz = sizeof(T) == 4 ? to_f(g[u][k].v[j]) : act_bwd(decltype(act)::value, fmaf(xh, w[k][j], b[k][j]), to_f(g[u][k].v[j]));
+                            dx.v[j] = from_f<T>(rstd[u] * (fmaf(dz, w[k][j], -a1) - xh * a2));
+                        }
+                        reinterpret_cast<V*>(A.dx)[at + k * W.LG] = dx;
+                    }
+            });
+        }
+    }
+    if (!A.dw) return;
+    // the CTA's row of dw and db: c of each, with zeros where another grid.y has the channels
+    float* row = (float*)A.ws + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 2 * A.c;
+    const int tall = W.tall ? W.tall : 1, k0 = W.tall ? (S.first - (int)blockIdx.x * W.tall) : 0;
+    const int cols = W.tall ? A.c : min(W.segs, A.g - (int)blockIdx.y * W.segs) * cgr, c0 = W.tall ? 0 : blockIdx.y * W.segs * cgr;
+    if (S.on) {
+#pragma unroll
+        for (int k = 0; k < KV; k++)
+            if (has[k]) {
+#pragma unroll
+                for (int j = 0; j < VEC; j++) {
+                    const int c = S.g * cgr + (S.lane + k * W.LG) * VEC + j - c0;
+                    rw[k0 * cols + c] = dw[k][j]; rw[(tall + k0) * cols + c] = db[k][j];
+                }
+            }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * A.c; i += NT) {
+        const int c = (i < A.c ? i : i - A.c) - c0;
+        float s = 0.f;
+        if (c >= 0 && c < cols)
+            for (int k = 0; k < tall; k++) s += rw[((i < A.c ? 0 : tall) + k) * cols + c];
         row[i] = s;
     }
 }
@@ -460,11 +758,11 @@ __global__ void __launch_bounds__(NT) k_norm_join_bwd(const FmeGroupNorm A, cons
 }
 
 // ---------------------------------------------------------------- many channels of an odd number
-// Channel counts whose vectors repeat only after more than MAX_R threads (odd ones above 512, mostly): one thread a channel,
+// Channel counts whose vectors repeat only after more than MAX_THREADS (odd ones above 512, mostly): one thread a channel,
 // x read three times. One CTA walks samples blockIdx.x, + gridDim.x, ...; per-channel sums in shared memory, one thread a channel.
 template <typename T> __global__ void __launch_bounds__(NT) k_norm_wide_fwd(const FmeGroupNorm A) {
-    extern __shared__ float sm[];
-    float *s0 = sm, *s1 = sm + A.c, *s2 = sm + 2 * A.c;
+    extern __shared__ float wide[];
+    float *s0 = wide, *s1 = wide + A.c, *s2 = wide + 2 * A.c;
     const int cg = A.c / A.g;
     const float m = (float)((int64_t)A.p * cg);
     for (int64_t n = blockIdx.x; n < A.n; n += gridDim.x) {
@@ -523,8 +821,8 @@ template <typename T> __device__ __forceinline__ float x_of(const FmeGroupNorm& 
 
 // As the forward kernel; a CTA's sums of dw and db over its samples go to its row of the workspace.
 template <typename T> __global__ void __launch_bounds__(NT) k_norm_wide_bwd(const FmeGroupNorm A) {
-    extern __shared__ float sm[];
-    float *s0 = sm, *s1 = sm + A.c, *tw = sm + 2 * A.c, *tb = sm + 3 * A.c;
+    extern __shared__ float wide[];
+    float *s0 = wide, *s1 = wide + A.c, *tw = wide + 2 * A.c, *tb = wide + 3 * A.c;
     const int cg = A.c / A.g;
     const float m = (float)((int64_t)A.p * cg);
     for (int c = threadIdx.x; c < A.c; c += NT) tw[c] = tb[c] = 0.f;
@@ -580,7 +878,7 @@ __global__ void __launch_bounds__(1024) k_norm_params(const float* __restrict__ 
 }
 
 // ---------------------------------------------------------------- host side
-constexpr int SMS = 148, MAX_R = 512;
+constexpr int SMS = 148;
 
 int bad(const char* msg) { return host_fail(FME_E_ARG, msg); }
 int check_sizes(const FmeGroupNorm* a) {
@@ -592,54 +890,105 @@ int check_sizes(const FmeGroupNorm* a) {
     if (a->act < FME_ACT_NONE || a->act > FME_ACT_SILU) return bad("group norm: unknown activation");
     return FME_OK;
 }
+bool split_parts(const Plan& P) { return P.parts > 1 && !P.cluster; }
 int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
+
+Div divisor(int d) { return Div{(uint32_t)d, d <= 1 ? 0u : (uint32_t)((0x100000000ull + d - 1) / d)}; }
+int pow2_up(int x) { int p = 1; while (p < x) p *= 2; return p; }
+
+int vec_of(const FmeGroupNorm& a, bool bwd) {
+    const int e = a.dtype == FME_F32 ? 4 : 2, full = 16 / e;
+    auto al = [&](const void* p, int64_t sn) { return !((uintptr_t)p & 15) && !((sn * e) & 15); };
+    const bool wide = (int64_t)a.p * a.c % full == 0 && !((uintptr_t)a.codes & 7) &&
+                      (bwd ? al(a.dy, a.dy_sn) && al(a.dx, 0) && (a.codes || al(a.x, a.x_sn)) : al(a.x, a.x_sn) && al(a.y, 0));
+    return wide ? full : 1;
+}
+
+// Groups in a row: one pixel, whole vectors in a group, at most 4 of them for each lane.
+bool make_rows(const FmeGroupNorm& a, bool bwd, Rows* W, int* kv) {
+    const int vec = vec_of(a, bwd), cgr = a.c / a.g;
+    if (a.p != 1 || vec == 1 || cgr % vec) return false;
+    W->cgv = cgr / vec;
+    if (W->cgv > 128) return false;
+    W->LG = W->cgv > 32 ? 32 : pow2_up(W->cgv);
+    *kv = W->cgv <= 32 ? 1 : W->cgv <= 64 ? 2 : 4;
+    W->segs = NT / W->LG;
+    W->tall = W->segs / a.g;
+    W->gy = W->tall ? 1 : (a.g + W->segs - 1) / W->segs;
+    W->by_lg = divisor(W->LG);
+    W->by_g = divisor(a.g);
+    const int at_once = W->tall ? W->tall : 1;
+    const int64_t need = ((int64_t)a.n + (int64_t)at_once * (bwd ? 1 : ROW_U) - 1) / ((int64_t)at_once * (bwd ? 1 : ROW_U)), most = SMS * 8 / W->gy + 1;
+    W->grid = (int)(need < most ? need : most);
+    if (W->grid < 1) W->grid = 1;
+    W->smem = bwd ? (size_t)8 * (W->tall ? W->tall * a.c : W->segs * cgr) : 0;
+    return true;
+}
 
 // How a call is laid out. false: the kernels for many channels of an odd number.
 bool make_plan(const FmeGroupNorm& a, bool bwd, Plan* P) {
-    const int e = a.dtype == FME_F32 ? 4 : 2, full = 16 / e;
-    const int64_t S = (int64_t)a.p * a.c;
-    auto al = [&](const void* p, int64_t sn) { return !((uintptr_t)p & 15) && !((sn * e) & 15); };
-    const bool wide = S % full == 0 && (bwd ? al(a.dy, a.dy_sn) && al(a.dx, 0) && (a.codes || al(a.x, a.x_sn)) : al(a.x, a.x_sn) && al(a.y, 0)) &&
-                      !((uintptr_t)a.codes & 7);
-    P->vec = wide ? full : 1;
-    P->gr = (a.c / a.g) % P->vec == 0;
-    const int per = a.c / gcd(a.c, P->vec);            // threads after which a vector's channels repeat
-    if (per > MAX_R) return false;
-    const int64_t nvec = S / P->vec;
-    auto up = [&](int64_t x) { return (int)((x + per - 1) / per * per); };
-    const int cap = MAX_R / per * per;                 // threads of a team at most
-    P->parts = 1;
-    P->cluster = false;
-    P->M = 1;
-    P->K = nvec <= 2 * (int64_t)cap ? 2 : nvec <= 4 * (int64_t)cap ? 4 : 8;
-    if (nvec > 4 * (int64_t)cap) {
-        int parts = 1;
-        while (parts < 16 && nvec > (int64_t)parts * cap * 4) parts *= 2;
-        P->K = nvec <= (int64_t)parts * cap * 4 ? 4 : 8;
-        const bool fits = nvec <= (int64_t)parts * cap * 8;
-        if (fits) { P->cluster = true; P->parts = parts; }
-        else P->parts = (int)((nvec + cap * 8 - 1) / (cap * 8));
+    const int e = a.dtype == FME_F32 ? 4 : 2;
+    const int vec = vec_of(a, bwd);
+    P->vec = vec;
+    const int per = a.c / gcd(a.c, vec);               // threads after which a vector's channels repeat
+    if (per > MAX_THREADS) return false;
+    const int64_t nvec = (int64_t)a.p * a.c / vec;
+    const int bpv = vec * (bwd ? e + (a.codes ? 1 : e) : e);
+    auto up = [](int64_t x, int64_t to) { return (x + to - 1) / to * to; };
+    // Parts of some 50 KB: four CTAs an SM. With few samples, more and smaller parts.
+    const int64_t most = 50 * 1024 / bpv, bound = 200 * 1024 / bpv;
+    int parts = 1;
+    while (parts < 16 && (nvec > parts * most || (a.n * (int64_t)parts < 2 * SMS && nvec >= parts * 2048))) parts *= 2;
+    int64_t chunk = up((nvec + parts - 1) / parts, per);
+    P->cluster = parts > 1;
+    if (chunk > bound) {
+        P->cluster = false;
+        parts = (int)((nvec + most - 1) / most);
+        chunk = up((nvec + parts - 1) / parts, per);
     }
-    P->R = up((nvec + (int64_t)P->parts * P->K - 1) / ((int64_t)P->parts * P->K));
-    if (P->R > cap) P->R = cap;
-    if (P->R < 1) P->R = per;
-    if (P->parts == 1 && P->R <= 128) {
+    P->parts = parts;
+    P->chunk = (int)(chunk < per ? per : chunk);
+    P->nvec = (int)nvec;
+    const bool gr = (a.c / a.g) % vec == 0, whole = a.c % vec == 0;
+    const int cv = whole ? a.c / vec : 0;
+    const bool pow2 = gr && cv <= 32 && (cv & (cv - 1)) == 0 && ((cv / a.g) & (cv / a.g - 1)) == 0;
+    P->how = !gr ? EACH : pow2 ? WARP : ONE;
+    // About eight vectors a thread when there is much to do, two when not: then a call's time is one CTA's
+    const bool busy = (int64_t)a.n * parts >= 4 * SMS;
+    int64_t r = (P->chunk + (busy ? 8 : 2) - 1) / (busy ? 8 : 2);
+    if (r < 32) r = P->chunk < 32 ? P->chunk : 32;
+    if (r > (busy ? 256 : 512)) r = busy ? 256 : 512;
+    P->R = (int)up(r, P->how == WARP ? 32 : per);
+    if (P->R > MAX_THREADS) P->R = MAX_THREADS / per * per;
+    P->M = 1;
+    P->tile = (int)up((int64_t)P->chunk * bpv, 16);
+    if (parts == 1 && P->R <= 128) {
         P->M = 256 / P->R;
+        while (P->M > 1 && (int64_t)P->M * P->tile > 50 * 1024) P->M--;
         if (P->M > a.n) P->M = a.n > 0 ? a.n : 1;
     }
     P->threads = (P->R * P->M + 31) / 32 * 32;
+    const int ns = P->how == EACH ? vec : 1, pairs = P->M * a.g, warps = P->threads / 32;
+    P->L = ns == 1 ? a.c / vec : a.c;
+    P->gl = P->L / a.g;
+    P->rows = P->R * ns / P->L;
+    P->by_r = divisor(P->R); P->by_c = divisor(a.c); P->by_cg = divisor(a.c / a.g); P->by_gl = divisor(P->gl); P->by_g = divisor(a.g);
     const int64_t groups = ((int64_t)a.n + P->M - 1) / P->M;
-    const int ns = P->gr ? 1 : P->vec, pairs = P->M * a.g;
+    const int nv = bwd ? 2 : 3;
+    const size_t red = P->how == WARP ? (size_t)(bwd ? 4 : 4) * warps * a.g : (size_t)nv * P->R * P->M * ns;
+    P->smem = (size_t)P->M * P->tile + 4 * ((bwd ? 4 : 8) * (size_t)pairs + red);
     if (bwd) {
-        P->smem = 4 * ((size_t)2 * P->R * P->M * P->vec + 4 * (size_t)pairs);
-        const bool walk = P->parts == 1 || P->cluster;
-        const int64_t most = walk ? (int64_t)SMS * (1536 / P->threads > 8 ? 8 : 1536 / P->threads) / P->parts : groups;
-        P->grid = (int)((groups < most ? groups : most) * P->parts);
+        const size_t end = (size_t)8 * P->R * P->M * vec;
+        if (P->smem < end) P->smem = end;
+        int64_t at_once = (int64_t)(220 * 1024 / (P->smem + 1024)), by_threads = 1024 / P->threads;
+        at_once = at_once < by_threads ? at_once : by_threads;
+        if (at_once < 1) at_once = 1;
+        const int64_t walk = SMS * at_once / parts;
+        P->grid = (int)((split_parts(*P) || groups < walk ? groups : walk) * parts);
     } else {
-        P->smem = 4 * ((size_t)3 * P->R * P->M * ns + 8 * (size_t)pairs);
-        P->grid = (int)(groups * P->parts);
+        P->grid = (int)(groups * parts);
     }
-    return groups * P->parts <= 0x7fffffff;
+    return groups * parts <= 0x7fffffff && P->smem <= 220 * 1024;
 }
 
 template <typename... Args>
@@ -658,37 +1007,56 @@ int launch(const char* what, void (*kernel)(Args...), const Plan& P, cudaStream_
     return launch_status(what);
 }
 
-template <typename T, int VEC, bool GR> int run_fwd(const FmeGroupNorm& a, const Plan& P, cudaStream_t st) {
+int join_grid(const FmeGroupNorm& a) { return (int)(((int64_t)a.n * a.g + NT / 32 - 1) / (NT / 32)); }
+
+template <typename T, int VEC, int HOW> int run_fwd(const FmeGroupNorm& a, const Plan& P, cudaStream_t st) {
     const char* what = "fme_group_norm_fwd";
-    if (P.parts == 1 || P.cluster) {
-        if (P.K == 2) return launch(what, k_norm_fwd<T, VEC, 2, GR, WHOLE>, P, st, a, P.R, P.M, P.parts);
-        if (P.K == 4) return launch(what, k_norm_fwd<T, VEC, 4, GR, WHOLE>, P, st, a, P.R, P.M, P.parts);
-        return launch(what, k_norm_fwd<T, VEC, 8, GR, WHOLE>, P, st, a, P.R, P.M, P.parts);
-    }
-    int rc = launch(what, k_norm_fwd<T, VEC, 8, GR, STATS>, P, st, a, P.R, P.M, P.parts);
+    if (!split_parts(P)) return launch(what, k_norm_fwd<T, VEC, HOW, WHOLE>, P, st, a, P);
+    int rc = launch(what, k_norm_fwd<T, VEC, HOW, STATS>, P, st, a, P);
     if (rc) return rc;
-    k_norm_join_fwd<T, VEC><<<(int)(((int64_t)a.n * a.g + NT / 32 - 1) / (NT / 32)), NT, 0, st>>>(a, P.parts, P.R * P.K);
+    k_norm_join_fwd<T, VEC><<<join_grid(a), NT, 0, st>>>(a, P.parts, P.chunk);
     if ((rc = launch_status(what))) return rc;
-    return launch(what, k_norm_fwd<T, VEC, 8, GR, APPLY>, P, st, a, P.R, P.M, P.parts);
+    return launch(what, k_norm_fwd<T, VEC, HOW, APPLY>, P, st, a, P);
 }
-template <typename T, int VEC, bool GR, bool U8> int run_bwd(const FmeGroupNorm& a, const Plan& P, cudaStream_t st) {
+template <typename T, int VEC, int HOW, bool U8> int run_bwd(const FmeGroupNorm& a, const Plan& P, cudaStream_t st) {
     const char* what = "fme_group_norm_bwd";
-    if (P.parts == 1 || P.cluster) {
-        if (P.K == 2) return launch(what, k_norm_bwd<T, VEC, 2, GR, WHOLE, U8>, P, st, a, P.R, P.M, P.parts);
-        if (P.K == 4) return launch(what, k_norm_bwd<T, VEC, 4, GR, WHOLE, U8>, P, st, a, P.R, P.M, P.parts);
-        return launch(what, k_norm_bwd<T, VEC, 8, GR, WHOLE, U8>, P, st, a, P.R, P.M, P.parts);
-    }
-    int rc = launch(what, k_norm_bwd<T, VEC, 8, GR, STATS, U8>, P, st, a, P.R, P.M, P.parts);
+    if (!split_parts(P)) return launch(what, k_norm_bwd<T, VEC, HOW, WHOLE, U8>, P, st, a, P);
+    int rc = launch(what, k_norm_bwd<T, VEC, HOW, STATS, U8>, P, st, a, P);
     if (rc) return rc;
-    k_norm_join_bwd<<<(int)(((int64_t)a.n * a.g + NT / 32 - 1) / (NT / 32)), NT, 0, st>>>(a, P.parts);
+    k_norm_join_bwd<<<join_grid(a), NT, 0, st>>>(a, P.parts);
     if ((rc = launch_status(what))) return rc;
-    return launch(what, k_norm_bwd<T, VEC, 8, GR, APPLY, U8>, P, st, a, P.R, P.M, P.parts);
+    return launch(what, k_norm_bwd<T, VEC, HOW, APPLY, U8>, P, st, a, P);
+}
+template <typename T, bool U8> int run_bwd(const FmeGroupNorm& a, const Plan& P, cudaStream_t st) {
+    constexpr int full = 16 / sizeof(T);
+    if (P.vec == 1) return P.how == WARP ? run_bwd<T, 1, WARP, U8>(a, P, st) : run_bwd<T, 1, ONE, U8>(a, P, st);
+    if (P.how == WARP) return run_bwd<T, full, WARP, U8>(a, P, st);
+    return P.how == ONE ? run_bwd<T, full, ONE, U8>(a, P, st) : run_bwd<T, full, EACH, U8>(a, P, st);
+}
+template <typename T> int run_fwd(const FmeGroupNorm& a, const Plan& P, cudaStream_t st) {
+    constexpr int full = 16 / sizeof(T);
+    if (P.vec == 1) return P.how == WARP ? run_fwd<T, 1, WARP>(a, P, st) : run_fwd<T, 1, ONE>(a, P, st);
+    if (P.how == WARP) return run_fwd<T, full, WARP>(a, P, st);
+    return P.how == ONE ? run_fwd<T, full, ONE>(a, P, st) : run_fwd<T, full, EACH>(a, P, st);
+}
+
+template <typename T> int run_rows_fwd(const FmeGroupNorm& a, const Rows& W, int kv, cudaStream_t st) {
+    constexpr int full = 16 / sizeof(T);
+    auto kernel = kv == 1 ? k_norm_rows_fwd<T, full, 1> : kv == 2 ? k_norm_rows_fwd<T, full, 2> : k_norm_rows_fwd<T, full, 4>;
+    kernel<<<dim3(W.grid, W.gy), NT, 0, st>>>(a, W);
+    return launch_status("fme_group_norm_fwd");
+}
+template <typename T, bool U8> int run_rows_bwd(const FmeGroupNorm& a, const Rows& W, int kv, cudaStream_t st) {
+    constexpr int full = 16 / sizeof(T);
+    auto kernel = kv == 1 ? k_norm_rows_bwd<T, full, 1, U8> : kv == 2 ? k_norm_rows_bwd<T, full, 2, U8> : k_norm_rows_bwd<T, full, 4, U8>;
+    if (W.smem > 48 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)W.smem);
+    kernel<<<dim3(W.grid, W.gy), NT, W.smem, st>>>(a, W);
+    return launch_status("fme_group_norm_bwd");
 }
 
 constexpr int WIDE_GRID = 592;
-bool split(const Plan& P) { return P.parts > 1 && !P.cluster; }
 // floats of the workspace before the CTAs' rows of dw and db
-int64_t split_floats(const FmeGroupNorm& a, const Plan& P, int each) { return split(P) ? (int64_t)each * ((int64_t)a.n * P.parts * a.g + (int64_t)a.n * a.g) : 0; }
+int64_t split_floats(const FmeGroupNorm& a, const Plan& P, int each) { return split_parts(P) ? (int64_t)each * ((int64_t)a.n * P.parts * a.g + (int64_t)a.n * a.g) : 0; }
 
 }  // namespace
 }  // namespace fme
@@ -702,6 +1070,9 @@ int64_t fme_group_norm_bytes(const FmeGroupNorm* a, int32_t which) {
     if (rc) return rc;
     if (which < 0 || which > 1) return bad("group norm: which must be 0 or 1");
     Plan P;
+    Rows W;
+    int kv;
+    if (make_rows(*a, which == 1, &W, &kv)) return which == 0 ? 0 : (int64_t)W.grid * W.gy * 2 * a->c * 4;
     const bool planned = make_plan(*a, which == 1, &P);
     if (which == 0) return planned ? 4 * split_floats(*a, P, 4) : 0;
     return 4 * ((planned ? split_floats(*a, P, 2) : 0) + (int64_t)(planned ? P.grid : WIDE_GRID) * 2 * a->c);
@@ -718,6 +1089,9 @@ int fme_group_norm_fwd(const FmeGroupNorm* a, void* stream) {
         return bad("group norm: workspace too small or not aligned");
     cudaStream_t st = (cudaStream_t)stream;
     Plan P;
+    Rows W;
+    int kv;
+    if (make_rows(*a, false, &W, &kv)) return a->dtype == FME_F32 ? run_rows_fwd<float>(*a, W, kv, st) : run_rows_fwd<__nv_bfloat16>(*a, W, kv, st);
     if (!make_plan(*a, false, &P)) {
         const size_t smem = (size_t)3 * a->c * 4;
         const int grid = a->n < WIDE_GRID ? a->n : WIDE_GRID;
@@ -725,12 +1099,7 @@ int fme_group_norm_fwd(const FmeGroupNorm* a, void* stream) {
         else k_norm_wide_fwd<__nv_bfloat16><<<grid, NT, smem, st>>>(*a);
         return launch_status("fme_group_norm_fwd");
     }
-    if (a->dtype == FME_F32) {
-        if (P.vec == 1) return run_fwd<float, 1, true>(*a, P, st);
-        return P.gr ? run_fwd<float, 4, true>(*a, P, st) : run_fwd<float, 4, false>(*a, P, st);
-    }
-    if (P.vec == 1) return run_fwd<__nv_bfloat16, 1, true>(*a, P, st);
-    return P.gr ? run_fwd<__nv_bfloat16, 8, true>(*a, P, st) : run_fwd<__nv_bfloat16, 8, false>(*a, P, st);
+    return a->dtype == FME_F32 ? run_fwd<float>(*a, P, st) : run_fwd<__nv_bfloat16>(*a, P, st);
 }
 
 int fme_group_norm_bwd(const FmeGroupNorm* a, void* stream) {
@@ -749,9 +1118,15 @@ int fme_group_norm_bwd(const FmeGroupNorm* a, void* stream) {
     if (a->codes && (!a->lo || !a->hi)) return bad("group norm: codes need lo and hi");
     if (!a->ws || ((uintptr_t)a->ws & 15) || a->ws_bytes < fme_group_norm_bytes(a, 1)) return bad("group norm: workspace too small or not aligned");
     Plan P;
-    int rows = a->n < WIDE_GRID ? a->n : WIDE_GRID;
+    Rows W;
+    int rows = a->n < WIDE_GRID ? a->n : WIDE_GRID, kv;
     int64_t skip = 0;
-    if (!make_plan(*a, true, &P)) {
+    const bool u8 = a->codes != nullptr;
+    if (make_rows(*a, true, &W, &kv)) {
+        rows = W.grid * W.gy;
+        if (a->dtype == FME_F32) rc = u8 ? run_rows_bwd<float, true>(*a, W, kv, st) : run_rows_bwd<float, false>(*a, W, kv, st);
+        else rc = u8 ? run_rows_bwd<__nv_bfloat16, true>(*a, W, kv, st) : run_rows_bwd<__nv_bfloat16, false>(*a, W, kv, st);
+    } else if (!make_plan(*a, true, &P)) {
         const size_t smem = (size_t)4 * a->c * 4;
         auto kernel = a->dtype == FME_F32 ? k_norm_wide_bwd<float> : k_norm_wide_bwd<__nv_bfloat16>;
         if (smem > 48 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
@@ -760,16 +1135,8 @@ int fme_group_norm_bwd(const FmeGroupNorm* a, void* stream) {
     } else {
         rows = P.grid;
         skip = split_floats(*a, P, 2);
-        const bool u8 = a->codes != nullptr;
-        if (a->dtype == FME_F32) {
-            if (P.vec == 1) rc = u8 ? run_bwd<float, 1, true, true>(*a, P, st) : run_bwd<float, 1, true, false>(*a, P, st);
-            else if (P.gr) rc = u8 ? run_bwd<float, 4, true, true>(*a, P, st) : run_bwd<float, 4, true, false>(*a, P, st);
-            else rc = u8 ? run_bwd<float, 4, false, true>(*a, P, st) : run_bwd<float, 4, false, false>(*a, P, st);
-        } else {
-            if (P.vec == 1) rc = u8 ? run_bwd<__nv_bfloat16, 1, true, true>(*a, P, st) : run_bwd<__nv_bfloat16, 1, true, false>(*a, P, st);
-            else if (P.gr) rc = u8 ? run_bwd<__nv_bfloat16, 8, true, true>(*a, P, st) : run_bwd<__nv_bfloat16, 8, true, false>(*a, P, st);
-            else rc = u8 ? run_bwd<__nv_bfloat16, 8, false, true>(*a, P, st) : run_bwd<__nv_bfloat16, 8, false, false>(*a, P, st);
-        }
+        if (a->dtype == FME_F32) rc = u8 ? run_bwd<float, true>(*a, P, st) : run_bwd<float, false>(*a, P, st);
+        else rc = u8 ? run_bwd<__nv_bfloat16, true>(*a, P, st) : run_bwd<__nv_bfloat16, false>(*a, P, st);
     }
     if (rc || !a->dw) return rc;
     k_norm_params<<<(2 * a->c + 31) / 32, dim3(32, 32), 0, st>>>((const float*)a->ws + skip, rows, a->c, a->dw, a->db);
