@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_ENV_VAR = "FME_B200_LIB"
@@ -118,6 +119,12 @@ class FmeGroupNorm(ctypes.Structure):
                [("x", _P), ("x_sn", _i64), ("dy_sn", _i64)] + \
                [(f, _P) for f in ("y", "w", "b", "mean", "rstd", "codes", "lo", "hi", "dy", "dx", "dw", "db", "ws")] + \
                [("ws_bytes", _i64)]
+
+
+# The same two structures as packed bytes: a call's arguments in one step, where filling the fields would take longer than
+# the smallest kernels (null pointers are 0)
+ATTN = struct.Struct("@5if" + "Pqqq" * 4 + "PPqqPP" + "Pqqq" * 4 + "PPPPq")
+NORM = struct.Struct("@6ifPqq13Pq")
 
 
 class FmeError(RuntimeError):

@@ -13,6 +13,7 @@ same inputs give the same bits. There is no CPU path. The reference has no count
 from __future__ import annotations
 
 import ctypes
+from functools import lru_cache
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -23,22 +24,25 @@ _DTYPES = {torch.float32: N.FME_F32, torch.bfloat16: N.FME_BF16}
 _ACTS = {"none": N.FME_ACT_NONE, "relu": N.FME_ACT_RELU, "silu": N.FME_ACT_SILU}
 HEAD_DIMS = (32, 64, 128)
 MAX_CHANNELS = 4096
+_fns = {}
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current = torch._C._cuda_getDevice
 
 
-def _need(ok, what):
-    if not ok:
-        raise ValueError(what)
+def _call(name, args, index):
+    """One library call (args: the packed structure) on the current stream of device `index`, with that device current."""
+    if _current() != index:
+        with torch.cuda.device(index):
+            return _call(name, args, index)
+    f = _fns.get(name)
+    if f is None:
+        f = _fns[name] = getattr(N.lib(), name)
+    rc = f(args, _raw_stream(index))
+    if rc:
+        N.check(rc, name)
 
 
-def _call(name, args, dev):
-    """One library call on the current stream of dev, with dev current."""
-    if torch.cuda.current_device() != dev.index:
-        with torch.cuda.device(dev):
-            return _call(name, args, dev)
-    N.check(getattr(N.lib(), name)(ctypes.byref(args), torch.cuda.current_stream(dev).cuda_stream), name)
-
-
-def _bytes(name, args, which):
+def _size(name, args, which):
     n = getattr(N.lib(), name)(ctypes.byref(args), which)
     if n < 0:
         N.check(int(n), name)
@@ -49,69 +53,108 @@ def _scratch(nbytes, dev):
     return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
 
 
-def _p(t):
-    return None if t is None else t.data_ptr()
+def _ptr(t):
+    return 0 if t is None else t.data_ptr()
 
 
 # ---------------------------------------------------------------------------------------------- decayed attention
 def _rows(x):
     """x itself if the kernels can read its rows (last axis contiguous, rows on 16-byte boundaries), else a copy."""
-    e = x.element_size()
-    ok = x.stride(-1) == 1 and x.data_ptr() % 16 == 0
-    ok = ok and all(x.size(i) == 1 or x.stride(i) * e % 16 == 0 for i in range(x.dim() - 1))
-    return x if ok else x.clone(memory_format=torch.contiguous_format)
+    if x.data_ptr() & 15 == 0:
+        if x.is_contiguous():
+            return x
+        e = x.element_size()
+        if x.stride(-1) == 1 and all(x.size(i) == 1 or x.stride(i) * e % 16 == 0 for i in range(x.dim() - 1)):
+            return x
+    return x.clone(memory_format=torch.contiguous_format)
 
 
 def _t4(x):
     """(pointer, strides) of an (N, T, H, D) tensor; the stride of an axis of one element is not used and given as 0."""
-    s = x.stride()
-    return (x.data_ptr(), s[0] if x.size(0) > 1 else 0, s[1] if x.size(1) > 1 else 0, s[2] if x.size(2) > 1 else 0)
+    n, t, h, _ = x.shape
+    sn, st, sh, _ = x.stride()
+    return x.data_ptr(), sn if n > 1 else 0, st if t > 1 else 0, sh if h > 1 else 0
 
 
-_NO4 = (None, 0, 0, 0)
+_NO4 = (0, 0, 0, 0)
 
 
 def _check_qkv(q, k, v, log_decay, reset, state, lead):
-    _need(q.is_cuda, "decay attention runs on a CUDA device (there is no CPU path)")
-    _need(q.dim() == lead + 2, f"q must have {lead + 2} axes")
-    _need(q.dtype in _DTYPES, "q must be float32 or bfloat16")
-    for x, name in ((k, "k"), (v, "v")):
-        _need(x.shape == q.shape, f"{name} must have q's shape {tuple(q.shape)}")
-        _need(x.dtype == q.dtype and x.device == q.device, f"{name} must have q's dtype and device")
-    h, d = q.shape[-2], q.shape[-1]
-    _need(d in HEAD_DIMS, f"the head size must be one of {HEAD_DIMS}")
-    _need(h >= 1, "at least one head is needed")
-    _need(log_decay.shape == (h,) and log_decay.dtype == torch.float32 and log_decay.device == q.device,
-          f"log_decay must be a float32 ({h},) tensor on q's device")
-    _need(not log_decay.requires_grad, "log_decay is fixed for each head: it has no gradient")
+    if not q.is_cuda:
+        raise ValueError("decay attention runs on a CUDA device (there is no CPU path)")
+    shape, dtype, dev = q.shape, q.dtype, q.get_device()
+    if len(shape) != lead + 2:
+        raise ValueError(f"q must have {lead + 2} axes")
+    if dtype not in _DTYPES:
+        raise ValueError("q must be float32 or bfloat16")
+    if k.shape != shape or v.shape != shape:
+        raise ValueError(f"k and v must have q's shape {tuple(shape)}")
+    if k.dtype != dtype or v.dtype != dtype or k.get_device() != dev or v.get_device() != dev:
+        raise ValueError("k and v must have q's dtype and device")
+    n, h, d = shape[0], shape[-2], shape[-1]
+    if d not in HEAD_DIMS:
+        raise ValueError(f"the head size must be one of {HEAD_DIMS}")
+    if h < 1:
+        raise ValueError("at least one head is needed")
+    if log_decay.shape != (h,) or log_decay.dtype != torch.float32 or log_decay.get_device() != dev:
+        raise ValueError(f"log_decay must be a float32 ({h},) tensor on q's device")
+    if log_decay.requires_grad:
+        raise ValueError("log_decay is fixed for each head: it has no gradient")
     if reset is not None:
-        _need(reset.shape == q.shape[:lead], f"reset must have shape {tuple(q.shape[:lead])}")
-        _need(reset.dtype in (torch.bool, torch.uint8) and reset.device == q.device, "reset must be bool or uint8 on q's device")
-    if state is not None:
-        _need(state.shape == (q.shape[0], h, d, d) and state.dtype == torch.float32 and state.device == q.device,
-              f"state must be a float32 {(q.shape[0], h, d, d)} tensor on q's device")
+        if reset.shape != shape[:lead]:
+            raise ValueError(f"reset must have shape {tuple(shape[:lead])}")
+        if reset.dtype not in (torch.bool, torch.uint8) or reset.get_device() != dev:
+            raise ValueError("reset must be bool or uint8 on q's device")
+    if state is not None and (state.shape != (n, h, d, d) or state.dtype != torch.float32 or state.get_device() != dev):
+        raise ValueError(f"state must be a float32 {(n, h, d, d)} tensor on q's device")
 
 
-def _attn_args(q, k, v, o, log_decay, reset, s_in, s_out, scale):
-    n, t, h, d = q.shape
-    return N.FmeDecayAttn(n, t, h, d, _DTYPES[q.dtype], scale, _t4(q), _t4(k), _t4(v), _t4(o), log_decay.data_ptr(),
-                          _p(reset), 0 if reset is None else reset.stride(0), 0 if reset is None else reset.stride(1),
-                          _p(s_in), _p(s_out))
+@lru_cache(maxsize=4096)
+def _attn_sizes(n, t, h, d, dtype):
+    """Bytes of the forward workspace, the backward workspace, and of what the forward pass keeps for the backward pass."""
+    a = N.FmeDecayAttn(n=n, t=t, h=h, d=d, dtype=dtype)
+    return tuple(_size("fme_decay_attn_bytes", a, i) for i in range(3))
 
 
 def _attn_forward(q, k, v, log_decay, reset, state, scale, return_state, keep):
     """o, the state after the last token, and what the backward pass wants of the states in between."""
     n, t, h, d = q.shape
+    dev, dtype = q.device, _DTYPES[q.dtype]
     o = torch.empty_like(q)
-    if o.stride() != q.stride():      # q had a shared or overlapping axis
-        o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    last = torch.empty((n, h, d, d), dtype=torch.float32, device=q.device) if return_state else None
-    a = _attn_args(q, k, v, o, log_decay, reset, state, last, scale)
-    ws = _scratch(_bytes("fme_decay_attn_bytes", a, 0), q.device)
-    saved = _scratch(_bytes("fme_decay_attn_bytes", a, 2), q.device) if keep else None
-    a.saved, a.ws, a.ws_bytes = _p(saved), _p(ws), 0 if ws is None else ws.numel()
-    _call("fme_decay_attn_fwd", a, q.device)
+    if not q.is_contiguous() and o.stride() != q.stride():      # q had a shared or overlapping axis
+        o = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    last = torch.empty((n, h, d, d), dtype=torch.float32, device=dev) if return_state else None
+    sizes = _attn_sizes(n, t, h, d, dtype)
+    ws = _scratch(sizes[0], dev)
+    saved = _scratch(sizes[2], dev) if keep else None
+    rs = (0, 0) if reset is None else reset.stride()
+    _call("fme_decay_attn_fwd",
+          N.ATTN.pack(n, t, h, d, dtype, scale, *_t4(q), *_t4(k), *_t4(v), *_t4(o), log_decay.data_ptr(), _ptr(reset), *rs, _ptr(state), _ptr(last),
+                      *_NO4, *_NO4, *_NO4, *_NO4, 0, 0, _ptr(saved), _ptr(ws), sizes[0]), q.get_device())
     return o, last, saved
+
+
+def _attn_backward(ctx, do, dlast):
+    q, k, v, log_decay, reset, state, saved = ctx.saved_tensors
+    n, t, h, d = q.shape
+    dev, dtype = q.device, _DTYPES[q.dtype]
+    do = torch.zeros_like(q) if do is None else _rows(do)
+    dlast = None if dlast is None else dlast.contiguous()
+    if q.is_contiguous():
+        dq, dk, dv = torch.empty_like(q), torch.empty_like(q), torch.empty_like(q)
+    else:
+        dq, dk, dv = (torch.empty(q.shape, dtype=q.dtype, device=dev) for _ in range(3))
+    ds = torch.empty_like(state) if state is not None and ctx.needs_input_grad[5] else None
+    sizes = _attn_sizes(n, t, h, d, dtype)
+    ws = _scratch(sizes[1], dev)
+    rs = (0, 0) if reset is None else reset.stride()
+    _call("fme_decay_attn_bwd",
+          N.ATTN.pack(n, t, h, d, dtype, ctx.scale, *_t4(q), *_t4(k), *_t4(v), *_NO4, log_decay.data_ptr(), _ptr(reset), *rs, _ptr(state), 0,
+                      *_t4(do), *_t4(dq), *_t4(dk), *_t4(dv), _ptr(dlast), _ptr(ds), _ptr(saved), _ptr(ws), sizes[1]), q.get_device())
+    return dq, dk, dv, None, None, ds, None, None
+
+
+_attn_backward_once = once_differentiable(_attn_backward)
 
 
 class _DecayAttention(torch.autograd.Function):
@@ -124,19 +167,8 @@ class _DecayAttention(torch.autograd.Function):
         return o, last
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, do, dlast):
-        q, k, v, log_decay, reset, state, saved = ctx.saved_tensors
-        do = torch.zeros_like(q) if do is None else _rows(do)
-        dlast = None if dlast is None else dlast.contiguous()
-        dq, dk, dv = (torch.empty(q.shape, dtype=q.dtype, device=q.device) for _ in range(3))
-        ds = torch.empty_like(state) if state is not None and ctx.needs_input_grad[5] else None
-        a = _attn_args(q, k, v, q, log_decay, reset, state, None, ctx.scale)
-        a.d_o, a.dq, a.dk, a.dv = (N.FmeAttnTensor(*_t4(x)) for x in (do, dq, dk, dv))
-        ws = _scratch(_bytes("fme_decay_attn_bytes", a, 1), q.device)
-        a.ds_out, a.ds_in, a.saved, a.ws, a.ws_bytes = _p(dlast), _p(ds), _p(saved), _p(ws), 0 if ws is None else ws.numel()
-        _call("fme_decay_attn_bwd", a, q.device)
-        return dq, dk, dv, None, None, ds, None, None
+    def backward(ctx, do, dlast):   # under create_graph a second derivative has to be refused
+        return (_attn_backward_once if torch.is_grad_enabled() else _attn_backward)(ctx, do, dlast)
 
 
 def decay_attention(q, k, v, log_decay, *, reset=None, state=None, scale=None, return_state=True):
@@ -152,36 +184,45 @@ def decay_attention(q, k, v, log_decay, *, reset=None, state=None, scale=None, r
     _check_qkv(q, k, v, log_decay, reset, state, 2)
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
     q, k, v, log_decay = _rows(q), _rows(k), _rows(v), log_decay.contiguous()
-    state = None if state is None else state.contiguous()
+    if state is not None:
+        state = state.contiguous()
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (state is not None and state.requires_grad)):
         return _DecayAttention.apply(q, k, v, log_decay, reset, state, scale, return_state)
     o, last, _ = _attn_forward(q, k, v, log_decay, reset, state, scale, return_state, False)
     return o, last
 
 
-@torch.no_grad()
 def decay_attention_step(q, k, v, log_decay, state, *, reset=None, scale=None, out=None):
     """One token of `decay_attention` for each of N envs, for acting: q, k, v (N, H, D), reset (N,), and state
     (N, H, D, D) float32 contiguous, which is updated in place. Returns o (N, H, D), in `out` where given. No gradient."""
     _check_qkv(q, k, v, log_decay, reset, state, 1)
-    _need(state is not None and state.is_contiguous(), "state must be contiguous: it is updated in place")
+    if state is None or not state.is_contiguous():
+        raise ValueError("state must be contiguous: it is updated in place")
     n, h, d = q.shape
     if out is None:
         out = torch.empty((n, h, d), dtype=q.dtype, device=q.device)
-    else:
-        _need(out.shape == q.shape and out.dtype == q.dtype and out.device == q.device and _rows(out) is out,
-              "out must have q's shape, dtype and device, with 16-byte aligned rows")
-    q, k, v, log_decay = _rows(q), _rows(k), _rows(v), log_decay.contiguous()
-    t3 = lambda x: (x.data_ptr(), x.stride(0) if n > 1 else 0, 0, x.stride(1) if h > 1 else 0)  # noqa: E731
-    a = N.FmeDecayAttn(n, 1, h, d, _DTYPES[q.dtype], d ** -0.5 if scale is None else scale, t3(q), t3(k), t3(v), t3(out),
-                       log_decay.data_ptr(), _p(reset), 0 if reset is None else reset.stride(0), 0, state.data_ptr(), state.data_ptr())
-    _call("fme_decay_attn_step", a, q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.get_device() != q.get_device() or _rows(out) is not out:
+        raise ValueError("out must have q's shape, dtype and device, with 16-byte aligned rows")
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    log_decay = log_decay.contiguous()
+    s = state.data_ptr()
+    _call("fme_decay_attn_step",
+          N.ATTN.pack(n, 1, h, d, _DTYPES[q.dtype], d ** -0.5 if scale is None else scale, *_t3(q), *_t3(k), *_t3(v), *_t3(out), log_decay.data_ptr(),
+                      _ptr(reset), 0 if reset is None else reset.stride(0), 0, s, s, *_NO4, *_NO4, *_NO4, *_NO4, 0, 0, 0, 0, 0), q.get_device())
     return out
+
+
+def _t3(x):
+    n, h, _ = x.shape
+    sn, sh, _ = x.stride()
+    return x.data_ptr(), sn if n > 1 else 0, 0, sh if h > 1 else 0
 
 
 # ---------------------------------------------------------------------------------------------- group norm
 def _channels_last(x):
     """Whether each sample of x (N, C, ...) is dense with its channels innermost."""
+    if x.dim() == 4 and x.is_contiguous(memory_format=torch.channels_last) or x.dim() == 2 and x.is_contiguous():
+        return True
     want = 1
     for i in (1, *range(x.dim() - 1, 1, -1)):
         if x.size(i) != 1 and x.stride(i) != want:
@@ -192,37 +233,78 @@ def _channels_last(x):
 
 def _like(x):
     """A dense channels-last tensor of x's shape and dtype."""
+    if x.dim() == 4:
+        return torch.empty(x.shape, dtype=x.dtype, device=x.device, memory_format=torch.channels_last)
     if x.dim() == 2:
         return torch.empty(x.shape, dtype=x.dtype, device=x.device)
     return torch.empty((x.size(0), *x.shape[2:], x.size(1)), dtype=x.dtype, device=x.device).movedim(-1, 1)
 
 
-def _norm_args(x, groups, weight, bias, eps, act):
-    n, c = x.shape[0], x.shape[1]
+def _pixels(shape):
     p = 1
-    for s in x.shape[2:]:
+    for s in shape[2:]:
         p *= s
-    a = N.FmeGroupNorm(n, p, c, groups, _DTYPES[x.dtype], act, eps)
-    a.w, a.b = _p(weight), _p(bias)
-    return a
+    return p
+
+
+@lru_cache(maxsize=4096)
+def _norm_size(n, p, c, groups, dtype, u8, x_aligned, x_sn, dy_aligned, dy_sn, which):
+    """Workspace bytes of a call; they depend on whether x and dy can be read in 16-byte pieces."""
+    at = lambda ok: 256 if ok else 257  # noqa: E731
+    a = N.FmeGroupNorm(n=n, p=p, c=c, g=groups, dtype=dtype, x=at(x_aligned), x_sn=x_sn, dy=at(dy_aligned), dy_sn=dy_sn, y=256, dx=256,
+                       codes=256 if u8 else None)
+    return _size("fme_group_norm_bytes", a, which)
 
 
 def _norm_forward(x, groups, weight, bias, eps, act, keep, u8):
-    a = _norm_args(x, groups, weight, bias, eps, act)
+    shape = x.shape
+    n, c, p = shape[0], shape[1], _pixels(shape)
+    dtype, dev, xp, sn = _DTYPES[x.dtype], x.device, x.data_ptr(), x.stride(0)
     y = _like(x)
-    n, dev = x.shape[0], x.device
-    a.x, a.y, a.x_sn = x.data_ptr(), y.data_ptr(), x.stride(0)
     stats = codes = None
-    if keep:
-        stats = torch.empty((4 if u8 else 2, n, groups), dtype=torch.float32, device=dev)
-        a.mean, a.rstd = stats.data_ptr(), stats.data_ptr() + 4 * n * groups
+    mean = codes_p = lo = 0
+    if keep:      # rows: mean, rstd, and the ranges of the codes
+        stats = torch.empty((4 if u8 else 2) * n * groups, dtype=torch.float32, device=dev)
+        mean = stats.data_ptr()
         if u8:
-            codes = torch.empty((n, a.p, a.c), dtype=torch.uint8, device=dev)
-            a.codes, a.lo, a.hi = codes.data_ptr(), a.mean + 8 * n * groups, a.mean + 12 * n * groups
-    ws = _scratch(_bytes("fme_group_norm_bytes", a, 0), dev)
-    a.ws, a.ws_bytes = _p(ws), 0 if ws is None else ws.numel()
-    _call("fme_group_norm_fwd", a, dev)
+            codes = torch.empty(n * p * c, dtype=torch.uint8, device=dev)
+            codes_p, lo = codes.data_ptr(), mean + 8 * n * groups
+    need = _norm_size(n, p, c, groups, dtype, u8, xp & 15 == 0, sn, True, 0, 0)
+    ws = _scratch(need, dev)
+    _call("fme_group_norm_fwd",
+          N.NORM.pack(n, p, c, groups, dtype, act, eps, xp, sn, 0, y.data_ptr(), _ptr(weight), _ptr(bias), mean, mean and mean + 4 * n * groups, codes_p,
+                      lo, lo and lo + 4 * n * groups, 0, 0, 0, 0, _ptr(ws), need), x.get_device())
     return y, stats, codes
+
+
+def _norm_backward(ctx, dy):
+    kept, weight, bias, stats = ctx.saved_tensors
+    groups, eps, act, u8 = ctx.how
+    if not _channels_last(dy):
+        dy = dy.movedim(1, -1).contiguous().movedim(-1, 1)
+    shape = dy.shape
+    n, c, p = shape[0], shape[1], _pixels(shape)
+    dtype, dev, dyp, dy_sn, mean = _DTYPES[dy.dtype], dy.device, dy.data_ptr(), dy.stride(0), stats.data_ptr()
+    dx = _like(dy)
+    if u8:
+        xp, x_sn, codes, lo = 0, 0, kept.data_ptr(), mean + 8 * n * groups
+    else:
+        xp, x_sn, codes, lo = kept.data_ptr(), kept.stride(0), 0, 0
+    need = _norm_size(n, p, c, groups, dtype, u8, xp & 15 == 0, x_sn, dyp & 15 == 0, dy_sn, 1)
+    wants_w, wants_b = ctx.needs_input_grad[1], ctx.needs_input_grad[2]
+    dw = db = None
+    dwp = 0
+    if wants_w or wants_b:
+        dw, db = torch.empty((2, c), dtype=torch.float32, device=dev).unbind()
+        dwp = dw.data_ptr()
+    ws = _scratch(need, dev)
+    _call("fme_group_norm_bwd",
+          N.NORM.pack(n, p, c, groups, dtype, act, eps, xp, x_sn, dy_sn, 0, _ptr(weight), _ptr(bias), mean, mean + 4 * n * groups, codes, lo,
+                      lo and lo + 4 * n * groups, dyp, dx.data_ptr(), dwp, dwp and dwp + 4 * c, _ptr(ws), need), dy.get_device())
+    return dx, dw if wants_w else None, db if wants_b else None, None, None, None, None
+
+
+_norm_backward_once = once_differentiable(_norm_backward)
 
 
 class _GroupNormAct(torch.autograd.Function):
@@ -234,29 +316,8 @@ class _GroupNormAct(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        kept, weight, bias, stats = ctx.saved_tensors
-        groups, eps, act, u8 = ctx.how
-        if not _channels_last(dy):
-            dy = dy.movedim(1, -1).contiguous().movedim(-1, 1)
-        n, dev = dy.shape[0], dy.device
-        a = _norm_args(dy, groups, weight, bias, eps, act)
-        dx = _like(dy)
-        a.mean, a.rstd = stats.data_ptr(), stats.data_ptr() + 4 * n * groups
-        if u8:
-            a.codes, a.lo, a.hi = kept.data_ptr(), a.mean + 8 * n * groups, a.mean + 12 * n * groups
-        else:
-            a.x, a.x_sn = kept.data_ptr(), kept.stride(0)
-        a.dy, a.dy_sn, a.dx = dy.data_ptr(), dy.stride(0), dx.data_ptr()
-        dw = db = None
-        if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
-            dw, db = torch.empty((2, a.c), dtype=torch.float32, device=dev).unbind()
-            a.dw, a.db = dw.data_ptr(), db.data_ptr()
-        ws = _scratch(_bytes("fme_group_norm_bytes", a, 1), dev)
-        a.ws, a.ws_bytes = _p(ws), 0 if ws is None else ws.numel()
-        _call("fme_group_norm_bwd", a, dev)
-        return dx, dw if ctx.needs_input_grad[1] else None, db if ctx.needs_input_grad[2] else None, None, None, None, None
+        return (_norm_backward_once if torch.is_grad_enabled() else _norm_backward)(ctx, dy)
 
 
 def group_norm_act(x, groups, weight=None, bias=None, *, eps=1e-5, act="silu", checkpoint="full"):
@@ -267,18 +328,29 @@ def group_norm_act(x, groups, weight=None, bias=None, *, eps=1e-5, act="silu", c
     normalises heads. checkpoint: what the backward pass keeps of x: "full" x itself, "u8" one byte a value, with the
     range of each (sample, group); gradients then are those at the values the codes stand for (an error of at most
     1/510 of that range). Gradients for x, weight and bias."""
-    _need(x.is_cuda, "group norm runs on a CUDA device (there is no CPU path)")
-    _need(x.dim() >= 2, "x must be (N, C, ...)")
-    _need(x.dtype in _DTYPES, "x must be float32 or bfloat16")
-    c = x.shape[1]
-    _need(1 <= c <= MAX_CHANNELS, f"the number of channels must be in 1..{MAX_CHANNELS}")
-    _need(isinstance(groups, int) and groups >= 1 and c % groups == 0, f"groups must divide the {c} channels")
-    _need(act in _ACTS, f"act must be one of {tuple(_ACTS)}")
-    _need(checkpoint in ("full", "u8"), 'checkpoint must be "full" or "u8"')
-    _need(_channels_last(x), "x must have channels-last memory (x.contiguous(memory_format=torch.channels_last))")
+    if not x.is_cuda:
+        raise ValueError("group norm runs on a CUDA device (there is no CPU path)")
+    if x.dim() < 2:
+        raise ValueError("x must be (N, C, ...)")
+    if x.dtype not in _DTYPES:
+        raise ValueError("x must be float32 or bfloat16")
+    c = x.size(1)
+    if not 1 <= c <= MAX_CHANNELS:
+        raise ValueError(f"the number of channels must be in 1..{MAX_CHANNELS}")
+    if not isinstance(groups, int) or groups < 1 or c % groups:
+        raise ValueError(f"groups must divide the {c} channels")
+    if act not in _ACTS:
+        raise ValueError(f"act must be one of {tuple(_ACTS)}")
+    if checkpoint not in ("full", "u8"):
+        raise ValueError('checkpoint must be "full" or "u8"')
+    if not _channels_last(x):
+        raise ValueError("x must have channels-last memory (x.contiguous(memory_format=torch.channels_last))")
+    grad = x.requires_grad
     for t, name in ((weight, "weight"), (bias, "bias")):
-        _need(t is None or (t.shape == (c,) and t.dtype == torch.float32 and t.device == x.device and t.is_contiguous()),
-              f"{name} must be a contiguous float32 ({c},) tensor on x's device")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+        if t is not None:
+            if t.shape != (c,) or t.dtype != torch.float32 or t.get_device() != x.get_device() or not t.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous float32 ({c},) tensor on x's device")
+            grad = grad or t.requires_grad
+    if grad and torch.is_grad_enabled():
         return _GroupNormAct.apply(x, weight, bias, groups, eps, _ACTS[act], checkpoint == "u8")
     return _norm_forward(x, groups, weight, bias, eps, _ACTS[act], False, False)[0]

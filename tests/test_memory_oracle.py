@@ -106,6 +106,18 @@ def test_library_refuses_bad_norm_arguments(kw, said):
     assert N.lib().fme_group_norm_bwd(ctypes.byref(a), None) == -1 and "together" in N.last_error()
 
 
+def test_packed_arguments_have_the_structures_layout():
+    for packed, struct in ((N.ATTN, N.FmeDecayAttn), (N.NORM, N.FmeGroupNorm)):
+        assert packed.size == ctypes.sizeof(struct)
+        n = len(packed.unpack(bytes(packed.size)))
+        raw = struct.from_buffer_copy(packed.pack(*range(1, n + 1)))
+        flat = []
+        for name, _ in struct._fields_:
+            v = getattr(raw, name)
+            flat += [v.p, v.sn, v.st, v.sh] if isinstance(v, N.FmeAttnTensor) else [v]
+        assert [int(v) for v in flat] == list(range(1, n + 1))
+
+
 def test_empty_calls_need_no_buffers():
     assert N.lib().fme_decay_attn_fwd(ctypes.byref(_attn(n=0)), None) == 0
     a = N.FmeGroupNorm(n=0, p=1, c=8, g=2, dtype=N.FME_F32, act=0, eps=1e-5)
