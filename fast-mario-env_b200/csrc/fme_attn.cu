@@ -30,7 +30,7 @@ template <typename T, int D> struct Shape {
     static constexpr int NW = D / 16, NT = 32 * NW, RB = C / 16, CG = NW / RB, NC = D / CG;
     static constexpr int TILE = C * D * (int)sizeof(T), MAT = D * D * (int)sizeof(T);
     static constexpr int STAGE = 16 * NC * (int)sizeof(T);   // a warp's outputs on their way out
-    static constexpr int FLOATS = 2 * 72;                    // powers and weights
+    static constexpr int FLOATS = 3 * 72;                    // powers, powers one place on, weights
 };
 
 // Where a chunk restarts. Bit i: token i does; valid tokens only.
@@ -63,12 +63,14 @@ struct ResetBytes {
 // rows of one operand's chunk to shared memory; rows past the sequence's end become zeros
 template <typename T, int D, int C, int NT>
 __device__ __forceinline__ void load_tile(const Tile<T, D>& dst, const T* src, int64_t st, int t0, int n) {
-    constexpr int PIECES = D / Tile<T, D>::PER;
+    constexpr int PIECES = D / Tile<T, D>::PER, STEP = NT / PIECES;   // STEP: rows between a thread's pieces
+    const int row = threadIdx.x / PIECES, col = (threadIdx.x % PIECES) * Tile<T, D>::PER;
+    const char* p = reinterpret_cast<const char*>(src + (t0 + row) * st + col);
+    const int64_t step = STEP * st * (int64_t)sizeof(T);
 #pragma unroll
-    for (int i = 0; i < C * PIECES / NT; i++) {
-        const int e = i * NT + threadIdx.x, row = e / PIECES, col = (e % PIECES) * Tile<T, D>::PER;
-        const bool in = row < n;
-        cp16(dst.addr(row, col), src + (in ? (t0 + row) * st + col : 0), in);
+    for (int i = 0; i < C / STEP; i++) {
+        const bool in = row + i * STEP < n;
+        cp16(dst.base + dst.off(row + i * STEP, col), in ? p + i * step : reinterpret_cast<const char*>(src), in);
     }
 }
 
@@ -116,7 +118,7 @@ template <int N> __device__ __forceinline__ void zero(float (&a)[N][4]) {
 template <typename T, int NB, int K, bool TR, typename TA, typename TB>
 __device__ __forceinline__ void product(float (&acc)[NB][4], const TA& a, int m, const TB& b, int n) {
     using F = Frag<T>;
-#pragma unroll
+#pragma unroll(Frag<T>::UNROLL)
     for (int k = 0; k < K; k += F::KS) {
         const typename F::A fa = F::ldA(a, m, k);
 #pragma unroll
@@ -130,13 +132,34 @@ __device__ __forceinline__ void product(float (&acc)[NB][4], const TA& a, int m,
     }
 }
 
-// One chunk's scores: p[row][col] = (a_row . b_col) L scale for rows row0.. against all C columns. UP: rows are i, columns j
-// (a = q or do, b = k or v); otherwise rows are j and columns i. Blocks that L empties are skipped.
+// A warp's factors of L * scale: within the 16 x 16 block on the diagonal as they are (0 above it), elsewhere
+// lambda^(i-j) = lambda^(i-edge) lambda^(edge-j) with the edge between the block's rows and the column: neither power grows.
+// UP: rows are i, columns j; otherwise rows are j and columns i.
+template <bool UP> struct Decay {
+    float diag[2][4], row[2];
+    __device__ __forceinline__ Decay(const float* pw, float scale) {
+        const int l = threadIdx.x & 31, g = l >> 2, c = l & 3;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            row[h] = pw[UP ? g + 8 * h : 15 - g - 8 * h] * scale;
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const int far = (g + 8 * h) - (8 * i + 2 * c + e), d = UP ? far : -far;
+                    diag[i][2 * h + e] = d >= 0 ? pw[d < 0 ? 0 : d] * scale : 0.f;
+                }
+        }
+    }
+};
+
+// One chunk's scores: p[row][col] = (a_row . b_col) L scale for rows row0.. against all C columns (UP: a = q or do, b = k or v).
+// Blocks that L empties are skipped. pw1: the powers, one place on, so that the pairs read stand on 8 bytes.
 template <typename T, int D, int C, bool UP>
-__device__ __forceinline__ void scores(float (&p)[C / 8][4], const Tile<T, D>& a, const Tile<T, D>& b, int row0, const Cuts& cuts, const float* pw, float scale) {
+__device__ __forceinline__ void scores(float (&p)[C / 8][4], const Tile<T, D>& a, const Tile<T, D>& b, int row0, const Cuts& cuts, const float* pw1, const Decay<UP>& dec) {
     using F = Frag<T>;
     zero(p);
-#pragma unroll
+#pragma unroll(Frag<T>::UNROLL)
     for (int k = 0; k < D; k += F::KS) {
         const typename F::A fa = F::ldA(a, row0, k);
 #pragma unroll
@@ -148,21 +171,25 @@ __device__ __forceinline__ void scores(float (&p)[C / 8][4], const Tile<T, D>& a
             F::mma(p[i + 1], fa, b1);
         }
     }
-    const int l = threadIdx.x & 31, g = l >> 2, c = l & 3;
+    // No restart in (j, i] means none in (j, edge] and none in (edge, i]: outside the diagonal's block the mask is a product too
+    const int l = threadIdx.x & 31, g = l >> 2, c = 2 * (l & 3), edge = UP ? row0 : row0 + 15;
+    const int lim0 = UP ? cuts.last_up_to(row0 + g) : cuts.next_after(row0 + g), lim1 = UP ? cuts.last_up_to(row0 + g + 8) : cuts.next_after(row0 + g + 8);
+    const int lim = UP ? cuts.last_up_to(edge) : cuts.next_after(edge);
+    const float r0 = (UP ? lim0 <= edge : lim0 > edge) ? dec.row[0] : 0.f, r1 = (UP ? lim1 <= edge : lim1 > edge) ? dec.row[1] : 0.f;
 #pragma unroll
-    for (int half = 0; half < 2; half++) {
-        const int row = row0 + g + 8 * half;
-        const int lim = UP ? cuts.last_up_to(row) : cuts.next_after(row);
+    for (int i = 0; i < C / 8; i++) {
+        const int col = 8 * i + c;
+        if ((8 * i & ~15) == row0) {
 #pragma unroll
-        for (int i = 0; i < C / 8; i++)
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-                const int col = 8 * i + 2 * c + e;
-                float& x = p[i][2 * half + e];
-                const bool in = UP ? col <= row && col >= lim : col >= row && col < lim;
-                const int far = UP ? row - col : col - row;
-                x = in ? x * (pw[far < 0 ? 0 : far] * scale) : 0.f;
+            for (int j = 0; j < 4; j++) {
+                const int at = col + (j & 1), lim = j < 2 ? lim0 : lim1;
+                p[i][j] = (UP ? at >= lim : at < lim) ? p[i][j] * dec.diag[i & 1][j] : 0.f;
             }
+        } else if (UP ? 8 * i < row0 : 8 * i > row0) {
+            const float2 e = *reinterpret_cast<const float2*>(pw1 + (UP ? row0 - col : col - row0 - 14));
+            const float x = (UP ? col >= lim : col < lim) ? (UP ? e.y : e.x) : 0.f, y = (UP ? col + 1 >= lim : col + 1 < lim) ? (UP ? e.x : e.y) : 0.f;
+            p[i][0] *= x * r0; p[i][1] *= y * r0; p[i][2] *= x * r1; p[i][3] *= y * r1;
+        }
     }
 }
 
@@ -188,7 +215,7 @@ __device__ __forceinline__ void apply_scores(float (&acc)[NB][4], const float (&
 template <typename T, int D, int C, bool TWO>
 __device__ __forceinline__ void outer(float (&s)[D / 8][4], const Tile<T, D>& a, int m0, const float* w, const Tile<T, D>& b) {
     using F = Frag<T>;
-#pragma unroll
+#pragma unroll(Frag<T>::UNROLL)
     for (int k = 0; k < C; k += F::KS) {
         const typename F::A2 fa = F::template ldAt<TWO>(a, k, m0, w);
 #pragma unroll
@@ -282,8 +309,8 @@ struct Walkers {   // the grid's layout: CTA = (sequence and head) * segs + segm
     float* parts;            // state of the segments: D * D floats each, then one float each: what a segment passes on
 };
 
-__device__ __forceinline__ void powers(float* pw, int n, float log2_lam) {
-    for (int i = threadIdx.x; i < n; i += blockDim.x) pw[i] = i ? exp2f(log2_lam * (float)i) : 1.f;
+__device__ __forceinline__ void powers(float* pw, float* pw1, int n, float log2_lam) {
+    for (int i = threadIdx.x; i < n; i += blockDim.x) pw[i] = pw1[i + 1] = i ? exp2f(log2_lam * (float)i) : 1.f;
 }
 
 constexpr float LOG2E = 1.44269504088896340736f;
@@ -297,11 +324,11 @@ __global__ void __launch_bounds__(Shape<T, D>::NT, MINB) k_attn_fwd(const FmeDec
     extern __shared__ __align__(1024) char sm[];
     const Ti tk(sm), tv(sm + Z::TILE), tq(sm + 2 * Z::TILE), ts(sm + 3 * Z::TILE);
     float* pw = reinterpret_cast<float*>(sm + (LOCAL ? 2 * Z::TILE : 3 * Z::TILE + Z::MAT));   // C + 1
-    float* z = pw + 72;                                                                       // C
+    float *pw1 = pw + 72, *z = pw + 144;                                                      // C + 2, C
     const int warp = threadIdx.x >> 5, l = threadIdx.x & 31, g = l >> 2;
-    const int64_t pair = LOCAL ? blockIdx.x / (W.segs - 1) : blockIdx.x / W.segs;
-    const int seg = LOCAL ? blockIdx.x % (W.segs - 1) : blockIdx.x % W.segs;
-    const int64_t n = pair / A.h, h = pair % A.h;
+    const uint32_t across = LOCAL ? W.segs - 1 : W.segs, pair32 = across == 1 ? blockIdx.x : blockIdx.x / across, n32 = pair32 / (uint32_t)A.h;
+    const int64_t pair = pair32;
+    const int seg = blockIdx.x - pair32 * across, n = n32, h = pair32 - n32 * A.h;
     const T *q = at<T>(A.q, n, h), *k = at<T>(A.k, n, h), *v = at<T>(A.v, n, h);
     T* o = at<T>(A.o, n, h);
     const uint8_t* reset = A.reset ? A.reset + n * A.reset_sn : nullptr;
@@ -320,11 +347,13 @@ __global__ void __launch_bounds__(Shape<T, D>::NT, MINB) k_attn_fwd(const FmeDec
         rb.load(reset, A.reset_st, t0, nv);
     };
     if (c0 < c1) fetch(c0);
-    powers(pw, C + 1, g2);
+    powers(pw, pw1, C + 1, g2);
     if (seg > 0 && !LOCAL) move_part<D, NT, false>(s, W.parts, pair * (W.segs - 1) + seg - 1);
     else if (seg == 0 && A.s_in) move_state<D, true, false>(s, A.s_in + pair * D * D, m0);
     else { zero(s); some = false; }
     if (!LOCAL && some) put_state(ts, s, m0);
+    __syncthreads();
+    const Decay<true> dec(pw, A.scale);
     uint64_t any_cut = 0;
     for (int c = c0; c < c1; c++) {
         const int t0 = c * C;
@@ -347,14 +376,14 @@ __global__ void __launch_bounds__(Shape<T, D>::NT, MINB) k_attn_fwd(const FmeDec
                     acc[i][2] = in1 ? acc[i][2] * a1 : 0.f; acc[i][3] = in1 ? acc[i][3] * a1 : 0.f;
                 }
             }
-            scores<T, D, C, true>(p, tq, tk, row0, cuts, pw, A.scale);
+            scores<T, D, C, true>(p, tq, tk, row0, cuts, pw1, dec);
             apply_scores<T, D, C, NC / 8, true>(acc, p, tv, row0, col0);
             again = __syncthreads_or(not_finite(acc));
             // q and the old state have been read by all: the q tile takes the outputs
             if (!again) store_rows<T, NC>(sm + 2 * Z::TILE + warp * Z::STAGE, acc, o, A.o.st, row0, col0, t0, cuts.n);
         }
-        const bool more = c + 1 < c1;
-        if (more || LOCAL || A.s_out || A.saved) {
+        const bool more = c + 1 < c1, save = A.saved && c + 1 < W.chunks;
+        if (more || LOCAL || save || (A.s_out && c + 1 == W.chunks)) {
             const int j = threadIdx.x;
             if (j < C) z[j] = j < cuts.n && j >= last ? pw[cuts.n - 1 - j] : 0.f;
             __syncthreads();
@@ -378,8 +407,8 @@ __global__ void __launch_bounds__(Shape<T, D>::NT, MINB) k_attn_fwd(const FmeDec
         if (again) walk<T, D, false>(s, tv, tk, LOCAL ? tk : tq, 1.f, A.scale, m0, cuts, pw[1], LOCAL ? (T*)nullptr : o, A.o.st, t0);
         some = true;
         if constexpr (!LOCAL) {
-            if (more || A.saved) put_state(ts, s, m0);
-            if (A.saved && c + 1 < W.chunks) {
+            if (more || save) put_state(ts, s, m0);
+            if (save) {
                 __syncwarp();
                 T* dst = reinterpret_cast<T*>(A.saved) + ((pair * (W.chunks - 1) + c) * D + m0) * D;
                 constexpr int PIECES = D / Ti::PER;
@@ -415,12 +444,11 @@ __global__ void __launch_bounds__(Shape<T, D>::NT, MINB) k_attn_bwd(const FmeDec
     const Ti tq(sm), tg(sm + Z::TILE), tk(sm + 2 * Z::TILE), tv(sm + 3 * Z::TILE), ts(sm + 4 * Z::TILE), tu(sm + 4 * Z::TILE + Z::MAT);
     char* stage = sm + 4 * Z::TILE + 2 * Z::MAT + (threadIdx.x >> 5) * Z::STAGE;
     float* pw = reinterpret_cast<float*>(sm + (LOCAL ? 2 * Z::TILE : 4 * Z::TILE + 2 * Z::MAT + Z::NW * Z::STAGE));
-    float* a = pw + 72;
+    float *pw1 = pw + 72, *a = pw + 144;
     const int warp = threadIdx.x >> 5, l = threadIdx.x & 31, g = l >> 2;
-    const int64_t pair = LOCAL ? blockIdx.x / (W.segs - 1) : blockIdx.x / W.segs;
-    const int rseg = LOCAL ? blockIdx.x % (W.segs - 1) : blockIdx.x % W.segs;   // 0: the last in time
-    const int seg = W.segs - 1 - rseg;
-    const int64_t n = pair / A.h, h = pair % A.h;
+    const uint32_t across = LOCAL ? W.segs - 1 : W.segs, pair32 = across == 1 ? blockIdx.x : blockIdx.x / across, n32 = pair32 / (uint32_t)A.h;
+    const int64_t pair = pair32;
+    const int rseg = blockIdx.x - pair32 * across, seg = W.segs - 1 - rseg, n = n32, h = pair32 - n32 * A.h;   // rseg 0: the last in time
     const T *q = at<T>(A.q, n, h), *k = at<T>(A.k, n, h), *v = at<T>(A.v, n, h), *go = at<T>(A.d_o, n, h);
     T *dq = at<T>(A.dq, n, h), *dk = at<T>(A.dk, n, h), *dv = at<T>(A.dv, n, h);
     const uint8_t* reset = A.reset ? A.reset + n * A.reset_sn : nullptr;
@@ -446,10 +474,13 @@ __global__ void __launch_bounds__(Shape<T, D>::NT, MINB) k_attn_bwd(const FmeDec
         rb.load(reset, A.reset_st, t0, nv);
     };
     if (c0 < c1) fetch(c1 - 1);
-    powers(pw, C + 1, g2);
+    powers(pw, pw1, C + 1, g2);
     if (rseg > 0 && !LOCAL) move_part<D, NT, false>(u, W.parts, pair * (W.segs - 1) + rseg - 1);
     else if (rseg == 0 && A.ds_out) move_state<D, false, false>(u, A.ds_out + pair * D * D, m0);
     else { zero(u); some = false; }
+    __syncthreads();
+    const Decay<false> down(pw, A.scale);
+    const Decay<true> up(pw, A.scale);
     uint64_t any_cut = 0;
     for (int c = c1 - 1; c >= c0; c--) {
         const int t0 = c * C;
@@ -475,13 +506,13 @@ __global__ void __launch_bounds__(Shape<T, D>::NT, MINB) k_attn_bwd(const FmeDec
             };
             zero(acc);
             if (some) { product<T, NC / 8, D, true>(acc, tk, row0, tu, col0); weigh(z0, z1, w0, w1); }
-            scores<T, D, C, false>(p, tk, tq, row0, cuts, pw, A.scale);
+            scores<T, D, C, false>(p, tk, tq, row0, cuts, pw1, down);
             apply_scores<T, D, C, NC / 8, false>(acc, p, tg, row0, col0);
             again |= not_finite(acc);
             store_rows<T, NC>(stage, acc, dv, A.dv.st, row0, col0, t0, cuts.n);
             zero(acc);
             if (some) { product<T, NC / 8, D, false>(acc, tv, row0, tu, col0); weigh(z0, z1, w0, w1); }
-            scores<T, D, C, false>(p, tv, tg, row0, cuts, pw, A.scale);
+            scores<T, D, C, false>(p, tv, tg, row0, cuts, pw1, down);
             apply_scores<T, D, C, NC / 8, false>(acc, p, tq, row0, col0);
             again |= not_finite(acc);
             store_rows<T, NC>(stage, acc, dk, A.dk.st, row0, col0, t0, cuts.n);
@@ -490,7 +521,7 @@ __global__ void __launch_bounds__(Shape<T, D>::NT, MINB) k_attn_bwd(const FmeDec
                 product<T, NC / 8, D, true>(acc, tg, row0, ts, col0);
                 weigh(cuts.last_up_to(r0) < 0, cuts.last_up_to(r1) < 0, pw[r0 + 1] * A.scale, pw[r1 + 1] * A.scale);
             }
-            scores<T, D, C, true>(p, tg, tv, row0, cuts, pw, A.scale);
+            scores<T, D, C, true>(p, tg, tv, row0, cuts, pw1, up);
             apply_scores<T, D, C, NC / 8, true>(acc, p, tk, row0, col0);
             again |= not_finite(acc);
             store_rows<T, NC>(stage, acc, dq, A.dq.st, row0, col0, t0, cuts.n);
@@ -516,7 +547,7 @@ __global__ void __launch_bounds__(Shape<T, D>::NT, MINB) k_attn_bwd(const FmeDec
                 }
             } else if (!again) {
                 keep_state<D>(u, cuts, pw);
-                outer<T, D, C, TWO>(u, tq, m0, a, tg);
+                outer<T, D, C, true>(u, tq, m0, a, tg);
             } else {
                 float s[D / 8][4];
                 const int cc = l & 3;

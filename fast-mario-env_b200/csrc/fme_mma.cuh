@@ -41,7 +41,13 @@ template <typename T, int COLS> struct Tile {
         const uint32_t sw = ROW >= 128 ? (uint32_t)(row & 7) : (uint32_t)((row >> 1) & 3);
         return (uint32_t)row * ROW + ((piece ^ sw) << 4) + in;
     }
-    __device__ __forceinline__ uint32_t addr(int row, int col) const { return base + off(row, col); }
+    // A lane's address of piece x (0 or 1) of a row, and from there the same piece `bytes` (a multiple of 32) further along the
+    // row: the permutation is an exclusive or within 128 bytes, so that one instruction moves on
+    __device__ __forceinline__ uint32_t lane(int row, int x) const {
+        const uint32_t sw = ROW >= 128 ? (uint32_t)(row & 7) : (uint32_t)((row >> 1) & 3);
+        return base + (uint32_t)row * ROW + (((uint32_t)x ^ sw) << 4);
+    }
+    static __device__ __forceinline__ uint32_t along(uint32_t lane, int bytes) { return (lane ^ ((uint32_t)bytes & 127u)) + ((uint32_t)bytes & ~127u); }
     __device__ __forceinline__ T& at(int row, int col) const { return *reinterpret_cast<T*>(gen + off(row, col)); }
     __device__ __forceinline__ float2 two(int row, int col) const {   // col even
         if constexpr (sizeof(T) == 2) return unpack2(*reinterpret_cast<const uint32_t*>(gen + off(row, col)));
@@ -59,6 +65,11 @@ __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
 __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
 }
+__device__ __forceinline__ float lds(uint32_t addr) {
+    float x;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(addr));
+    return x;
+}
 __device__ __forceinline__ uint32_t tf32(float x) {
     uint32_t r;
     asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
@@ -72,7 +83,7 @@ __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) 
 template <typename T> struct Frag;
 
 template <> struct Frag<bf16> {
-    static constexpr int KS = 16;
+    static constexpr int KS = 16, UNROLL = 8;   // steps of a product in one piece of code
     struct A { uint32_t r[4]; };
     struct B { uint32_t r[2]; };
     struct A2 { A hi, lo; };    // a scaled operand in two bfloat16 numbers: 16 bits of it count
@@ -84,33 +95,32 @@ template <> struct Frag<bf16> {
     template <int COLS> static __device__ __forceinline__ A ldA(const Tile<bf16, COLS>& s, int m, int k) {
         const int l = threadIdx.x & 31;
         A a;
-        ldsm4(a.r, s.addr(m + (l & 15), k + ((l >> 4) << 3)));
+        ldsm4(a.r, s.along(s.lane(m + (l & 15), l >> 4), 2 * k));
         return a;
     }
     // B[k][n] = tile[n][k], 16 columns n
     template <int COLS> static __device__ __forceinline__ void ldB(const Tile<bf16, COLS>& s, int n, int k, B& b0, B& b1) {
         const int l = threadIdx.x & 31;
         uint32_t r[4];
-        ldsm4(r, s.addr(n + (l & 7) + ((l >> 4) << 3), k + (l & 8)));
+        ldsm4(r, s.along(s.lane(n + (l & 7) + ((l >> 4) << 3), (l >> 3) & 1), 2 * k));
         b0.r[0] = r[0]; b0.r[1] = r[1]; b1.r[0] = r[2]; b1.r[1] = r[3];
     }
     // B[k][n] = tile[k][n], 16 columns n
     template <bool NAT, int COLS> static __device__ __forceinline__ void ldBt(const Tile<bf16, COLS>& s, int k, int n, B& b0, B& b1) {
         const int l = threadIdx.x & 31;
         uint32_t r[4];
-        ldsm4t(r, s.addr(k + (l & 15), n + ((l >> 4) << 3)));
+        ldsm4t(r, s.along(s.lane(k + (l & 15), l >> 4), 2 * n));
         b0.r[0] = r[0]; b0.r[1] = r[1]; b1.r[0] = r[2]; b1.r[1] = r[3];
     }
     // A[m][k] = weight[k] * tile[k][m], weights in shared memory
     template <bool TWO, int COLS> static __device__ __forceinline__ A2 ldAt(const Tile<bf16, COLS>& s, int k, int m, const float* w) {
         const int l = threadIdx.x & 31;
         A2 a;
-        ldsm4t(a.hi.r, s.addr(k + (l & 7) + ((l >> 4) << 3), m + (l & 8)));
+        ldsm4t(a.hi.r, s.along(s.lane(k + (l & 7) + ((l >> 4) << 3), (l >> 3) & 1), 2 * m));
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const int at = k + ((i >> 1) << 3) + 2 * (l & 3);
-            const float2 v = unpack2(a.hi.r[i]);
-            const float x = v.x * w[at], y = v.y * w[at + 1];
+            const float2 v = unpack2(a.hi.r[i]), f = *reinterpret_cast<const float2*>(w + k + ((i >> 1) << 3) + 2 * (l & 3));
+            const float x = v.x * f.x, y = v.y * f.y;
             a.hi.r[i] = pack2(x, y);
             if (TWO) {
                 const float2 h = unpack2(a.hi.r[i]);
@@ -131,7 +141,7 @@ template <> struct Frag<bf16> {
 };
 
 template <> struct Frag<float> {
-    static constexpr int KS = 8;
+    static constexpr int KS = 8, UNROLL = 1;    // longer steps, and code that outgrows the instruction cache stalls
     struct A { uint32_t hi[4], lo[4]; };
     struct B { uint32_t hi[2], lo[2]; };
     using A2 = A;
@@ -147,7 +157,7 @@ template <> struct Frag<float> {
     template <int COLS> static __device__ __forceinline__ A ldA(const Tile<float, COLS>& s, int m, int k) {
         const int l = threadIdx.x & 31;
         uint32_t r[4];
-        ldsm4(r, s.addr(m + (l & 15), k + ((l >> 4) << 2)));
+        ldsm4(r, s.along(s.lane(m + (l & 15), l >> 4), 4 * k));
         A a;
 #pragma unroll
         for (int i = 0; i < 4; i++) split_tf32(__uint_as_float(r[i]), a.hi[i], a.lo[i]);
@@ -156,7 +166,7 @@ template <> struct Frag<float> {
     template <int COLS> static __device__ __forceinline__ void ldB(const Tile<float, COLS>& s, int n, int k, B& b0, B& b1) {
         const int l = threadIdx.x & 31;
         uint32_t r[4];
-        ldsm4(r, s.addr(n + (l & 7) + ((l >> 4) << 3), k + ((l & 8) >> 1)));
+        ldsm4(r, s.along(s.lane(n + (l & 7) + ((l >> 4) << 3), (l >> 3) & 1), 4 * k));
 #pragma unroll
         for (int i = 0; i < 2; i++) {
             split_tf32(__uint_as_float(r[i]), b0.hi[i], b0.lo[i]);
@@ -173,8 +183,9 @@ template <> struct Frag<float> {
         const int g = (threadIdx.x & 31) >> 2;
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-            split_tf32(s.at(k + row_of<NAT>(i), n + g), b0.hi[i], b0.lo[i]);
-            split_tf32(s.at(k + row_of<NAT>(i), n + 8 + g), b1.hi[i], b1.lo[i]);
+            const uint32_t at = s.lane(k + row_of<NAT>(i), g >> 2) + 4 * (g & 3);
+            split_tf32(lds(s.along(at, 4 * n)), b0.hi[i], b0.lo[i]);
+            split_tf32(lds(s.along(at, 4 * n + 32)), b1.hi[i], b1.lo[i]);
         }
     }
     template <bool TWO, int COLS> static __device__ __forceinline__ A2 ldAt(const Tile<float, COLS>& s, int k, int m, const float* w) {
@@ -183,7 +194,7 @@ template <> struct Frag<float> {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int row = k + row_of<false>(i >> 1);
-            split_tf32(s.at(row, m + g + 8 * (i & 1)) * w[row], a.hi[i], a.lo[i]);
+            split_tf32(lds(s.along(s.lane(row, g >> 2) + 4 * (g & 3), 4 * (m + 8 * (i & 1)))) * w[row], a.hi[i], a.lo[i]);
         }
         return a;
     }
