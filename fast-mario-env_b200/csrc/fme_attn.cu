@@ -67,10 +67,15 @@ __device__ __forceinline__ void load_tile(const Tile<T, D>& dst, const T* src, i
     const int row = threadIdx.x / PIECES, col = (threadIdx.x % PIECES) * Tile<T, D>::PER;
     const char* p = reinterpret_cast<const char*>(src + (t0 + row) * st + col);
     const int64_t step = STEP * st * (int64_t)sizeof(T);
+    if (n == C) {
 #pragma unroll
-    for (int i = 0; i < C / STEP; i++) {
-        const bool in = row + i * STEP < n;
-        cp16(dst.base + dst.off(row + i * STEP, col), in ? p + i * step : reinterpret_cast<const char*>(src), in);
+        for (int i = 0; i < C / STEP; i++) cp16(dst.base + dst.off(row + i * STEP, col), p + i * step, true);
+    } else {
+#pragma unroll
+        for (int i = 0; i < C / STEP; i++) {
+            const bool in = row + i * STEP < n;
+            cp16(dst.base + dst.off(row + i * STEP, col), in ? p + i * step : reinterpret_cast<const char*>(src), in);
+        }
     }
 }
 
@@ -107,6 +112,15 @@ template <int N> __device__ __forceinline__ bool not_finite(const float (&a)[N][
     return z != 0.f;
 }
 
+// Rows g and g + 8 times f0 and f1, or zero: a product with 0 would keep what is not a number
+template <int N> __device__ __forceinline__ void weigh(float (&a)[N][4], bool in0, bool in1, float f0, float f1) {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        a[i][0] = in0 ? a[i][0] * f0 : 0.f; a[i][1] = in0 ? a[i][1] * f0 : 0.f;
+        a[i][2] = in1 ? a[i][2] * f1 : 0.f; a[i][3] = in1 ? a[i][3] * f1 : 0.f;
+    }
+}
+
 template <int N> __device__ __forceinline__ void zero(float (&a)[N][4]) {
 #pragma unroll
     for (int i = 0; i < N; i++)
@@ -114,13 +128,33 @@ template <int N> __device__ __forceinline__ void zero(float (&a)[N][4]) {
         for (int j = 0; j < 4; j++) a[i][j] = 0.f;
 }
 
-// acc (16 x 8 NB) += A (16 x K) B: A rows of one tile; B rows of another as columns, or, TR, its columns as columns
-template <typename T, int NB, int K, bool TR, typename TA, typename TB>
-__device__ __forceinline__ void product(float (&acc)[NB][4], const TA& a, int m, const TB& b, int n) {
+// Sixteen rows of a tile as the left operand of several products: bf16 keeps them in registers, fp32 reads them again
+template <typename T, int D> struct Left {
     using F = Frag<T>;
+    static constexpr bool KEPT = sizeof(T) == 2;
+    typename F::A f[KEPT ? D / F::KS : 1];
+    const Tile<T, D>& t;
+    int m;
+    __device__ __forceinline__ Left(const Tile<T, D>& tile, int row) : t(tile), m(row) {
+        if (KEPT) {
+#pragma unroll
+            for (int k = 0; k < D; k += F::KS) f[k / F::KS] = F::ldA(t, m, k);
+        }
+    }
+    __device__ __forceinline__ typename F::A get(int k) const {
+        if constexpr (KEPT) return f[k / F::KS];
+        else return F::ldA(t, m, k);
+    }
+};
+
+// acc (16 x 8 NB) = A B, B the rows of a D x D tile as columns or, TR, its columns as columns
+template <typename T, int NB, int D, bool TR>
+__device__ __forceinline__ void product(float (&acc)[NB][4], const Left<T, D>& a, const Tile<T, D>& b, int n) {
+    using F = Frag<T>;
+    zero(acc);
 #pragma unroll(Frag<T>::UNROLL)
-    for (int k = 0; k < K; k += F::KS) {
-        const typename F::A fa = F::ldA(a, m, k);
+    for (int k = 0; k < D; k += F::KS) {
+        const typename F::A fa = a.get(k);
 #pragma unroll
         for (int i = 0; i < NB; i += 2) {
             typename F::B b0, b1;
@@ -153,58 +187,72 @@ template <bool UP> struct Decay {
     }
 };
 
-// One chunk's scores: p[row][col] = (a_row . b_col) L scale for rows row0.. against all C columns (UP: a = q or do, b = k or v).
-// Blocks that L empties are skipped. pw1: the powers, one place on, so that the pairs read stand on 8 bytes.
-template <typename T, int D, int C, bool UP>
-__device__ __forceinline__ void scores(float (&p)[C / 8][4], const Tile<T, D>& a, const Tile<T, D>& b, int row0, const Cuts& cuts, const float* pw1, const Decay<UP>& dec) {
+// What a warp's rows row0..row0+15 of a chunk's L come from: the latest restart up to each row (UP) or the next one after it.
+// No restart in (j, i] means none in (j, edge] and none in (edge, i]: outside the diagonal's block the mask is a product too.
+template <bool UP> struct Mask {
+    int row0, lim0, lim1, lim;
+    float r0, r1;
+    __device__ __forceinline__ Mask(const Cuts& cuts, int row0_, const Decay<UP>& dec) : row0(row0_) {
+        const int g = (threadIdx.x & 31) >> 2, edge = UP ? row0 : row0 + 15;
+        lim0 = UP ? cuts.last_up_to(row0 + g) : cuts.next_after(row0 + g);
+        lim1 = UP ? cuts.last_up_to(row0 + g + 8) : cuts.next_after(row0 + g + 8);
+        lim = UP ? cuts.last_up_to(edge) : cuts.next_after(edge);
+        r0 = (UP ? lim0 <= edge : lim0 > edge) ? dec.row[0] : 0.f;
+        r1 = (UP ? lim1 <= edge : lim1 > edge) ? dec.row[1] : 0.f;
+    }
+    // L * scale of the rows against columns col0..col0+15. pw1: the powers, one place on, so that pairs stand on 8 bytes
+    __device__ __forceinline__ void factors(float (&f)[2][4], int col0, const float* pw1, const Decay<UP>& dec) const {
+        const int c = 2 * (threadIdx.x & 3);
+        if (col0 == row0) {
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const int at = col0 + 8 * i + c + (j & 1), l = j < 2 ? lim0 : lim1;
+                    f[i][j] = (UP ? at >= l : at < l) ? dec.diag[i][j] : 0.f;
+                }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const int col = col0 + 8 * i + c;
+                const float2 e = *reinterpret_cast<const float2*>(pw1 + (UP ? row0 - col : col - row0 - 14));
+                const float x = (UP ? col >= lim : col < lim) ? (UP ? e.y : e.x) : 0.f, y = (UP ? col + 1 >= lim : col + 1 < lim) ? (UP ? e.x : e.y) : 0.f;
+                f[i][0] = x * r0; f[i][1] = y * r0; f[i][2] = x * r1; f[i][3] = y * r1;
+            }
+        }
+    }
+};
+
+// p = (16 rows) . (rows col0..col0+15 of b) * f
+template <typename T, int D>
+__device__ __forceinline__ void block_scores(float (&p)[2][4], const Left<T, D>& a, const Tile<T, D>& b, int col0, const float (&f)[2][4]) {
     using F = Frag<T>;
     zero(p);
-#pragma unroll(Frag<T>::UNROLL)
+#pragma unroll(sizeof(T) == 2 ? 8 : 2)
     for (int k = 0; k < D; k += F::KS) {
-        const typename F::A fa = F::ldA(a, row0, k);
-#pragma unroll
-        for (int i = 0; i < C / 8; i += 2) {
-            if (UP ? 8 * i > row0 : 8 * i < row0) continue;   // 16 columns against 16 rows
-            typename F::B b0, b1;
-            F::ldB(b, 8 * i, k, b0, b1);
-            F::mma(p[i], fa, b0);
-            F::mma(p[i + 1], fa, b1);
-        }
+        const typename F::A fa = a.get(k);
+        typename F::B b0, b1;
+        F::ldB(b, col0, k, b0, b1);
+        F::mma(p[0], fa, b0);
+        F::mma(p[1], fa, b1);
     }
-    // No restart in (j, i] means none in (j, edge] and none in (edge, i]: outside the diagonal's block the mask is a product too
-    const int l = threadIdx.x & 31, g = l >> 2, c = 2 * (l & 3), edge = UP ? row0 : row0 + 15;
-    const int lim0 = UP ? cuts.last_up_to(row0 + g) : cuts.next_after(row0 + g), lim1 = UP ? cuts.last_up_to(row0 + g + 8) : cuts.next_after(row0 + g + 8);
-    const int lim = UP ? cuts.last_up_to(edge) : cuts.next_after(edge);
-    const float r0 = (UP ? lim0 <= edge : lim0 > edge) ? dec.row[0] : 0.f, r1 = (UP ? lim1 <= edge : lim1 > edge) ? dec.row[1] : 0.f;
 #pragma unroll
-    for (int i = 0; i < C / 8; i++) {
-        const int col = 8 * i + c;
-        if ((8 * i & ~15) == row0) {
+    for (int i = 0; i < 2; i++)
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const int at = col + (j & 1), lim = j < 2 ? lim0 : lim1;
-                p[i][j] = (UP ? at >= lim : at < lim) ? p[i][j] * dec.diag[i & 1][j] : 0.f;
-            }
-        } else if (UP ? 8 * i < row0 : 8 * i > row0) {
-            const float2 e = *reinterpret_cast<const float2*>(pw1 + (UP ? row0 - col : col - row0 - 14));
-            const float x = (UP ? col >= lim : col < lim) ? (UP ? e.y : e.x) : 0.f, y = (UP ? col + 1 >= lim : col + 1 < lim) ? (UP ? e.x : e.y) : 0.f;
-            p[i][0] *= x * r0; p[i][1] *= y * r0; p[i][2] *= x * r1; p[i][3] *= y * r1;
-        }
-    }
+        for (int j = 0; j < 4; j++) p[i][j] *= f[i][j];
 }
 
-// acc += p (16 x C) times rows of a tile, blocks that the scores left empty skipped
-template <typename T, int D, int C, int NB, bool UP>
-__device__ __forceinline__ void apply_scores(float (&acc)[NB][4], const float (&p)[C / 8][4], const Tile<T, D>& b, int row0, int n) {
+// acc += p (16 x 16) times rows row..row+15 of a tile, columns n..
+template <typename T, int D, int NB>
+__device__ __forceinline__ void block_apply(float (&acc)[NB][4], const float (&p)[2][4], const Tile<T, D>& b, int row, int n) {
     using F = Frag<T>;
 #pragma unroll
-    for (int ks = 0; ks < C / F::KS; ks++) {
-        if (UP ? ks * F::KS > row0 + 15 : (ks + 1) * F::KS <= row0) continue;
+    for (int ks = 0; ks < 16 / F::KS; ks++) {
         const typename F::A fa = F::chain(p, ks);
 #pragma unroll
         for (int i = 0; i < NB; i += 2) {
             typename F::B b0, b1;
-            F::template ldBt<false>(b, ks * F::KS, n + 8 * i, b0, b1);
+            F::template ldBt<false>(b, row + ks * F::KS, n + 8 * i, b0, b1);
             F::mma(acc[i], fa, b0);
             F::mma(acc[i + 1], fa, b1);
         }
@@ -364,20 +412,21 @@ __global__ void __launch_bounds__(Shape<T, D>::NT, MINB) k_attn_fwd(const FmeDec
         const int last = cuts.last_up_to(63);
         bool again = false;
         if constexpr (!LOCAL) {
-            float acc[NC / 8][4], p[C / 8][4];
-            zero(acc);
+            float acc[NC / 8][4];
+            const Left<T, D> lq(tq, row0);
             if (some) {
-                product<T, NC / 8, D, false>(acc, tq, row0, ts, col0);
+                product<T, NC / 8, D, false>(acc, lq, ts, col0);
                 const bool in0 = cuts.last_up_to(row0 + g) < 0, in1 = cuts.last_up_to(row0 + g + 8) < 0;
-                const float a0 = pw[row0 + g + 1] * A.scale, a1 = pw[row0 + g + 9] * A.scale;
-#pragma unroll
-                for (int i = 0; i < NC / 8; i++) {
-                    acc[i][0] = in0 ? acc[i][0] * a0 : 0.f; acc[i][1] = in0 ? acc[i][1] * a0 : 0.f;
-                    acc[i][2] = in1 ? acc[i][2] * a1 : 0.f; acc[i][3] = in1 ? acc[i][3] * a1 : 0.f;
-                }
+                weigh(acc, in0, in1, pw[row0 + g + 1] * A.scale, pw[row0 + g + 9] * A.scale);
+            } else zero(acc);
+            const Mask<true> mask(cuts, row0, dec);
+#pragma unroll 1
+            for (int j = 0; j <= row0; j += 16) {
+                float p[2][4], f[2][4];
+                mask.factors(f, j, pw1, dec);
+                block_scores<T, D>(p, lq, tk, j, f);
+                block_apply<T, D>(acc, p, tv, j, col0);
             }
-            scores<T, D, C, true>(p, tq, tk, row0, cuts, pw1, dec);
-            apply_scores<T, D, C, NC / 8, true>(acc, p, tv, row0, col0);
             again = __syncthreads_or(not_finite(acc));
             // q and the old state have been read by all: the q tile takes the outputs
             if (!again) store_rows<T, NC>(sm + 2 * Z::TILE + warp * Z::STAGE, acc, o, A.o.st, row0, col0, t0, cuts.n);
@@ -493,36 +542,44 @@ __global__ void __launch_bounds__(Shape<T, D>::NT, MINB) k_attn_bwd(const FmeDec
         const bool before = c > 0 || A.s_in;   // whether the state before the chunk may be other than zero
         bool again = false;
         if constexpr (!LOCAL) {
-            float acc[NC / 8][4], p[C / 8][4];
             const int r0 = row0 + g, r1 = r0 + 8;
-            const bool z0 = r0 >= last && r0 < cuts.n, z1 = r1 >= last && r1 < cuts.n;
-            const float w0 = pw[z0 ? cuts.n - 1 - r0 : 0], w1 = pw[z1 ? cuts.n - 1 - r1 : 0];
-            auto weigh = [&](bool in0, bool in1, float f0, float f1) {
-#pragma unroll
-                for (int i = 0; i < NC / 8; i++) {
-                    acc[i][0] = in0 ? acc[i][0] * f0 : 0.f; acc[i][1] = in0 ? acc[i][1] * f0 : 0.f;
-                    acc[i][2] = in1 ? acc[i][2] * f1 : 0.f; acc[i][3] = in1 ? acc[i][3] * f1 : 0.f;
+            {
+                const bool z0 = r0 >= last && r0 < cuts.n, z1 = r1 >= last && r1 < cuts.n;
+                const float w0 = pw[z0 ? cuts.n - 1 - r0 : 0], w1 = pw[z1 ? cuts.n - 1 - r1 : 0];
+                const Mask<false> mask(cuts, row0, down);
+                float av[NC / 8][4], ak[NC / 8][4];
+                const Left<T, D> lk(tk, row0), lv(tv, row0);
+                if (some) {
+                    product<T, NC / 8, D, true>(av, lk, tu, col0); weigh(av, z0, z1, w0, w1);
+                    product<T, NC / 8, D, false>(ak, lv, tu, col0); weigh(ak, z0, z1, w0, w1);
+                } else { zero(av); zero(ak); }
+#pragma unroll 1
+                for (int i = row0; i < C; i += 16) {
+                    float p[2][4], f[2][4];
+                    mask.factors(f, i, pw1, down);
+                    block_scores<T, D>(p, lk, tq, i, f);
+                    block_apply<T, D>(av, p, tg, i, col0);
+                    block_scores<T, D>(p, lv, tg, i, f);
+                    block_apply<T, D>(ak, p, tq, i, col0);
                 }
-            };
-            zero(acc);
-            if (some) { product<T, NC / 8, D, true>(acc, tk, row0, tu, col0); weigh(z0, z1, w0, w1); }
-            scores<T, D, C, false>(p, tk, tq, row0, cuts, pw1, down);
-            apply_scores<T, D, C, NC / 8, false>(acc, p, tg, row0, col0);
-            again |= not_finite(acc);
-            store_rows<T, NC>(stage, acc, dv, A.dv.st, row0, col0, t0, cuts.n);
-            zero(acc);
-            if (some) { product<T, NC / 8, D, false>(acc, tv, row0, tu, col0); weigh(z0, z1, w0, w1); }
-            scores<T, D, C, false>(p, tv, tg, row0, cuts, pw1, down);
-            apply_scores<T, D, C, NC / 8, false>(acc, p, tq, row0, col0);
-            again |= not_finite(acc);
-            store_rows<T, NC>(stage, acc, dk, A.dk.st, row0, col0, t0, cuts.n);
-            zero(acc);
-            if (before) {
-                product<T, NC / 8, D, true>(acc, tg, row0, ts, col0);
-                weigh(cuts.last_up_to(r0) < 0, cuts.last_up_to(r1) < 0, pw[r0 + 1] * A.scale, pw[r1 + 1] * A.scale);
+                again |= not_finite(av) || not_finite(ak);
+                store_rows<T, NC>(stage, av, dv, A.dv.st, row0, col0, t0, cuts.n);
+                store_rows<T, NC>(stage, ak, dk, A.dk.st, row0, col0, t0, cuts.n);
             }
-            scores<T, D, C, true>(p, tg, tv, row0, cuts, pw1, up);
-            apply_scores<T, D, C, NC / 8, true>(acc, p, tk, row0, col0);
+            const Mask<true> mask(cuts, row0, up);
+            float acc[NC / 8][4];
+            const Left<T, D> lg(tg, row0);
+            if (before) {
+                product<T, NC / 8, D, true>(acc, lg, ts, col0);
+                weigh(acc, cuts.last_up_to(r0) < 0, cuts.last_up_to(r1) < 0, pw[r0 + 1] * A.scale, pw[r1 + 1] * A.scale);
+            } else zero(acc);
+#pragma unroll 1
+            for (int j = 0; j <= row0; j += 16) {
+                float p[2][4], f[2][4];
+                mask.factors(f, j, pw1, up);
+                block_scores<T, D>(p, lg, tv, j, f);
+                block_apply<T, D>(acc, p, tk, j, col0);
+            }
             again |= not_finite(acc);
             store_rows<T, NC>(stage, acc, dq, A.dq.st, row0, col0, t0, cuts.n);
         }
