@@ -21,20 +21,91 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float
 
 namespace cg = cooperative_groups;
 
-// sigmoid by the fast exponential and division: both are off by a few units of 2^-23, as the sums around them
-__device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.f, 1.f + __expf(-z)); }
+// 1 / (1 + 2^(-z log2 e)) by the approximate exponential and reciprocal: each is off by a few units of 2^-23, as the sums around
+// it. Both of +-inf come out as limits (2^inf = inf, 1 / inf = 0).
+__device__ __forceinline__ float sigmoid(float z) {
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z * -1.44269504088896340736f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+    return r;
+}
 __device__ __forceinline__ float act_fwd(int act, float z) {
     return act == FME_ACT_SILU ? z * sigmoid(z) : act == FME_ACT_RELU ? (z < 0.f ? 0.f : z) : z;
 }
 __device__ __forceinline__ float act_bwd(int act, float z, float dy) {
-    if (act == FME_ACT_SILU) { const float s = sigmoid(z); return dy * s * (1.f + z * (1.f - s)); }
+    if (act == FME_ACT_SILU) { const float s = sigmoid(z); return dy * (s * fmaf(-z, s, 1.f + z)); }   // s (1 + z (1 - s))
     return act == FME_ACT_RELU ? (z <= 0.f ? 0.f : dy) : dy;
 }
 
 constexpr int NT = 256;
 constexpr int MAX_C = 4096;
 
-template <typename T, int VEC> struct alignas(sizeof(T) * VEC) Pack { T v[VEC]; };
+// A vector of VEC values as the words that it is loaded in: values are taken out of registers, not out of memory
+template <int BYTES> struct Words;
+template <> struct Words<16> { using type = uint4; };
+template <> struct Words<8> { using type = uint2; };
+template <> struct Words<4> { using type = uint32_t; };
+template <> struct Words<2> { using type = uint16_t; };
+template <> struct Words<1> { using type = uint8_t; };
+template <typename T, int VEC> using Pack = typename Words<(int)sizeof(T) * VEC>::type;
+__device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+__device__ __forceinline__ uint32_t word(const uint2& v, int i) { return i ? v.y : v.x; }
+__device__ __forceinline__ uint32_t word(uint32_t v, int) { return v; }
+__device__ __forceinline__ void set_word(uint4& v, int i, uint32_t x) { (i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w) = x; }
+__device__ __forceinline__ void set_word(uint2& v, int i, uint32_t x) { (i ? v.y : v.x) = x; }
+__device__ __forceinline__ void set_word(uint32_t& v, int, uint32_t x) { v = x; }
+
+// Codes by the float32 that is 2^23 + code: adding 2^23 rounds to the nearest integer, ties to even, and leaves it in the low
+// byte. Conversions between float and integer go at a quarter of that rate. (A group with NaN gets some code.)
+__device__ __forceinline__ uint32_t code_of(float x, float lo, float inv) { return __float_as_uint(__fadd_rn(__fmul_rn(__fsub_rn(x, lo), inv), 8388608.f)); }
+template <int VEC> __device__ __forceinline__ Pack<uint8_t, VEC> codes_of(const float (&x)[VEC], const float* lo, const float* inv, bool each) {
+    Pack<uint8_t, VEC> q;
+    if constexpr (VEC % 4 == 0) {
+#pragma unroll
+        for (int j = 0; j < VEC; j += 4) {
+            uint32_t c[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) c[i] = code_of(x[j + i], lo[each ? j + i : 0], inv[each ? j + i : 0]);
+            set_word(q, j / 4, __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410));
+        }
+    } else {
+        static_assert(VEC == 1, "");
+        q = (uint8_t)code_of(x[0], lo[0], inv[0]);
+    }
+    return q;
+}
+// The values of a vector as float32
+template <typename T, int VEC> __device__ __forceinline__ void floats(float (&f)[VEC], const Pack<T, VEC>& r) {
+    if constexpr (VEC == 1) {
+        if constexpr (sizeof(T) == 1) f[0] = (float)r;
+        else if constexpr (sizeof(T) == 2) f[0] = __uint_as_float((uint32_t)r << 16);
+        else f[0] = __uint_as_float(r);
+    } else {
+#pragma unroll
+        for (int j = 0; j < VEC; j++) {
+            if constexpr (sizeof(T) == 1) f[j] = __uint_as_float(__byte_perm(word(r, j / 4), 0x4b000000u, 0x7540 + (j & 3))) - 8388608.f;
+            else if constexpr (sizeof(T) == 2) f[j] = __uint_as_float(j & 1 ? word(r, j / 2) & 0xffff0000u : word(r, j / 2) << 16);
+            else f[j] = __uint_as_float(word(r, j));
+        }
+    }
+}
+template <typename T, int VEC> __device__ __forceinline__ Pack<T, VEC> packed(const float (&f)[VEC]) {
+    Pack<T, VEC> r;
+    if constexpr (VEC == 1) {
+        if constexpr (sizeof(T) == 2) r = __bfloat16_as_ushort(__float2bfloat16(f[0]));
+        else r = __float_as_uint(f[0]);
+    } else if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int j = 0; j < VEC; j += 2) {
+            const __nv_bfloat162 two = __floats2bfloat162_rn(f[j], f[j + 1]);
+            set_word(r, j / 2, *reinterpret_cast<const uint32_t*>(&two));
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < VEC; j++) set_word(r, j, __float_as_uint(f[j]));
+    }
+    return r;
+}
 
 // ---------------------------------------------------------------- samples held in shared memory
 // A sample is p * c values in a row. Threads take vectors of VEC of them, R threads form a team and R * VEC is a multiple of
@@ -214,12 +285,13 @@ __global__ void __launch_bounds__(MAX_THREADS, 2) k_norm_fwd(const FmeGroupNorm 
         if (u8) {
 #pragma unroll 4
             for (int i = t; i < count; i += P.R) {
-                const V r = tile[i];
+                float f[VEC];
+                const V r = tile[i];   // in one piece
+                floats<T, VEC>(f, r);
 #pragma unroll
                 for (int j = 0; j < VEC; j++) {
-                    const float f = to_f(r.v[j]);
                     const int s = NS == 1 ? 0 : j;
-                    v[0][s] += f; v[1][s] = fminf(v[1][s], f); v[2][s] = fmaxf(v[2][s], f);
+                    v[0][s] += f[j]; v[1][s] = fminf(v[1][s], f[j]); v[2][s] = fmaxf(v[2][s], f[j]);
                 }
             }
             group_sums<3, NS, HOW, true>(P, A.g, v, grp, team, t, red, out, 0);
@@ -229,9 +301,11 @@ __global__ void __launch_bounds__(MAX_THREADS, 2) k_norm_fwd(const FmeGroupNorm 
             for (int j = 0; j < NS; j++) s1[0][j] = 0.f;
 #pragma unroll 4
             for (int i = t; i < count; i += P.R) {
-                const V r = tile[i];
+                float f[VEC];
+                const V r = tile[i];   // in one piece
+                floats<T, VEC>(f, r);
 #pragma unroll
-                for (int j = 0; j < VEC; j++) s1[0][NS == 1 ? 0 : j] += to_f(r.v[j]);
+                for (int j = 0; j < VEC; j++) s1[0][NS == 1 ? 0 : j] += f[j];
             }
             group_sums<1, NS, HOW, false>(P, A.g, s1, grp, team, t, red, out, 0);
 #pragma unroll
@@ -241,9 +315,11 @@ __global__ void __launch_bounds__(MAX_THREADS, 2) k_norm_fwd(const FmeGroupNorm 
         for (int j = 0; j < NS; j++) { mean[j] = cnt > 0.f ? v[0][j] / cnt : 0.f; lo[j] = v[1][j]; hi[j] = v[2][j]; }
 #pragma unroll 4
         for (int i = t; i < count; i += P.R) {
+            float f[VEC];
             const V r = tile[i];
+            floats<T, VEC>(f, r);
 #pragma unroll
-            for (int j = 0; j < VEC; j++) { const int s = NS == 1 ? 0 : j; const float d = to_f(r.v[j]) - mean[s]; q[0][s] = fmaf(d, d, q[0][s]); }
+            for (int j = 0; j < VEC; j++) { const int s = NS == 1 ? 0 : j; const float d = f[j] - mean[s]; q[0][s] = fmaf(d, d, q[0][s]); }
         }
         // 3 * warps * g floats on: past what the first sums used
         group_sums<1, NS, HOW, false>(P, A.g, q, grp, team, t, HOW == WARP ? red + 3 * (blockDim.x >> 5) * A.g : red, out + 3 * pairs, 0);
@@ -303,36 +379,29 @@ __global__ void __launch_bounds__(MAX_THREADS, 2) k_norm_fwd(const FmeGroupNorm 
             }
         }
         V* y = reinterpret_cast<V*>(A.y) + n * P.nvec + v0;
+        Pack<uint8_t, VEC>* codes = reinterpret_cast<Pack<uint8_t, VEC>*>(A.codes) + n * P.nvec + v0;
+        float inv[NS];
+#pragma unroll
+        for (int j = 0; j < NS; j++) inv[j] = u8 ? code_inv(lo[j], hi[j]) : 0.f;
         by_act(A.act, [&](auto act) {
-#pragma unroll 4
-            for (int i = t; i < count; i += P.R) {
-                const V r = tile[i];
-                V o;
+            auto values = [&](auto with) {
+#pragma unroll 2
+                for (int i = t; i < count; i += P.R) {
+                    float f[VEC], o[VEC];
+                    const V r = tile[i];   // in one piece
+                floats<T, VEC>(f, r);
 #pragma unroll
-                for (int j = 0; j < VEC; j++) {
-                    const int s = NS == 1 ? 0 : j;
-                    o.v[j] = from_f<T>(act_fwd(decltype(act)::value, fmaf((to_f(r.v[j]) - mean[s]) * rstd[s], w[j], b[j])));
+                    for (int j = 0; j < VEC; j++) {
+                        const int s = NS == 1 ? 0 : j;
+                        o[j] = act_fwd(decltype(act)::value, fmaf((f[j] - mean[s]) * rstd[s], w[j], b[j]));
+                    }
+                    y[i] = packed<T, VEC>(o);
+                    if (decltype(with)::value) codes[i] = codes_of<VEC>(f, lo, inv, NS > 1);
                 }
-                y[i] = o;
-            }
+            };
+            if (u8) values(std::true_type{});
+            else values(std::false_type{});
         });
-        if (u8) {
-            float inv[NS];
-#pragma unroll
-            for (int j = 0; j < NS; j++) inv[j] = code_inv(lo[j], hi[j]);
-            Pack<uint8_t, VEC>* codes = reinterpret_cast<Pack<uint8_t, VEC>*>(A.codes) + n * P.nvec + v0;
-#pragma unroll 4
-            for (int i = t; i < count; i += P.R) {
-                const V r = tile[i];
-                Pack<uint8_t, VEC> o;
-#pragma unroll
-                for (int j = 0; j < VEC; j++) {
-                    const int s = NS == 1 ? 0 : j;   // in 0..255 by construction; a group with NaN gets some code
-                    o.v[j] = (uint8_t)__float2uint_rn(__fmul_rn(__fsub_rn(to_f(r.v[j]), lo[s]), inv[s]));
-                }
-                codes[i] = o;
-            }
-        }
     }
     if (PH == WHOLE && P.parts > 1) cg::this_cluster().barrier_wait();
 }
@@ -372,7 +441,8 @@ __global__ void __launch_bounds__(MAX_THREADS, 2) k_norm_bwd(const FmeGroupNorm 
     constexpr int NS = HOW == EACH ? VEC : 1;
     constexpr bool KEEP = sizeof(T) == 4 && PH != APPLY;
     using V = Pack<T, VEC>;
-    using X = typename std::conditional<U8, Pack<uint8_t, VEC>, V>::type;
+    using XT = typename std::conditional<U8, uint8_t, T>::type;
+    using X = Pack<XT, VEC>;
     extern __shared__ __align__(16) char sm[];
     const int pairs = P.M * A.g, team = P.M == 1 ? (threadIdx.x < P.R ? 0 : 1) : P.by_r(threadIdx.x), t = threadIdx.x - team * P.R;
     V* td = reinterpret_cast<V*>(sm + team * P.tile);      // only for team < M
@@ -415,10 +485,13 @@ __global__ void __launch_bounds__(MAX_THREADS, 2) k_norm_bwd(const FmeGroupNorm 
                 xa[j] = code_step(lo, hi) * rstd[j]; xb[j] = (lo - mean) * rstd[j];
             } else { xa[j] = rstd[j]; xb[j] = mean; }
         }
-        auto hat = [&](const X& r, int j) {
-            const int s = NS == 1 ? 0 : j;
-            if constexpr (U8) return fmaf((float)r.v[j], xa[s], xb[s]);
-            else return (to_f(r.v[j]) - xb[s]) * xa[s];
+        auto hats = [&](float (&xh)[VEC], const X r) {
+            floats<XT, VEC>(xh, r);
+#pragma unroll
+            for (int j = 0; j < VEC; j++) {
+                const int s = NS == 1 ? 0 : j;
+                xh[j] = U8 ? fmaf(xh[j], xa[s], xb[s]) : (xh[j] - xb[s]) * xa[s];
+            }
         };
         fetched();
         float v[2][NS];
@@ -428,18 +501,20 @@ __global__ void __launch_bounds__(MAX_THREADS, 2) k_norm_bwd(const FmeGroupNorm 
             by_act(A.act, [&](auto act) {
 #pragma unroll 2
                 for (int i = t; i < count; i += P.R) {
+                    float xh[VEC], dz[VEC];
                     const X r = tx[i];
-                    V g = td[i];
+                    const V g = td[i];
+                    hats(xh, r);
+                    floats<T, VEC>(dz, g);
 #pragma unroll
                     for (int j = 0; j < VEC; j++) {
                         const int s = NS == 1 ? 0 : j;
-                        const float xh = hat(r, j), dz = act_bwd(decltype(act)::value, fmaf(xh, w[j], b[j]), to_f(g.v[j]));
-                        if (KEEP) g.v[j] = from_f<T>(dz);
-                        const float wd = w[j] * dz;
-                        v[0][s] += wd; v[1][s] = fmaf(wd, xh, v[1][s]);
-                        db[j] += dz; dw[j] = fmaf(dz, xh, dw[j]);
+                        dz[j] = act_bwd(decltype(act)::value, fmaf(xh[j], w[j], b[j]), dz[j]);
+                        const float wd = w[j] * dz[j];
+                        v[0][s] += wd; v[1][s] = fmaf(wd, xh[j], v[1][s]);
+                        db[j] += dz[j]; dw[j] = fmaf(dz[j], xh[j], dw[j]);
                     }
-                    if (KEEP && decltype(act)::value != FME_ACT_NONE) td[i] = g;
+                    if (KEEP && decltype(act)::value != FME_ACT_NONE) td[i] = packed<T, VEC>(dz);
                 }
             });
             group_sums<2, NS, HOW, false>(P, A.g, v, grp, team, t, red, out, buf);
@@ -481,17 +556,18 @@ __global__ void __launch_bounds__(MAX_THREADS, 2) k_norm_bwd(const FmeGroupNorm 
             by_act(A.act, [&](auto act) {
 #pragma unroll 2
                 for (int i = t; i < count; i += P.R) {
+                    float xh[VEC], dz[VEC];
                     const X r = tx[i];
                     const V g = td[i];
-                    V o;
+                    hats(xh, r);
+                    floats<T, VEC>(dz, g);
 #pragma unroll
                     for (int j = 0; j < VEC; j++) {
                         const int s = NS == 1 ? 0 : j;
-                        const float xh = hat(r, j);
-                        const float dz = KEEP ? to_f(g.v[j]) : act_bwd(decltype(act)::value, fmaf(xh, w[j], b[j]), to_f(g.v[j]));
-                        o.v[j] = from_f<T>(rstd[s] * (fmaf(dz, w[j], -a1[s]) - xh * a2[s]));
+                        if (!KEEP) dz[j] = act_bwd(decltype(act)::value, fmaf(xh[j], w[j], b[j]), dz[j]);
+                        dz[j] = rstd[s] * fmaf(-xh[j], a2[s], fmaf(dz[j], w[j], -a1[s]));
                     }
-                    dx[i] = o;
+                    dx[i] = packed<T, VEC>(dz);
                 }
             });
         }
@@ -517,23 +593,35 @@ __global__ void __launch_bounds__(MAX_THREADS, 2) k_norm_bwd(const FmeGroupNorm 
     }
 }
 
+// The parts' sums in order, to the end of the workspace
+__global__ void __launch_bounds__(NT) k_norm_join_bwd(const FmeGroupNorm A, const int parts) {
+    const int64_t i = (int64_t)blockIdx.x * (NT / 32) + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (i >= (int64_t)A.n * A.g) return;
+    const int64_t n = i / A.g;
+    const int g = (int)(i % A.g);
+    float2 s = make_float2(0.f, 0.f);
+    const float2* src = reinterpret_cast<const float2*>(A.ws);
+    for (int r = lane; r < parts; r += 32) { const float2 f = src[(n * parts + r) * A.g + g]; s.x += f.x; s.y += f.y; }
+    for (int o = 16; o > 0; o >>= 1) { s.x += __shfl_xor_sync(0xffffffffu, s.x, o); s.y += __shfl_xor_sync(0xffffffffu, s.y, o); }
+    if (lane == 0) reinterpret_cast<float2*>(A.ws)[(int64_t)A.n * parts * A.g + i] = s;
+}
+
 // ---------------------------------------------------------------- groups in a row
 // p = 1 (tokens, heads): a (sample, group) is c / g values in a row, KV vectors for each of LG lanes of a warp. No shared
 // memory and no barrier: shuffles. A lane keeps its channels over the samples that it walks, U of them loaded at a time.
 struct Rows {
     int LG, segs, tall;   // lanes of a group; groups of a CTA at once; samples of a CTA at once (0: the groups take grid.y)
-    Div by_lg, by_g;
+    Div by_g;
     int cgv, grid, gy;
     size_t smem;
 };
-constexpr int ROW_U = 4;
-
-template <int KV> struct RowSpot {
+template <int LG> struct RowSpot {
     int lane, g, first, step;   // lane within the group, group, first sample, samples between
     bool on;
     __device__ RowSpot(const Rows& W, int G) {
-        const int seg = W.by_lg(threadIdx.x);
-        lane = threadIdx.x - seg * W.LG;
+        const int seg = threadIdx.x / LG;
+        lane = threadIdx.x % LG;
         if (W.tall) {
             const int k = W.by_g(seg);
             g = seg - k * G;
@@ -548,174 +636,176 @@ template <int KV> struct RowSpot {
         }
     }
 };
-__device__ __forceinline__ float lanes_sum(float x, int LG) {
-    for (int o = LG >> 1; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+template <int LG> __device__ __forceinline__ float lanes_sum(float x) {
+#pragma unroll
+    for (int o = LG / 2; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
     return x;
 }
+// samples loaded at a time: four vectors a lane (backward: of x and of dy two each)
+template <int KV> __host__ __device__ constexpr int rows_at_once(bool bwd) { return KV == 1 ? (bwd ? 2 : 4) : KV == 2 && !bwd ? 2 : 1; }
 
-template <typename T, int VEC, int KV>
-__global__ void __launch_bounds__(NT) k_norm_rows_fwd(const FmeGroupNorm A, const __grid_constant__ Rows W) {
+template <typename T, int VEC, int KV, int LG, bool U8>
+__global__ void __launch_bounds__(NT, KV == 1 ? 4 : 2) k_norm_rows_fwd(const FmeGroupNorm A, const __grid_constant__ Rows W) {
     using V = Pack<T, VEC>;
-    const RowSpot<KV> S(W, A.g);
+    constexpr int U = rows_at_once<KV>(false);
+    const RowSpot<LG> S(W, A.g);
     const int cgr = W.cgv * VEC;
-    const bool u8 = A.codes != nullptr;
     const float inv_m = 1.f / (float)cgr;
     bool has[KV];
     float w[KV][VEC], b[KV][VEC];
 #pragma unroll
     for (int k = 0; k < KV; k++) {
-        has[k] = S.on && S.lane + k * W.LG < W.cgv;
+        has[k] = S.on && S.lane + k * LG < W.cgv;
 #pragma unroll
         for (int j = 0; j < VEC; j++) {
-            const int c = S.g * cgr + (S.lane + k * W.LG) * VEC + j;
+            const int c = S.g * cgr + (S.lane + k * LG) * VEC + j;
             w[k][j] = has[k] && A.w ? __ldg(A.w + c) : 1.f;
             b[k][j] = has[k] && A.b ? __ldg(A.b + c) : 0.f;
         }
     }
-    for (int64_t base = 0; base < A.n; base += (int64_t)ROW_U * S.step) {   // the same trips for all lanes: shuffles
-        V x[ROW_U][KV];
+    const T* x0 = (const T*)A.x + S.first * A.x_sn + S.g * cgr + S.lane * VEC;
+    const int64_t xs = S.step * A.x_sn, ys = (int64_t)S.step * A.c;
+    int64_t at = (int64_t)S.first * A.c + S.g * cgr + S.lane * VEC, ng = (int64_t)S.first * A.g + S.g;
+    for (int64_t n = S.first, base = 0; base < A.n; base += (int64_t)U * S.step) {   // the same trips for all lanes: shuffles
+        V x[U][KV];
 #pragma unroll
-        for (int u = 0; u < ROW_U; u++) {
-            const int64_t n = base + (int64_t)u * S.step + S.first;
+        for (int u = 0; u < U; u++)
 #pragma unroll
             for (int k = 0; k < KV; k++)
-                if (has[k] && n < A.n) x[u][k] = reinterpret_cast<const V*>((const T*)A.x + n * A.x_sn + S.g * cgr)[S.lane + k * W.LG];
-        }
+                if (has[k] && n + u * S.step < A.n) x[u][k] = *reinterpret_cast<const V*>(x0 + u * xs + k * LG * VEC);
 #pragma unroll
-        for (int u = 0; u < ROW_U; u++) {
-            const int64_t n = base + (int64_t)u * S.step + S.first;
+        for (int u = 0; u < U; u++) {
             const bool ok = n < A.n;
-            float s = 0.f, lo = INFINITY, hi = -INFINITY, q = 0.f;
+            float f[KV][VEC], s = 0.f, lo = INFINITY, hi = -INFINITY, q = 0.f;
 #pragma unroll
-            for (int k = 0; k < KV; k++)
-                if (has[k] && ok) {
+            for (int k = 0; k < KV; k++) {
+                floats<T, VEC>(f[k], x[u][k]);
+                if (has[k]) {
 #pragma unroll
-                    for (int j = 0; j < VEC; j++) { const float f = to_f(x[u][k].v[j]); s += f; if (u8) { lo = fminf(lo, f); hi = fmaxf(hi, f); } }
+                    for (int j = 0; j < VEC; j++) { s += f[k][j]; if (U8) { lo = fminf(lo, f[k][j]); hi = fmaxf(hi, f[k][j]); } }
                 }
-            s = lanes_sum(s, W.LG);
-            if (u8) for (int o = W.LG >> 1; o > 0; o >>= 1) { lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o)); hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o)); }
+            }
+            s = lanes_sum<LG>(s);
+            if (U8) {
+#pragma unroll
+                for (int o = LG / 2; o > 0; o >>= 1) { lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o)); hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o)); }
+            }
             const float mean = s * inv_m;
 #pragma unroll
             for (int k = 0; k < KV; k++)
-                if (has[k] && ok) {
+                if (has[k]) {
 #pragma unroll
-                    for (int j = 0; j < VEC; j++) { const float d = to_f(x[u][k].v[j]) - mean; q = fmaf(d, d, q); }
+                    for (int j = 0; j < VEC; j++) { const float d = f[k][j] - mean; q = fmaf(d, d, q); }
                 }
-            q = lanes_sum(q, W.LG);
+            q = lanes_sum<LG>(q);
             const float rstd = __frsqrt_rn(fmaf(q, inv_m, A.eps));
-            if (!ok || !S.on) continue;
-            if (A.mean && S.lane == 0) {
-                const int64_t ng = n * A.g + S.g;
-                A.mean[ng] = mean; A.rstd[ng] = rstd;
-                if (u8) { A.lo[ng] = lo; A.hi[ng] = hi; }
-            }
-            const float inv = u8 ? code_inv(lo, hi) : 0.f;
-            const int64_t at = (n * A.c + S.g * cgr) / VEC + S.lane;
-            by_act(A.act, [&](auto act) {
+            if (ok && S.on) {
+                if (A.mean && S.lane == 0) {
+                    A.mean[ng] = mean; A.rstd[ng] = rstd;
+                    if (U8) { A.lo[ng] = lo; A.hi[ng] = hi; }
+                }
+                const float inv = U8 ? code_inv(lo, hi) : 0.f;
 #pragma unroll
                 for (int k = 0; k < KV; k++)
                     if (has[k]) {
-                        V y;
+                        if (U8) *reinterpret_cast<Pack<uint8_t, VEC>*>(A.codes + at + k * LG * VEC) = codes_of<VEC>(f[k], &lo, &inv, false);
+                        by_act(A.act, [&](auto act) {
+                            float y[VEC];
 #pragma unroll
-                        for (int j = 0; j < VEC; j++) y.v[j] = from_f<T>(act_fwd(decltype(act)::value, fmaf((to_f(x[u][k].v[j]) - mean) * rstd, w[k][j], b[k][j])));
-                        reinterpret_cast<V*>(A.y)[at + k * W.LG] = y;
-                    }
-            });
-            if (u8) {
-#pragma unroll
-                for (int k = 0; k < KV; k++)
-                    if (has[k]) {
-                        Pack<uint8_t, VEC> y;
-#pragma unroll
-                        for (int j = 0; j < VEC; j++) y.v[j] = (uint8_t)__float2uint_rn(__fmul_rn(__fsub_rn(to_f(x[u][k].v[j]), lo), inv));
-                        reinterpret_cast<Pack<uint8_t, VEC>*>(A.codes)[at + k * W.LG] = y;
+                            for (int j = 0; j < VEC; j++) y[j] = act_fwd(decltype(act)::value, fmaf((f[k][j] - mean) * rstd, w[k][j], b[k][j]));
+                            *reinterpret_cast<V*>((T*)A.y + at + k * LG * VEC) = packed<T, VEC>(y);
+                        });
                     }
             }
+            n += S.step; at += ys; ng += (int64_t)S.step * A.g; x0 += xs;
         }
     }
 }
 
-template <typename T, int VEC, int KV, bool U8>
-__global__ void __launch_bounds__(NT) k_norm_rows_bwd(const FmeGroupNorm A, const __grid_constant__ Rows W) {
+template <typename T, int VEC, int KV, int LG, bool U8>
+__global__ void __launch_bounds__(NT, KV == 1 ? 3 : KV == 2 ? 2 : 1) k_norm_rows_bwd(const FmeGroupNorm A, const __grid_constant__ Rows W) {
     using V = Pack<T, VEC>;
-    using X = typename std::conditional<U8, Pack<uint8_t, VEC>, V>::type;
-    constexpr int U = KV == 1 ? ROW_U : KV == 2 ? 2 : 1;
+    using XT = typename std::conditional<U8, uint8_t, T>::type;
+    using X = Pack<XT, VEC>;
+    constexpr int U = rows_at_once<KV>(true);
     extern __shared__ float rw[];
-    const RowSpot<KV> S(W, A.g);
+    const RowSpot<LG> S(W, A.g);
     const int cgr = W.cgv * VEC;
     const float inv_m = 1.f / (float)cgr;
     bool has[KV];
     float w[KV][VEC], b[KV][VEC], dw[KV][VEC], db[KV][VEC];
 #pragma unroll
     for (int k = 0; k < KV; k++) {
-        has[k] = S.on && S.lane + k * W.LG < W.cgv;
+        has[k] = S.on && S.lane + k * LG < W.cgv;
 #pragma unroll
         for (int j = 0; j < VEC; j++) {
-            const int c = S.g * cgr + (S.lane + k * W.LG) * VEC + j;
+            const int c = S.g * cgr + (S.lane + k * LG) * VEC + j;
             w[k][j] = has[k] && A.w ? __ldg(A.w + c) : 1.f;
-            b[k][j] = has[k] && A.b ? __ldg(A.b + c) : 0.f;
+            b[k][j] = has[k] && A.b && A.act != FME_ACT_NONE ? __ldg(A.b + c) : 0.f;   // without an activation b is not used
             dw[k][j] = db[k][j] = 0.f;
         }
     }
-    for (int64_t base = 0; base < A.n; base += (int64_t)U * S.step) {
+    const int col = S.g * cgr + S.lane * VEC;
+    const T *x0 = (const T*)A.x + S.first * A.x_sn + col, *g0 = (const T*)A.dy + S.first * A.dy_sn + col;
+    const int64_t xs = S.step * A.x_sn, gs = S.step * A.dy_sn, ys = (int64_t)S.step * A.c;
+    int64_t at = (int64_t)S.first * A.c + col, ng = (int64_t)S.first * A.g + S.g;
+    for (int64_t n = S.first, base = 0; base < A.n; base += (int64_t)U * S.step) {
         V g[U][KV];
         X x[U][KV];
         float mean[U], rstd[U], lo[U], hi[U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const int64_t n = base + (int64_t)u * S.step + S.first, at = (n * A.c + S.g * cgr) / VEC + S.lane, ng = n * A.g + S.g;
-            const bool ok = S.on && n < A.n;
+            const bool ok = S.on && n + u * S.step < A.n;
 #pragma unroll
             for (int k = 0; k < KV; k++)
                 if (has[k] && ok) {
-                    if constexpr (U8) x[u][k] = reinterpret_cast<const X*>(A.codes)[at + k * W.LG];
-                    else x[u][k] = reinterpret_cast<const X*>((const T*)A.x + n * A.x_sn + S.g * cgr)[S.lane + k * W.LG];
-                    g[u][k] = reinterpret_cast<const V*>((const T*)A.dy + n * A.dy_sn + S.g * cgr)[S.lane + k * W.LG];
+                    if constexpr (U8) x[u][k] = *reinterpret_cast<const X*>(A.codes + at + u * ys + k * LG * VEC);
+                    else x[u][k] = *reinterpret_cast<const X*>(x0 + u * xs + k * LG * VEC);
+                    g[u][k] = *reinterpret_cast<const V*>(g0 + u * gs + k * LG * VEC);
                 }
-            mean[u] = ok ? __ldg(A.mean + ng) : 0.f;
-            rstd[u] = ok ? __ldg(A.rstd + ng) : 0.f;
-            lo[u] = U8 && ok ? __ldg(A.lo + ng) : 0.f;
-            hi[u] = U8 && ok ? __ldg(A.hi + ng) : 0.f;
+            const int64_t i = ng + (int64_t)u * S.step * A.g;
+            mean[u] = ok ? __ldg(A.mean + i) : 0.f;
+            rstd[u] = ok ? __ldg(A.rstd + i) : 0.f;
+            lo[u] = U8 && ok ? __ldg(A.lo + i) : 0.f;
+            hi[u] = U8 && ok ? __ldg(A.hi + i) : 0.f;
         }
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const int64_t n = base + (int64_t)u * S.step + S.first;
             const bool ok = n < A.n;
-            const float step = U8 ? code_step(lo[u], hi[u]) : 0.f;
-            auto hat = [&](int k, int j) {
-                if constexpr (U8) return fmaf((float)x[u][k].v[j], step * rstd[u], (lo[u] - mean[u]) * rstd[u]);
-                else return (to_f(x[u][k].v[j]) - mean[u]) * rstd[u];
-            };
+            const float xa = U8 ? code_step(lo[u], hi[u]) * rstd[u] : rstd[u], xb = U8 ? (lo[u] - mean[u]) * rstd[u] : mean[u];
+            float xh[KV][VEC], dz[KV][VEC], s1 = 0.f, s2 = 0.f;
+#pragma unroll
+            for (int k = 0; k < KV; k++) {
+                floats<XT, VEC>(xh[k], x[u][k]);
+                floats<T, VEC>(dz[k], g[u][k]);
+#pragma unroll
+                for (int j = 0; j < VEC; j++) xh[k][j] = U8 ? fmaf(xh[k][j], xa, xb) : (xh[k][j] - xb) * xa;
+            }
             by_act(A.act, [&](auto act) {
-                float s1 = 0.f, s2 = 0.f;
 #pragma unroll
                 for (int k = 0; k < KV; k++)
-                    if (has[k] && ok) {
 #pragma unroll
-                        for (int j = 0; j < VEC; j++) {
-                            const float xh = hat(k, j), dz = act_bwd(decltype(act)::value, fmaf(xh, w[k][j], b[k][j]), to_f(g[u][k].v[j]));
-                            if (sizeof(T) == 4) g[u][k].v[j] = from_f<T>(dz);
-                            const float wd = w[k][j] * dz;
-                            s1 += wd; s2 = fmaf(wd, xh, s2);
-                            db[k][j] += dz; dw[k][j] = fmaf(dz, xh, dw[k][j]);
-                        }
-                    }
-                const float a1 = lanes_sum(s1, W.LG) * inv_m, a2 = lanes_sum(s2, W.LG) * inv_m;
-                if (!ok) return;
-                const int64_t at = (n * A.c + S.g * cgr) / VEC + S.lane;
-#pragma unroll
-                for (int k = 0; k < KV; k++)
-                    if (has[k]) {
-                        V dx;
-#pragma unroll
-                        for (int j = 0; j < VEC; j++) {
-                            const float xh = hat(k, j);
-                            const float dz = sizeof(T) == 4 ? to_f(g[u][k].v[j]) : act_bwd(decltype(act)::value, fmaf(xh, w[k][j], b[k][j]), to_f(g[u][k].v[j]));
-                            dx.v[j] = from_f<T>(rstd[u] * (fmaf(dz, w[k][j], -a1) - xh * a2));
-                        }
-                        reinterpret_cast<V*>(A.dx)[at + k * W.LG] = dx;
-                    }
+                    for (int j = 0; j < VEC; j++) dz[k][j] = act_bwd(decltype(act)::value, fmaf(xh[k][j], w[k][j], b[k][j]), dz[k][j]);
             });
+#pragma unroll
+            for (int k = 0; k < KV; k++)
+                if (has[k] && ok) {
+#pragma unroll
+                    for (int j = 0; j < VEC; j++) {
+                        const float wd = w[k][j] * dz[k][j];
+                        s1 += wd; s2 = fmaf(wd, xh[k][j], s2);
+                        db[k][j] += dz[k][j]; dw[k][j] = fmaf(dz[k][j], xh[k][j], dw[k][j]);
+                    }
+                }
+            const float a1 = lanes_sum<LG>(s1) * inv_m, a2 = lanes_sum<LG>(s2) * inv_m;
+#pragma unroll
+            for (int k = 0; k < KV; k++)
+                if (has[k] && ok) {
+#pragma unroll
+                    for (int j = 0; j < VEC; j++) dz[k][j] = rstd[u] * fmaf(-xh[k][j], a2, fmaf(dz[k][j], w[k][j], -a1));
+                    *reinterpret_cast<V*>((T*)A.dx + at + k * LG * VEC) = packed<T, VEC>(dz[k]);
+                }
+            n += S.step; at += ys; ng += (int64_t)S.step * A.g; x0 += xs; g0 += gs;
         }
     }
     if (!A.dw) return;
@@ -723,17 +813,15 @@ __global__ void __launch_bounds__(NT) k_norm_rows_bwd(const FmeGroupNorm A, cons
     float* row = (float*)A.ws + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 2 * A.c;
     const int tall = W.tall ? W.tall : 1, k0 = W.tall ? (S.first - (int)blockIdx.x * W.tall) : 0;
     const int cols = W.tall ? A.c : min(W.segs, A.g - (int)blockIdx.y * W.segs) * cgr, c0 = W.tall ? 0 : blockIdx.y * W.segs * cgr;
-    if (S.on) {
 #pragma unroll
-        for (int k = 0; k < KV; k++)
-            if (has[k]) {
+    for (int k = 0; k < KV; k++)
+        if (has[k]) {
 #pragma unroll
-                for (int j = 0; j < VEC; j++) {
-                    const int c = S.g * cgr + (S.lane + k * W.LG) * VEC + j - c0;
-                    rw[k0 * cols + c] = dw[k][j]; rw[(tall + k0) * cols + c] = db[k][j];
-                }
+            for (int j = 0; j < VEC; j++) {
+                const int c = S.g * cgr + (S.lane + k * LG) * VEC + j - c0;
+                rw[k0 * cols + c] = dw[k][j]; rw[(tall + k0) * cols + c] = db[k][j];
             }
-    }
+        }
     __syncthreads();
     for (int i = threadIdx.x; i < 2 * A.c; i += NT) {
         const int c = (i < A.c ? i : i - A.c) - c0;
@@ -742,19 +830,6 @@ __global__ void __launch_bounds__(NT) k_norm_rows_bwd(const FmeGroupNorm A, cons
             for (int k = 0; k < tall; k++) s += rw[((i < A.c ? 0 : tall) + k) * cols + c];
         row[i] = s;
     }
-}
-
-__global__ void __launch_bounds__(NT) k_norm_join_bwd(const FmeGroupNorm A, const int parts) {
-    const int64_t i = (int64_t)blockIdx.x * (NT / 32) + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (i >= (int64_t)A.n * A.g) return;
-    const int64_t n = i / A.g;
-    const int g = (int)(i % A.g);
-    float2 s = make_float2(0.f, 0.f);
-    const float2* src = reinterpret_cast<const float2*>(A.ws);
-    for (int r = lane; r < parts; r += 32) { const float2 f = src[(n * parts + r) * A.g + g]; s.x += f.x; s.y += f.y; }
-    for (int o = 16; o > 0; o >>= 1) { s.x += __shfl_xor_sync(0xffffffffu, s.x, o); s.y += __shfl_xor_sync(0xffffffffu, s.y, o); }
-    if (lane == 0) reinterpret_cast<float2*>(A.ws)[(int64_t)A.n * parts * A.g + i] = s;
 }
 
 // ---------------------------------------------------------------- many channels of an odd number
@@ -866,8 +941,18 @@ __global__ void __launch_bounds__(1024) k_norm_params(const float* __restrict__ 
     __shared__ float sm[32][33];
     const int i = blockIdx.x * 32 + threadIdx.x;
     float s = 0.f;
-    if (i < 2 * c)
-        for (int r = threadIdx.y; r < rows; r += 32) s += ws[(int64_t)r * 2 * c + i];
+    if (i < 2 * c) {
+        const float* p = ws + i;
+        int r = threadIdx.y;
+        for (; r + 7 * 32 < rows; r += 8 * 32) {
+            float x[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) x[k] = p[(int64_t)(r + k * 32) * 2 * c];
+#pragma unroll
+            for (int k = 0; k < 8; k++) s += x[k];
+        }
+        for (; r < rows; r += 32) s += p[(int64_t)r * 2 * c];
+    }
     sm[threadIdx.y][threadIdx.x] = s;
     __syncthreads();
     s = sm[threadIdx.x][threadIdx.y];
@@ -915,11 +1000,10 @@ bool make_rows(const FmeGroupNorm& a, bool bwd, Rows* W, int* kv) {
     W->segs = NT / W->LG;
     W->tall = W->segs / a.g;
     W->gy = W->tall ? 1 : (a.g + W->segs - 1) / W->segs;
-    W->by_lg = divisor(W->LG);
     W->by_g = divisor(a.g);
     const int at_once = W->tall ? W->tall : 1;
-    const int64_t need = ((int64_t)a.n + (int64_t)at_once * (bwd ? 1 : ROW_U) - 1) / ((int64_t)at_once * (bwd ? 1 : ROW_U)), most = SMS * 8 / W->gy + 1;
-    W->grid = (int)(need < most ? need : most);
+    const int64_t need = ((int64_t)a.n + at_once - 1) / at_once, most = (int64_t)SMS * (*kv == 1 ? (bwd ? 3 : 4) : *kv == 2 || !bwd ? 2 : 1) / W->gy + 1;
+    W->grid = (int)(need < most ? need : most);   // as many CTAs as the GPU holds
     if (W->grid < 1) W->grid = 1;
     W->smem = bwd ? (size_t)8 * (W->tall ? W->tall * a.c : W->segs * cgr) : 0;
     return true;
@@ -957,9 +1041,11 @@ bool make_plan(const FmeGroupNorm& a, bool bwd, Plan* P) {
     const bool busy = (int64_t)a.n * parts >= 4 * SMS;
     int64_t r = (P->chunk + (busy ? 8 : 2) - 1) / (busy ? 8 : 2);
     if (r < 32) r = P->chunk < 32 ? P->chunk : 32;
-    if (r > (busy ? 256 : 512)) r = busy ? 256 : 512;
-    P->R = (int)up(r, P->how == WARP ? 32 : per);
-    if (P->R > MAX_THREADS) P->R = MAX_THREADS / per * per;
+    // (64 registers a thread: four CTAs of 256, five of 192; where clusters have to fit beside each other, five)
+    const int unit = P->how == WARP ? 32 : per, top = busy ? (parts > 1 ? 192 : 256) : MAX_THREADS;
+    if (r > top) r = top;
+    P->R = (int)up(r, unit);
+    if (P->R > top) P->R = top / unit > 0 ? top / unit * unit : unit;
     P->M = 1;
     P->tile = (int)up((int64_t)P->chunk * bpv, 16);
     if (parts == 1 && P->R <= 128) {
@@ -1040,18 +1126,23 @@ template <typename T> int run_fwd(const FmeGroupNorm& a, const Plan& P, cudaStre
     return P.how == ONE ? run_fwd<T, full, ONE>(a, P, st) : run_fwd<T, full, EACH>(a, P, st);
 }
 
-template <typename T> int run_rows_fwd(const FmeGroupNorm& a, const Rows& W, int kv, cudaStream_t st) {
+template <typename T, bool U8, bool BWD, int KV, int LG> auto rows_kernel() {
     constexpr int full = 16 / sizeof(T);
-    auto kernel = kv == 1 ? k_norm_rows_fwd<T, full, 1> : kv == 2 ? k_norm_rows_fwd<T, full, 2> : k_norm_rows_fwd<T, full, 4>;
-    kernel<<<dim3(W.grid, W.gy), NT, 0, st>>>(a, W);
-    return launch_status("fme_group_norm_fwd");
+    if constexpr (BWD) return &k_norm_rows_bwd<T, full, KV, LG, U8>;
+    else return &k_norm_rows_fwd<T, full, KV, LG, U8>;
 }
-template <typename T, bool U8> int run_rows_bwd(const FmeGroupNorm& a, const Rows& W, int kv, cudaStream_t st) {
-    constexpr int full = 16 / sizeof(T);
-    auto kernel = kv == 1 ? k_norm_rows_bwd<T, full, 1, U8> : kv == 2 ? k_norm_rows_bwd<T, full, 2, U8> : k_norm_rows_bwd<T, full, 4, U8>;
+template <typename T, bool U8, bool BWD> int run_rows(const FmeGroupNorm& a, const Rows& W, int kv, cudaStream_t st) {
+    auto kernel = rows_kernel<T, U8, BWD, 4, 32>();
+    if (kv == 2) kernel = rows_kernel<T, U8, BWD, 2, 32>();
+    if (kv == 1) kernel = W.LG == 1 ? rows_kernel<T, U8, BWD, 1, 1>() : W.LG == 2 ? rows_kernel<T, U8, BWD, 1, 2>() : W.LG == 4 ? rows_kernel<T, U8, BWD, 1, 4>()
+                        : W.LG == 8 ? rows_kernel<T, U8, BWD, 1, 8>() : W.LG == 16 ? rows_kernel<T, U8, BWD, 1, 16>() : rows_kernel<T, U8, BWD, 1, 32>();
     if (W.smem > 48 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)W.smem);
     kernel<<<dim3(W.grid, W.gy), NT, W.smem, st>>>(a, W);
-    return launch_status("fme_group_norm_bwd");
+    return launch_status(BWD ? "fme_group_norm_bwd" : "fme_group_norm_fwd");
+}
+template <bool BWD> int run_rows(const FmeGroupNorm& a, const Rows& W, int kv, cudaStream_t st) {
+    if (a.dtype == FME_F32) return a.codes ? run_rows<float, true, BWD>(a, W, kv, st) : run_rows<float, false, BWD>(a, W, kv, st);
+    return a.codes ? run_rows<__nv_bfloat16, true, BWD>(a, W, kv, st) : run_rows<__nv_bfloat16, false, BWD>(a, W, kv, st);
 }
 
 constexpr int WIDE_GRID = 592;
@@ -1091,7 +1182,7 @@ int fme_group_norm_fwd(const FmeGroupNorm* a, void* stream) {
     Plan P;
     Rows W;
     int kv;
-    if (make_rows(*a, false, &W, &kv)) return a->dtype == FME_F32 ? run_rows_fwd<float>(*a, W, kv, st) : run_rows_fwd<__nv_bfloat16>(*a, W, kv, st);
+    if (make_rows(*a, false, &W, &kv)) return run_rows<false>(*a, W, kv, st);
     if (!make_plan(*a, false, &P)) {
         const size_t smem = (size_t)3 * a->c * 4;
         const int grid = a->n < WIDE_GRID ? a->n : WIDE_GRID;
@@ -1124,8 +1215,7 @@ int fme_group_norm_bwd(const FmeGroupNorm* a, void* stream) {
     const bool u8 = a->codes != nullptr;
     if (make_rows(*a, true, &W, &kv)) {
         rows = W.grid * W.gy;
-        if (a->dtype == FME_F32) rc = u8 ? run_rows_bwd<float, true>(*a, W, kv, st) : run_rows_bwd<float, false>(*a, W, kv, st);
-        else rc = u8 ? run_rows_bwd<__nv_bfloat16, true>(*a, W, kv, st) : run_rows_bwd<__nv_bfloat16, false>(*a, W, kv, st);
+        rc = run_rows<true>(*a, W, kv, st);
     } else if (!make_plan(*a, true, &P)) {
         const size_t smem = (size_t)4 * a->c * 4;
         auto kernel = a->dtype == FME_F32 ? k_norm_wide_bwd<float> : k_norm_wide_bwd<__nv_bfloat16>;
