@@ -223,7 +223,7 @@ struct Moments {
     }
 };
 
-__device__ __forceinline__ float rstd_of(float m2, float m, float eps) { return __frsqrt_rn(m2 / m + eps); }
+__device__ __forceinline__ float rstd_of(float m2, float m, float eps) { return rsqrtf(m2 / m + eps); }
 __device__ __forceinline__ float code_inv(float lo, float hi) { return hi > lo ? __fmul_rn(__frcp_rn(__fsub_rn(hi, lo)), 255.f) : 0.f; }
 __device__ __forceinline__ float code_step(float lo, float hi) { return __fdiv_rn(__fsub_rn(hi, lo), 255.f); }
 
@@ -641,13 +641,13 @@ template <int LG> __device__ __forceinline__ float lanes_sum(float x) {
     for (int o = LG / 2; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
     return x;
 }
-// samples loaded at a time: four vectors a lane (backward: of x and of dy two each)
-template <int KV> __host__ __device__ constexpr int rows_at_once(bool bwd) { return KV == 1 ? (bwd ? 2 : 4) : KV == 2 && !bwd ? 2 : 1; }
+// samples on their way at a time: four vectors a lane (backward: of x and of dy each)
+template <int KV> __host__ __device__ constexpr int rows_at_once() { return KV == 1 ? 4 : KV == 2 ? 2 : 1; }
 
 template <typename T, int VEC, int KV, int LG, bool U8>
 __global__ void __launch_bounds__(NT, KV == 1 ? 4 : 2) k_norm_rows_fwd(const FmeGroupNorm A, const __grid_constant__ Rows W) {
     using V = Pack<T, VEC>;
-    constexpr int U = rows_at_once<KV>(false);
+    constexpr int U = rows_at_once<KV>();
     const RowSpot<LG> S(W, A.g);
     const int cgr = W.cgv * VEC;
     const float inv_m = 1.f / (float)cgr;
@@ -666,13 +666,15 @@ __global__ void __launch_bounds__(NT, KV == 1 ? 4 : 2) k_norm_rows_fwd(const Fme
     const T* x0 = (const T*)A.x + S.first * A.x_sn + S.g * cgr + S.lane * VEC;
     const int64_t xs = S.step * A.x_sn, ys = (int64_t)S.step * A.c;
     int64_t at = (int64_t)S.first * A.c + S.g * cgr + S.lane * VEC, ng = (int64_t)S.first * A.g + S.g;
+    V x[U][KV];
+    auto load = [&](int u, int64_t n, const T* p) {
+#pragma unroll
+        for (int k = 0; k < KV; k++)
+            if (has[k] && n < A.n) x[u][k] = *reinterpret_cast<const V*>(p + k * LG * VEC);
+    };
+#pragma unroll
+    for (int u = 0; u < U; u++) load(u, S.first + (int64_t)u * S.step, x0 + u * xs);
     for (int64_t n = S.first, base = 0; base < A.n; base += (int64_t)U * S.step) {   // the same trips for all lanes: shuffles
-        V x[U][KV];
-#pragma unroll
-        for (int u = 0; u < U; u++)
-#pragma unroll
-            for (int k = 0; k < KV; k++)
-                if (has[k] && n + u * S.step < A.n) x[u][k] = *reinterpret_cast<const V*>(x0 + u * xs + k * LG * VEC);
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const bool ok = n < A.n;
@@ -685,37 +687,36 @@ __global__ void __launch_bounds__(NT, KV == 1 ? 4 : 2) k_norm_rows_fwd(const Fme
                     for (int j = 0; j < VEC; j++) { s += f[k][j]; if (U8) { lo = fminf(lo, f[k][j]); hi = fmaxf(hi, f[k][j]); } }
                 }
             }
+            load(u, n + (int64_t)U * S.step, x0 + U * xs);   // on its way while the next samples are computed
             s = lanes_sum<LG>(s);
             if (U8) {
 #pragma unroll
                 for (int o = LG / 2; o > 0; o >>= 1) { lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o)); hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o)); }
             }
             const float mean = s * inv_m;
+            const float inv = U8 ? code_inv(lo, hi) : 0.f;
 #pragma unroll
             for (int k = 0; k < KV; k++)
                 if (has[k]) {
+                    if (U8 && ok) *reinterpret_cast<Pack<uint8_t, VEC>*>(A.codes + at + k * LG * VEC) = codes_of<VEC>(f[k], &lo, &inv, false);
 #pragma unroll
-                    for (int j = 0; j < VEC; j++) { const float d = f[k][j] - mean; q = fmaf(d, d, q); }
+                    for (int j = 0; j < VEC; j++) { f[k][j] -= mean; q = fmaf(f[k][j], f[k][j], q); }
                 }
-            q = lanes_sum<LG>(q);
-            const float rstd = __frsqrt_rn(fmaf(q, inv_m, A.eps));
+            const float rstd = rsqrtf(fmaf(lanes_sum<LG>(q), inv_m, A.eps));
             if (ok && S.on) {
                 if (A.mean && S.lane == 0) {
                     A.mean[ng] = mean; A.rstd[ng] = rstd;
                     if (U8) { A.lo[ng] = lo; A.hi[ng] = hi; }
                 }
-                const float inv = U8 ? code_inv(lo, hi) : 0.f;
+                by_act(A.act, [&](auto act) {
 #pragma unroll
-                for (int k = 0; k < KV; k++)
-                    if (has[k]) {
-                        if (U8) *reinterpret_cast<Pack<uint8_t, VEC>*>(A.codes + at + k * LG * VEC) = codes_of<VEC>(f[k], &lo, &inv, false);
-                        by_act(A.act, [&](auto act) {
-                            float y[VEC];
+                    for (int k = 0; k < KV; k++)
+                        if (has[k]) {
 #pragma unroll
-                            for (int j = 0; j < VEC; j++) y[j] = act_fwd(decltype(act)::value, fmaf((f[k][j] - mean) * rstd, w[k][j], b[k][j]));
-                            *reinterpret_cast<V*>((T*)A.y + at + k * LG * VEC) = packed<T, VEC>(y);
-                        });
-                    }
+                            for (int j = 0; j < VEC; j++) f[k][j] = act_fwd(decltype(act)::value, fmaf(f[k][j] * rstd, w[k][j], b[k][j]));
+                            *reinterpret_cast<V*>((T*)A.y + at + k * LG * VEC) = packed<T, VEC>(f[k]);
+                        }
+                });
             }
             n += S.step; at += ys; ng += (int64_t)S.step * A.g; x0 += xs;
         }
@@ -723,11 +724,11 @@ __global__ void __launch_bounds__(NT, KV == 1 ? 4 : 2) k_norm_rows_fwd(const Fme
 }
 
 template <typename T, int VEC, int KV, int LG, bool U8>
-__global__ void __launch_bounds__(NT, KV == 1 ? 3 : KV == 2 ? 2 : 1) k_norm_rows_bwd(const FmeGroupNorm A, const __grid_constant__ Rows W) {
+__global__ void __launch_bounds__(NT, KV == 4 ? 1 : 2) k_norm_rows_bwd(const FmeGroupNorm A, const __grid_constant__ Rows W) {
     using V = Pack<T, VEC>;
     using XT = typename std::conditional<U8, uint8_t, T>::type;
     using X = Pack<XT, VEC>;
-    constexpr int U = rows_at_once<KV>(true);
+    constexpr int U = rows_at_once<KV>();
     extern __shared__ float rw[];
     const RowSpot<LG> S(W, A.g);
     const int cgr = W.cgv * VEC;
@@ -749,26 +750,26 @@ __global__ void __launch_bounds__(NT, KV == 1 ? 3 : KV == 2 ? 2 : 1) k_norm_rows
     const T *x0 = (const T*)A.x + S.first * A.x_sn + col, *g0 = (const T*)A.dy + S.first * A.dy_sn + col;
     const int64_t xs = S.step * A.x_sn, gs = S.step * A.dy_sn, ys = (int64_t)S.step * A.c;
     int64_t at = (int64_t)S.first * A.c + col, ng = (int64_t)S.first * A.g + S.g;
+    V g[U][KV];
+    X x[U][KV];
+    float mean[U], rstd[U], lo[U], hi[U];
+    auto load = [&](int u, int64_t n, int64_t at, int64_t ng, const T* px, const T* pg) {
+        const bool ok = S.on && n < A.n;
+#pragma unroll
+        for (int k = 0; k < KV; k++)
+            if (has[k] && ok) {
+                if constexpr (U8) x[u][k] = *reinterpret_cast<const X*>(A.codes + at + k * LG * VEC);
+                else x[u][k] = *reinterpret_cast<const X*>(px + k * LG * VEC);
+                g[u][k] = *reinterpret_cast<const V*>(pg + k * LG * VEC);
+            }
+        mean[u] = ok ? __ldg(A.mean + ng) : 0.f;
+        rstd[u] = ok ? __ldg(A.rstd + ng) : 0.f;
+        lo[u] = U8 && ok ? __ldg(A.lo + ng) : 0.f;
+        hi[u] = U8 && ok ? __ldg(A.hi + ng) : 0.f;
+    };
+#pragma unroll
+    for (int u = 0; u < U; u++) load(u, S.first + (int64_t)u * S.step, at + u * ys, ng + (int64_t)u * S.step * A.g, x0 + u * xs, g0 + u * gs);
     for (int64_t n = S.first, base = 0; base < A.n; base += (int64_t)U * S.step) {
-        V g[U][KV];
-        X x[U][KV];
-        float mean[U], rstd[U], lo[U], hi[U];
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            const bool ok = S.on && n + u * S.step < A.n;
-#pragma unroll
-            for (int k = 0; k < KV; k++)
-                if (has[k] && ok) {
-                    if constexpr (U8) x[u][k] = *reinterpret_cast<const X*>(A.codes + at + u * ys + k * LG * VEC);
-                    else x[u][k] = *reinterpret_cast<const X*>(x0 + u * xs + k * LG * VEC);
-                    g[u][k] = *reinterpret_cast<const V*>(g0 + u * gs + k * LG * VEC);
-                }
-            const int64_t i = ng + (int64_t)u * S.step * A.g;
-            mean[u] = ok ? __ldg(A.mean + i) : 0.f;
-            rstd[u] = ok ? __ldg(A.rstd + i) : 0.f;
-            lo[u] = U8 && ok ? __ldg(A.lo + i) : 0.f;
-            hi[u] = U8 && ok ? __ldg(A.hi + i) : 0.f;
-        }
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const bool ok = n < A.n;
@@ -781,6 +782,8 @@ __global__ void __launch_bounds__(NT, KV == 1 ? 3 : KV == 2 ? 2 : 1) k_norm_rows
 #pragma unroll
                 for (int j = 0; j < VEC; j++) xh[k][j] = U8 ? fmaf(xh[k][j], xa, xb) : (xh[k][j] - xb) * xa;
             }
+            const float scale = rstd[u];
+            load(u, n + (int64_t)U * S.step, at + U * ys, ng + (int64_t)U * S.step * A.g, x0 + U * xs, g0 + U * gs);   // while this one is computed
             by_act(A.act, [&](auto act) {
 #pragma unroll
                 for (int k = 0; k < KV; k++)
@@ -802,7 +805,7 @@ __global__ void __launch_bounds__(NT, KV == 1 ? 3 : KV == 2 ? 2 : 1) k_norm_rows
             for (int k = 0; k < KV; k++)
                 if (has[k] && ok) {
 #pragma unroll
-                    for (int j = 0; j < VEC; j++) dz[k][j] = rstd[u] * fmaf(-xh[k][j], a2, fmaf(dz[k][j], w[k][j], -a1));
+                    for (int j = 0; j < VEC; j++) dz[k][j] = scale * fmaf(-xh[k][j], a2, fmaf(dz[k][j], w[k][j], -a1));
                     *reinterpret_cast<V*>((T*)A.dx + at + k * LG * VEC) = packed<T, VEC>(dz[k]);
                 }
             n += S.step; at += ys; ng += (int64_t)S.step * A.g; x0 += xs; g0 += gs;
@@ -1002,7 +1005,7 @@ bool make_rows(const FmeGroupNorm& a, bool bwd, Rows* W, int* kv) {
     W->gy = W->tall ? 1 : (a.g + W->segs - 1) / W->segs;
     W->by_g = divisor(a.g);
     const int at_once = W->tall ? W->tall : 1;
-    const int64_t need = ((int64_t)a.n + at_once - 1) / at_once, most = (int64_t)SMS * (*kv == 1 ? (bwd ? 3 : 4) : *kv == 2 || !bwd ? 2 : 1) / W->gy + 1;
+    const int64_t need = ((int64_t)a.n + at_once - 1) / at_once, most = (int64_t)SMS * (bwd ? (*kv == 4 ? 1 : 2) : (*kv == 1 ? 4 : 2)) / W->gy;
     W->grid = (int)(need < most ? need : most);   // as many CTAs as the GPU holds
     if (W->grid < 1) W->grid = 1;
     W->smem = bwd ? (size_t)8 * (W->tall ? W->tall * a.c : W->segs * cgr) : 0;
