@@ -364,14 +364,16 @@ __device__ __forceinline__ void powers(float* pw, float* pw1, int n, float log2_
 constexpr float LOG2E = 1.44269504088896340736f;
 
 // The forward pass of a segment (state rows: features of v). LOCAL: only its part of the state, from zero (the first: from s_in).
-template <typename T, int D, bool LOCAL, int MINB>
+// STAGES: 2 loads the next chunk while this one is computed, for CTAs that have an SM to themselves or nearly so.
+template <typename T, int D, bool LOCAL, int STAGES, int MINB>
 __global__ void __launch_bounds__(Shape<T, D>::NT, MINB) k_attn_fwd(const FmeDecayAttn A, const Walkers W) {
     using Z = Shape<T, D>;
     using Ti = Tile<T, D>;
     constexpr int C = Z::C, NT = Z::NT, NC = Z::NC;
     extern __shared__ __align__(1024) char sm[];
-    const Ti tk(sm), tv(sm + Z::TILE), tq(sm + 2 * Z::TILE), ts(sm + 3 * Z::TILE);
-    float* pw = reinterpret_cast<float*>(sm + (LOCAL ? 2 * Z::TILE : 3 * Z::TILE + Z::MAT));   // C + 1
+    constexpr int SET = (LOCAL ? 2 : 3) * Z::TILE;
+    const Ti ts(sm + STAGES * SET);
+    float* pw = reinterpret_cast<float*>(sm + STAGES * SET + (LOCAL ? 0 : Z::MAT));   // C + 1
     float *pw1 = pw + 72, *z = pw + 144;                                                      // C + 2, C
     const int warp = threadIdx.x >> 5, l = threadIdx.x & 31, g = l >> 2;
     const uint32_t across = LOCAL ? W.segs - 1 : W.segs, pair32 = across == 1 ? blockIdx.x : blockIdx.x / across, n32 = pair32 / (uint32_t)A.h;
@@ -388,9 +390,10 @@ __global__ void __launch_bounds__(Shape<T, D>::NT, MINB) k_attn_fwd(const FmeDec
     ResetBytes rb;
     auto fetch = [&](int c) {
         const int t0 = c * C, nv = min(C, A.t - t0);
-        load_tile<T, D, C, NT>(tk, k, A.k.st, t0, nv);
-        load_tile<T, D, C, NT>(tv, v, A.v.st, t0, nv);
-        if (!LOCAL) load_tile<T, D, C, NT>(tq, q, A.q.st, t0, nv);
+        char* set = sm + (STAGES == 2 ? ((c - c0) & 1) * SET : 0);
+        load_tile<T, D, C, NT>(Ti(set), k, A.k.st, t0, nv);
+        load_tile<T, D, C, NT>(Ti(set + Z::TILE), v, A.v.st, t0, nv);
+        if (!LOCAL) load_tile<T, D, C, NT>(Ti(set + 2 * Z::TILE), q, A.q.st, t0, nv);
         cp_commit();
         rb.load(reset, A.reset_st, t0, nv);
     };
@@ -405,9 +408,12 @@ __global__ void __launch_bounds__(Shape<T, D>::NT, MINB) k_attn_fwd(const FmeDec
     uint64_t any_cut = 0;
     for (int c = c0; c < c1; c++) {
         const int t0 = c * C;
+        char* set = sm + (STAGES == 2 ? ((c - c0) & 1) * SET : 0);
+        const Ti tk(set), tv(set + Z::TILE), tq(set + 2 * Z::TILE);
         cp_wait<0>();
         __syncthreads();
         const Cuts cuts{rb.bits(), min(C, A.t - t0)};
+        if (STAGES == 2 && c + 1 < c1) fetch(c + 1);   // the other set has been read by all
         any_cut |= cuts.m;
         const int last = cuts.last_up_to(63);
         bool again = false;
@@ -429,28 +435,18 @@ __global__ void __launch_bounds__(Shape<T, D>::NT, MINB) k_attn_fwd(const FmeDec
             }
             again = __syncthreads_or(not_finite(acc));
             // q and the old state have been read by all: the q tile takes the outputs
-            if (!again) store_rows<T, NC>(sm + 2 * Z::TILE + warp * Z::STAGE, acc, o, A.o.st, row0, col0, t0, cuts.n);
+            if (!again) store_rows<T, NC>(set + 2 * Z::TILE + warp * Z::STAGE, acc, o, A.o.st, row0, col0, t0, cuts.n);
         }
         const bool more = c + 1 < c1, save = A.saved && c + 1 < W.chunks;
         if (more || LOCAL || save || (A.s_out && c + 1 == W.chunks)) {
             const int j = threadIdx.x;
             if (j < C) z[j] = j < cuts.n && j >= last ? pw[cuts.n - 1 - j] : 0.f;
             __syncthreads();
-            if (LOCAL) {
-                float add[D / 8][4];
-                zero(add);
-                outer<T, D, C, true>(add, tv, m0, z, tk);
-                again = __any_sync(0xffffffffu, not_finite(add));
-                if (!again) {
-                    keep_state<D>(s, cuts, pw);
-#pragma unroll
-                    for (int i = 0; i < D / 8; i++)
-#pragma unroll
-                        for (int j = 0; j < 4; j++) s[i][j] += add[i][j];
-                }
-            } else if (!again) {
+            if (!again) {
                 keep_state<D>(s, cuts, pw);
                 outer<T, D, C, true>(s, tv, m0, z, tk);
+                // after a restart nothing of the state before is left: if what came out is no number, the walk starts over
+                if (LOCAL) again = cuts.m && __any_sync(0xffffffffu, not_finite(s));
             }
         }
         if (again) walk<T, D, false>(s, tv, tk, LOCAL ? tk : tq, 1.f, A.scale, m0, cuts, pw[1], LOCAL ? (T*)nullptr : o, A.o.st, t0);
@@ -468,8 +464,10 @@ __global__ void __launch_bounds__(Shape<T, D>::NT, MINB) k_attn_fwd(const FmeDec
                 }
             }
         }
-        __syncthreads();   // the tiles have been read by all
-        if (more) fetch(c + 1);
+        if (STAGES == 1) {
+            __syncthreads();   // the tiles have been read by all
+            if (more) fetch(c + 1);
+        }
     }
     if (LOCAL) {
         move_part<D, NT, true>(s, W.parts, blockIdx.x);
@@ -589,19 +587,10 @@ __global__ void __launch_bounds__(Shape<T, D>::NT, MINB) k_attn_bwd(const FmeDec
         again = __syncthreads_or(again);
         if (LOCAL || again || more || TWO) {
             if (LOCAL) {
-                float add[D / 8][4];
-                zero(add);
-                outer<T, D, C, true>(add, tq, m0, a, tg);
-                again = __any_sync(0xffffffffu, not_finite(add));
-                if (!again) {
-                    keep_state<D>(u, cuts, pw);
-#pragma unroll
-                    for (int i = 0; i < D / 8; i++)
-#pragma unroll
-                        for (int j = 0; j < 4; j++) u[i][j] += add[i][j];
-                } else {
+                keep_state<D>(u, cuts, pw);
+                outer<T, D, C, true>(u, tq, m0, a, tg);
+                if (cuts.m && __any_sync(0xffffffffu, not_finite(u)))   // as in the forward pass: the walk starts over
                     walk<T, D, true>(u, tq, tg, tg, A.scale, 1.f, m0, cuts, pw[1], (T*)nullptr, 0, t0);
-                }
             } else if (!again) {
                 keep_state<D>(u, cuts, pw);
                 outer<T, D, C, true>(u, tq, m0, a, tg);
@@ -639,25 +628,26 @@ __global__ void __launch_bounds__(Shape<T, D>::NT, MINB) k_attn_bwd(const FmeDec
     }
 }
 
-// The segments' parts joined: parts[s] becomes the state after segments 0..s. One thread for four values of one pair.
-__global__ void __launch_bounds__(256) k_attn_join(float* parts, int64_t pairs, int segs, int dd) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, per = dd / 4;
-    if (i >= pairs * per) return;
-    const int64_t pair = i / per;
-    float4* p = reinterpret_cast<float4*>(parts) + pair * segs * per + i % per;
+// The segments' parts joined: parts[s] becomes the state after segments 0..s. One thread a value; a segment's loads depend on
+// nothing, so JOIN of them are on their way at a time.
+constexpr int JOIN = 16;
+__global__ void __launch_bounds__(128) k_attn_join(float* parts, int64_t pairs, int segs, int dd) {
+    const int64_t i = (int64_t)blockIdx.x * 128 + threadIdx.x;
+    if (i >= pairs * dd) return;
+    const int64_t pair = i / dd;
+    float* p = parts + pair * segs * dd + i % dd;
     const float* keep = parts + pairs * segs * dd + pair * segs;
-    float4 s = p[0];
-    for (int b = 1; b < segs; b += 8) {
-        float4 x[8];
+    float s = p[0];
+    for (int b = 1; b < segs; b += JOIN) {
+        float x[JOIN], f[JOIN];
 #pragma unroll
-        for (int j = 0; j < 8; j++)
-            if (b + j < segs) x[j] = p[(b + j) * per];
+        for (int j = 0; j < JOIN; j++)
+            if (b + j < segs) { x[j] = p[(int64_t)(b + j) * dd]; f[j] = keep[b + j]; }   // negative: a restart
 #pragma unroll
-        for (int j = 0; j < 8; j++)
+        for (int j = 0; j < JOIN; j++)
             if (b + j < segs) {
-                const float f = keep[b + j];   // negative: a restart
-                s = f < 0.f ? x[j] : make_float4(fmaf(s.x, f, x[j].x), fmaf(s.y, f, x[j].y), fmaf(s.z, f, x[j].z), fmaf(s.w, f, x[j].w));
-                p[(b + j) * per] = s;
+                s = f[j] < 0.f ? x[j] : fmaf(s, f[j], x[j]);
+                p[(int64_t)(b + j) * dd] = s;
             }
     }
 }
@@ -710,7 +700,7 @@ template <typename T, int D> __global__ void __launch_bounds__(STEP_THREADS) k_a
 }
 
 // ---------------------------------------------------------------- host side
-constexpr int FEW_PAIRS = 592;   // four CTAs for each of 148 SMs: with fewer sequences and heads, segments
+constexpr int SMS = 148;
 constexpr int SEG_CHUNKS = 4;    // chunks of a segment at least
 
 int bad(const char* msg) { return host_fail(FME_E_ARG, msg); }
@@ -744,14 +734,16 @@ template <typename T, int D> struct Plan {
     using Z = Shape<T, D>;
     Walkers W;
     int64_t pairs;
-    explicit Plan(const FmeDecayAttn& a) {
+    Plan(const FmeDecayAttn& a, int ctas) {   // ctas: what an SM holds
         pairs = (int64_t)a.n * a.h;
         W.chunks = (a.t + Z::C - 1) / Z::C;
         W.segs = 1;
         W.per = W.chunks;
         W.parts = (float*)a.ws;
-        if (pairs > 0 && pairs < FEW_PAIRS && W.chunks >= 2 * SEG_CHUNKS) {
-            int64_t want = (FEW_PAIRS + pairs - 1) / pairs;
+        // Segments where half the GPU or more would idle: as many as make one wave, and not too short
+        const int64_t slots = (int64_t)SMS * ctas;
+        if (pairs > 0 && 2 * pairs <= slots && W.chunks >= 2 * SEG_CHUNKS) {
+            int64_t want = slots / pairs;
             if (want > W.chunks / SEG_CHUNKS) want = W.chunks / SEG_CHUNKS;
             W.per = (int)((W.chunks + want - 1) / want);
             W.segs = (W.chunks + W.per - 1) / W.per;
@@ -760,11 +752,13 @@ template <typename T, int D> struct Plan {
     int64_t ws_bytes() const { return W.segs > 1 ? pairs * (W.segs - 1) * (4 * D * D + 4) : 0; }
     int64_t saved_bytes() const { return W.chunks > 1 ? pairs * (W.chunks - 1) * D * D * (int64_t)sizeof(T) : 0; }
     static constexpr int FLOAT_BYTES = Z::FLOATS * 4;
-    static constexpr int FWD = 3 * Z::TILE + Z::MAT + FLOAT_BYTES, BWD = 4 * Z::TILE + 2 * Z::MAT + Z::NW * Z::STAGE + FLOAT_BYTES, LOCAL = 2 * Z::TILE + FLOAT_BYTES;
+    static constexpr int FWD = 3 * Z::TILE + Z::MAT + FLOAT_BYTES, FWD2 = FWD + 3 * Z::TILE, BWD = 4 * Z::TILE + 2 * Z::MAT + Z::NW * Z::STAGE + FLOAT_BYTES;
+    static constexpr int LOCAL_FWD = 4 * Z::TILE + FLOAT_BYTES, LOCAL_BWD = 2 * Z::TILE + FLOAT_BYTES;
 };
 // CTAs an SM that the registers are bounded for: what shared memory allows, and no more than keeps the accumulators in registers
 template <typename T, int D> constexpr int fwd_ctas() { return D == 128 ? 1 : sizeof(T) == 4 ? 3 : D == 64 ? 4 : 8; }
 template <typename T, int D> constexpr int bwd_ctas() { return D == 128 ? 1 : sizeof(T) == 4 ? 2 : D == 64 ? 3 : 6; }
+template <typename T, int D> constexpr int local_ctas() { return D == 128 ? 2 : sizeof(T) == 4 ? 2 : 4; }
 
 template <typename K> int go(const char* what, K kernel, int64_t grid, int threads, int smem, cudaStream_t st, const FmeDecayAttn& a, const Walkers& W) {
     if (smem > 48 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
@@ -773,7 +767,7 @@ template <typename K> int go(const char* what, K kernel, int64_t grid, int threa
 }
 int join(const char* what, const Walkers& W, int64_t pairs, int dd, cudaStream_t st) {
     if (W.segs == 2) return FME_OK;   // one part: nothing to add
-    k_attn_join<<<(unsigned)((pairs * (dd / 4) + 255) / 256), 256, 0, st>>>(W.parts, pairs, W.segs - 1, dd);
+    k_attn_join<<<(unsigned)((pairs * dd + 127) / 128), 128, 0, st>>>(W.parts, pairs, W.segs - 1, dd);
     return launch_status(what);
 }
 bool has_ws(const FmeDecayAttn& a, int64_t need) { return need == 0 || (a.ws && !((uintptr_t)a.ws & 255) && a.ws_bytes >= need); }
@@ -784,27 +778,28 @@ int pass_on(const char* what, const FmeDecayAttn& a, const float* from, float* t
 
 template <typename T, int D> int launch_fwd(const FmeDecayAttn& a, cudaStream_t st) {
     const char* what = "fme_decay_attn_fwd";
-    const Plan<T, D> P(a);
+    const Plan<T, D> P(a, fwd_ctas<T, D>());
     if (a.t == 0) return pass_on(what, a, a.s_in, a.s_out, st);
     if (!has_ws(a, P.ws_bytes())) return bad("decay attention: workspace too small or not aligned");
     if (P.pairs * P.W.segs > 0x7fffffff) return bad("decay attention: too many sequences");
     constexpr int NT = Shape<T, D>::NT;
     if (P.W.segs > 1) {
-        int rc = go(what, k_attn_fwd<T, D, true, 1>, P.pairs * (P.W.segs - 1), NT, Plan<T, D>::LOCAL, st, a, P.W);
+        int rc = go(what, k_attn_fwd<T, D, true, 2, local_ctas<T, D>()>, P.pairs * (P.W.segs - 1), NT, Plan<T, D>::LOCAL_FWD, st, a, P.W);
         if (rc || (rc = join(what, P.W, P.pairs, D * D, st))) return rc;
+        if constexpr (D == 128) return go(what, k_attn_fwd<T, D, false, 2, 1>, P.pairs * P.W.segs, NT, Plan<T, D>::FWD2, st, a, P.W);
     }
-    return go(what, k_attn_fwd<T, D, false, fwd_ctas<T, D>()>, P.pairs * P.W.segs, NT, Plan<T, D>::FWD, st, a, P.W);
+    return go(what, k_attn_fwd<T, D, false, 1, fwd_ctas<T, D>()>, P.pairs * P.W.segs, NT, Plan<T, D>::FWD, st, a, P.W);
 }
 template <typename T, int D> int launch_bwd(const FmeDecayAttn& a, cudaStream_t st) {
     const char* what = "fme_decay_attn_bwd";
-    const Plan<T, D> P(a);
+    const Plan<T, D> P(a, bwd_ctas<T, D>());
     if (a.t == 0) return pass_on(what, a, a.ds_out, a.ds_in, st);
     if (!has_ws(a, P.ws_bytes())) return bad("decay attention: workspace too small or not aligned");
     if (P.saved_bytes() && !a.saved) return bad("decay attention: the backward pass needs what the forward pass saved");
     if (P.pairs * P.W.segs > 0x7fffffff) return bad("decay attention: too many sequences");
     constexpr int NT = Shape<T, D>::NT;
     if (P.W.segs > 1) {
-        int rc = go(what, k_attn_bwd<T, D, true, true, 1>, P.pairs * (P.W.segs - 1), NT, Plan<T, D>::LOCAL, st, a, P.W);
+        int rc = go(what, k_attn_bwd<T, D, true, true, local_ctas<T, D>()>, P.pairs * (P.W.segs - 1), NT, Plan<T, D>::LOCAL_BWD, st, a, P.W);
         if (rc || (rc = join(what, P.W, P.pairs, D * D, st))) return rc;
     }
     if (a.ds_in) return go(what, k_attn_bwd<T, D, false, true, bwd_ctas<T, D>()>, P.pairs * P.W.segs, NT, Plan<T, D>::BWD, st, a, P.W);
@@ -815,7 +810,7 @@ template <typename T, int D> int launch_step(const FmeDecayAttn& a, cudaStream_t
     return launch_status("fme_decay_attn_step");
 }
 template <typename T, int D> int64_t sizes(const FmeDecayAttn& a, int which) {
-    const Plan<T, D> P(a);
+    const Plan<T, D> P(a, which == 1 ? bwd_ctas<T, D>() : fwd_ctas<T, D>());
     return which == 2 ? P.saved_bytes() : P.ws_bytes();
 }
 #define FME_BY_TYPE(a, FN, arg)                                                                                              \
