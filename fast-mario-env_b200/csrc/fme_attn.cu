@@ -13,6 +13,8 @@
 // part of the state, then these joined in order, then all segments at once with the state that they begin with.
 #include <math.h>
 
+#include <type_traits>
+
 #include "fme_host.h"
 #include "fme_mma.cuh"
 
@@ -30,6 +32,7 @@ template <typename T, int D> struct Shape {
     static constexpr int NW = D / 16, NT = 32 * NW, RB = C / 16, CG = NW / RB, NC = D / CG;
     static constexpr int TILE = C * D * (int)sizeof(T), MAT = D * D * (int)sizeof(T);
     static constexpr int STAGE = 16 * NC * (int)sizeof(T);   // a warp's outputs on their way out
+    static constexpr int BWD_STAGE = sizeof(T) == 2 ? 0 : STAGE;
     static constexpr int FLOATS = 3 * 72;                    // powers, powers one place on, weights
 };
 
@@ -86,12 +89,9 @@ __device__ __forceinline__ void store_rows(char* stage, const float (&acc)[NC / 
     constexpr int PW = NC < 32 ? 32 : NC;
     static_assert(NC >= 32, "");
     const Tile<T, PW> s(stage);
-    const int l = threadIdx.x & 31, g = l >> 2, c = l & 3;
+    const int l = threadIdx.x & 31;
 #pragma unroll
-    for (int i = 0; i < NC / 8; i++) {
-        s.put2(g, 8 * i + 2 * c, acc[i][0], acc[i][1]);
-        s.put2(g + 8, 8 * i + 2 * c, acc[i][2], acc[i][3]);
-    }
+    for (int i = 0; i < NC / 8; i += 2) Frag<T>::put16(s, 0, 8 * i, acc[i], acc[i + 1]);
     __syncwarp();
     constexpr int PIECES = NC / Tile<T, PW>::PER;
 #pragma unroll
@@ -103,6 +103,27 @@ __device__ __forceinline__ void store_rows(char* stage, const float (&acc)[NC / 
     __syncwarp();
 }
 
+// The same without shared memory, for bf16: lanes 2x and 2x + 1 hold two words each of two neighbouring blocks of 8 columns and
+// trade one, so that each has 8 bytes in a row and four lanes write a row's 32 bytes
+template <int NC>
+__device__ __forceinline__ void put_rows(const float (&acc)[NC / 8][4], bf16* dst, int64_t st, int row0, int col0, int t0, int n) {
+    const int l = threadIdx.x & 31, g = l >> 2, c = l & 3;
+    const bool odd = c & 1;
+    bf16* p = dst + (int64_t)(t0 + row0 + g) * st + col0 + (odd ? 8 : 0) + 4 * (c >> 1);
+    const int64_t down = 8 * st;
+    const bool in0 = row0 + g < n, in1 = row0 + g + 8 < n;
+#pragma unroll
+    for (int i = 0; i < NC / 8; i += 2) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const uint32_t a = pack2(acc[i][2 * h], acc[i][2 * h + 1]), b = pack2(acc[i + 1][2 * h], acc[i + 1][2 * h + 1]);
+            const uint32_t got = __shfl_xor_sync(0xffffffffu, odd ? a : b, 1);
+            const uint2 w = odd ? make_uint2(got, b) : make_uint2(a, got);
+            if (h ? in1 : in0) *reinterpret_cast<uint2*>(p + (h ? down : 0) + 8 * i) = w;
+        }
+    }
+}
+
 template <int N> __device__ __forceinline__ bool not_finite(const float (&a)[N][4]) {
     float z = 0.f;   // x * 0 is NaN unless x is finite
 #pragma unroll
@@ -112,13 +133,10 @@ template <int N> __device__ __forceinline__ bool not_finite(const float (&a)[N][
     return z != 0.f;
 }
 
-// Rows g and g + 8 times f0 and f1, or zero: a product with 0 would keep what is not a number
-template <int N> __device__ __forceinline__ void weigh(float (&a)[N][4], bool in0, bool in1, float f0, float f1) {
+// Rows g and g + 8 times f0 and f1. A product with 0 keeps what is not a number: such a chunk is done again, see walk()
+template <int N> __device__ __forceinline__ void weigh(float (&a)[N][4], float f0, float f1) {
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-        a[i][0] = in0 ? a[i][0] * f0 : 0.f; a[i][1] = in0 ? a[i][1] * f0 : 0.f;
-        a[i][2] = in1 ? a[i][2] * f1 : 0.f; a[i][3] = in1 ? a[i][3] * f1 : 0.f;
-    }
+    for (int i = 0; i < N; i++) { a[i][0] *= f0; a[i][1] *= f0; a[i][2] *= f1; a[i][3] *= f1; }
 }
 
 template <int N> __device__ __forceinline__ void zero(float (&a)[N][4]) {
@@ -151,19 +169,21 @@ template <typename T, int D> struct Left {
 template <typename T, int NB, int D, bool TR>
 __device__ __forceinline__ void product(float (&acc)[NB][4], const Left<T, D>& a, const Tile<T, D>& b, int n) {
     using F = Frag<T>;
-    zero(acc);
-#pragma unroll(Frag<T>::UNROLL)
-    for (int k = 0; k < D; k += F::KS) {
+    auto step = [&](int k, auto first) {
         const typename F::A fa = a.get(k);
 #pragma unroll
         for (int i = 0; i < NB; i += 2) {
             typename F::B b0, b1;
             if (TR) F::template ldBt<true>(b, k, n + 8 * i, b0, b1);
             else F::ldB(b, n + 8 * i, k, b0, b1);
-            F::mma(acc[i], fa, b0);
-            F::mma(acc[i + 1], fa, b1);
+            if (decltype(first)::value) { F::mma0(acc[i], fa, b0); F::mma0(acc[i + 1], fa, b1); }
+            else { F::mma(acc[i], fa, b0); F::mma(acc[i + 1], fa, b1); }
         }
-    }
+    };
+    if constexpr (sizeof(T) == 2) step(0, std::true_type{});
+    else zero(acc);
+#pragma unroll(Frag<T>::UNROLL)
+    for (int k = sizeof(T) == 2 ? F::KS : 0; k < D; k += F::KS) step(k, std::false_type{});
 }
 
 // A warp's factors of L * scale: within the 16 x 16 block on the diagonal as they are (0 above it), elsewhere
@@ -227,9 +247,15 @@ template <bool UP> struct Mask {
 template <typename T, int D>
 __device__ __forceinline__ void block_scores(float (&p)[2][4], const Left<T, D>& a, const Tile<T, D>& b, int col0, const float (&f)[2][4]) {
     using F = Frag<T>;
-    zero(p);
+    if constexpr (sizeof(T) == 2) {
+        const typename F::A fa = a.get(0);
+        typename F::B b0, b1;
+        F::ldB(b, col0, 0, b0, b1);
+        F::mma0(p[0], fa, b0);
+        F::mma0(p[1], fa, b1);
+    } else zero(p);
 #pragma unroll(sizeof(T) == 2 ? 8 : 2)
-    for (int k = 0; k < D; k += F::KS) {
+    for (int k = sizeof(T) == 2 ? F::KS : 0; k < D; k += F::KS) {
         const typename F::A fa = a.get(k);
         typename F::B b0, b1;
         F::ldB(b, col0, k, b0, b1);
@@ -259,40 +285,37 @@ __device__ __forceinline__ void block_apply(float (&acc)[NB][4], const float (&p
     }
 }
 
-// state (rows m0..m0+15 of the D x D matrix) += (w a)^T b over the chunk's tokens; TWO: the scaled rows in 16 bits at least
-template <typename T, int D, int C, bool TWO>
-__device__ __forceinline__ void outer(float (&s)[D / 8][4], const Tile<T, D>& a, int m0, const float* w, const Tile<T, D>& b) {
+// state (rows m0..m0+15 of the D x D matrix) += (w a)^T b over the chunk's tokens. The scaled rows of bf16 are taken in 16 bits,
+// fine: in 24, where the state itself is asked for, in fp32.
+template <typename T, int D, int C, int UNROLL>
+__device__ __forceinline__ void outer(float (&s)[D / 8][4], const Tile<T, D>& a, int m0, const float* w, const Tile<T, D>& b, bool fine) {
     using F = Frag<T>;
-#pragma unroll(Frag<T>::UNROLL)
+#pragma unroll(sizeof(T) == 2 ? UNROLL : 1)
     for (int k = 0; k < C; k += F::KS) {
-        const typename F::A2 fa = F::template ldAt<TWO>(a, k, m0, w);
+        const typename F::A2 fa = F::ldAt(a, k, m0, w, fine);
 #pragma unroll
         for (int i = 0; i < D / 8; i += 2) {
             typename F::B b0, b1;
             F::template ldBt<false>(b, k, 8 * i, b0, b1);
-            F::template mma2<TWO>(s[i], fa, b0);
-            F::template mma2<TWO>(s[i + 1], fa, b1);
+            F::mma2(s[i], fa, b0, fine);
+            F::mma2(s[i + 1], fa, b1, fine);
         }
     }
 }
 
 template <int D> __device__ __forceinline__ void keep_state(float (&s)[D / 8][4], const Cuts& cuts, const float* pw) {
+    if (cuts.m) { zero(s); return; }
     const float thru = pw[cuts.n];
-    const bool cut = cuts.m != 0ull;
 #pragma unroll
     for (int i = 0; i < D / 8; i++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) s[i][j] = cut ? 0.f : s[i][j] * thru;
+        for (int j = 0; j < 4; j++) s[i][j] *= thru;
 }
 
 // A warp's rows of the state in a tile of the operands' type
 template <typename T, int D> __device__ __forceinline__ void put_state(const Tile<T, D>& m, const float (&s)[D / 8][4], int row0) {
-    const int l = threadIdx.x & 31, g = l >> 2, c = l & 3;
 #pragma unroll
-    for (int i = 0; i < D / 8; i++) {
-        m.put2(row0 + g, 8 * i + 2 * c, s[i][0], s[i][1]);
-        m.put2(row0 + g + 8, 8 * i + 2 * c, s[i][2], s[i][3]);
-    }
+    for (int i = 0; i < D / 8; i += 2) Frag<T>::put16(m, row0, 8 * i, s[i], s[i + 1]);
 }
 // ... and to or from a (d, d) fp32 matrix. FLIP: the warp's rows are the matrix's columns.
 template <int D, bool FLIP, bool STORE, typename P> __device__ __forceinline__ void move_state(float (&s)[D / 8][4], P* mat, int row0) {
@@ -357,6 +380,17 @@ struct Walkers {   // the grid's layout: CTA = (sequence and head) * segs + segm
     float* parts;            // state of the segments: D * D floats each, then one float each: what a segment passes on
 };
 
+// The CTA's segment, head and sequence
+struct Spot {
+    int seg, h, n;
+    __device__ __forceinline__ Spot(const FmeDecayAttn& A, uint32_t across) {
+        const uint32_t pair = across == 1 ? blockIdx.x : blockIdx.x / across;
+        seg = blockIdx.x - pair * across;
+        n = pair / (uint32_t)A.h;
+        h = pair - n * A.h;
+    }
+};
+
 __device__ __forceinline__ void powers(float* pw, float* pw1, int n, float log2_lam) {
     for (int i = threadIdx.x; i < n; i += blockDim.x) pw[i] = pw1[i + 1] = i ? exp2f(log2_lam * (float)i) : 1.f;
 }
@@ -376,35 +410,34 @@ __global__ void __launch_bounds__(Shape<T, D>::NT, MINB) k_attn_fwd(const FmeDec
     float* pw = reinterpret_cast<float*>(sm + STAGES * SET + (LOCAL ? 0 : Z::MAT));   // C + 1
     float *pw1 = pw + 72, *z = pw + 144;                                                      // C + 2, C
     const int warp = threadIdx.x >> 5, l = threadIdx.x & 31, g = l >> 2;
-    const uint32_t across = LOCAL ? W.segs - 1 : W.segs, pair32 = across == 1 ? blockIdx.x : blockIdx.x / across, n32 = pair32 / (uint32_t)A.h;
-    const int64_t pair = pair32;
-    const int seg = blockIdx.x - pair32 * across, n = n32, h = pair32 - n32 * A.h;
-    const T *q = at<T>(A.q, n, h), *k = at<T>(A.k, n, h), *v = at<T>(A.v, n, h);
-    T* o = at<T>(A.o, n, h);
-    const uint8_t* reset = A.reset ? A.reset + n * A.reset_sn : nullptr;
+    const Spot P(A, LOCAL ? W.segs - 1 : W.segs);
+    const int seg = P.seg, h = P.h, n = P.n;
+    const bool fine = A.s_out != nullptr;
     const int c0 = seg * W.per, c1 = min(c0 + W.per, W.chunks);
     const int row0 = 16 * (warp % Z::RB), col0 = NC * (warp / Z::RB), m0 = 16 * warp;
     const float g2 = A.log_decay[h] * LOG2E;
     float s[D / 8][4];
-    bool some = true;   // whether the state before the chunk may be other than zero
+    bool some;   // whether the state before the chunk may be other than zero
     ResetBytes rb;
     auto fetch = [&](int c) {
         const int t0 = c * C, nv = min(C, A.t - t0);
         char* set = sm + (STAGES == 2 ? ((c - c0) & 1) * SET : 0);
-        load_tile<T, D, C, NT>(Ti(set), k, A.k.st, t0, nv);
-        load_tile<T, D, C, NT>(Ti(set + Z::TILE), v, A.v.st, t0, nv);
-        if (!LOCAL) load_tile<T, D, C, NT>(Ti(set + 2 * Z::TILE), q, A.q.st, t0, nv);
+        load_tile<T, D, C, NT>(Ti(set), at<T>(A.k, n, h), A.k.st, t0, nv);
+        load_tile<T, D, C, NT>(Ti(set + Z::TILE), at<T>(A.v, n, h), A.v.st, t0, nv);
+        if (!LOCAL) load_tile<T, D, C, NT>(Ti(set + 2 * Z::TILE), at<T>(A.q, n, h), A.q.st, t0, nv);
         cp_commit();
-        rb.load(reset, A.reset_st, t0, nv);
+        rb.load(A.reset ? A.reset + n * A.reset_sn : nullptr, A.reset_st, t0, nv);
     };
     if (c0 < c1) fetch(c0);
     powers(pw, pw1, C + 1, g2);
+    __syncthreads();
+    const Decay<true> dec(pw, A.scale);
+    const int64_t pair = (int64_t)n * A.h + h;
+    some = true;
     if (seg > 0 && !LOCAL) move_part<D, NT, false>(s, W.parts, pair * (W.segs - 1) + seg - 1);
     else if (seg == 0 && A.s_in) move_state<D, true, false>(s, A.s_in + pair * D * D, m0);
     else { zero(s); some = false; }
     if (!LOCAL && some) put_state(ts, s, m0);
-    __syncthreads();
-    const Decay<true> dec(pw, A.scale);
     uint64_t any_cut = 0;
     for (int c = c0; c < c1; c++) {
         const int t0 = c * C;
@@ -415,15 +448,19 @@ __global__ void __launch_bounds__(Shape<T, D>::NT, MINB) k_attn_fwd(const FmeDec
         const Cuts cuts{rb.bits(), min(C, A.t - t0)};
         if (STAGES == 2 && c + 1 < c1) fetch(c + 1);   // the other set has been read by all
         any_cut |= cuts.m;
-        const int last = cuts.last_up_to(63);
         bool again = false;
+        {
+            const int j = threadIdx.x, last = cuts.last_up_to(63);
+            if (j < C) z[j] = j < cuts.n && j >= last ? pw[cuts.n - 1 - j] : 0.f;
+        }
+        if constexpr (LOCAL) __syncthreads();
         if constexpr (!LOCAL) {
             float acc[NC / 8][4];
             const Left<T, D> lq(tq, row0);
             if (some) {
                 product<T, NC / 8, D, false>(acc, lq, ts, col0);
                 const bool in0 = cuts.last_up_to(row0 + g) < 0, in1 = cuts.last_up_to(row0 + g + 8) < 0;
-                weigh(acc, in0, in1, pw[row0 + g + 1] * A.scale, pw[row0 + g + 9] * A.scale);
+                weigh(acc, in0 ? pw[row0 + g + 1] * A.scale : 0.f, in1 ? pw[row0 + g + 9] * A.scale : 0.f);
             } else zero(acc);
             const Mask<true> mask(cuts, row0, dec);
 #pragma unroll 1
@@ -435,21 +472,18 @@ __global__ void __launch_bounds__(Shape<T, D>::NT, MINB) k_attn_fwd(const FmeDec
             }
             again = __syncthreads_or(not_finite(acc));
             // q and the old state have been read by all: the q tile takes the outputs
-            if (!again) store_rows<T, NC>(set + 2 * Z::TILE + warp * Z::STAGE, acc, o, A.o.st, row0, col0, t0, cuts.n);
+            if (!again) store_rows<T, NC>(set + 2 * Z::TILE + warp * Z::STAGE, acc, at<T>(A.o, n, h), A.o.st, row0, col0, t0, cuts.n);
         }
         const bool more = c + 1 < c1, save = A.saved && c + 1 < W.chunks;
         if (more || LOCAL || save || (A.s_out && c + 1 == W.chunks)) {
-            const int j = threadIdx.x;
-            if (j < C) z[j] = j < cuts.n && j >= last ? pw[cuts.n - 1 - j] : 0.f;
-            __syncthreads();
             if (!again) {
                 keep_state<D>(s, cuts, pw);
-                outer<T, D, C, true>(s, tv, m0, z, tk);
+                outer<T, D, C, 4>(s, tv, m0, z, tk, fine);
                 // after a restart nothing of the state before is left: if what came out is no number, the walk starts over
                 if (LOCAL) again = cuts.m && __any_sync(0xffffffffu, not_finite(s));
             }
         }
-        if (again) walk<T, D, false>(s, tv, tk, LOCAL ? tk : tq, 1.f, A.scale, m0, cuts, pw[1], LOCAL ? (T*)nullptr : o, A.o.st, t0);
+        if (again) walk<T, D, false>(s, tv, tk, LOCAL ? tk : tq, 1.f, A.scale, m0, cuts, pw[1], LOCAL ? (T*)nullptr : at<T>(A.o, n, h), A.o.st, t0);
         some = true;
         if constexpr (!LOCAL) {
             if (more || save) put_state(ts, s, m0);
@@ -464,9 +498,9 @@ __global__ void __launch_bounds__(Shape<T, D>::NT, MINB) k_attn_fwd(const FmeDec
                 }
             }
         }
-        if (STAGES == 1) {
+        if (STAGES == 1 && more) {
             __syncthreads();   // the tiles have been read by all
-            if (more) fetch(c + 1);
+            fetch(c + 1);
         }
     }
     if (LOCAL) {
@@ -489,45 +523,48 @@ __global__ void __launch_bounds__(Shape<T, D>::NT, MINB) k_attn_bwd(const FmeDec
     constexpr int C = Z::C, NT = Z::NT, NC = Z::NC;
     extern __shared__ __align__(1024) char sm[];
     const Ti tq(sm), tg(sm + Z::TILE), tk(sm + 2 * Z::TILE), tv(sm + 3 * Z::TILE), ts(sm + 4 * Z::TILE), tu(sm + 4 * Z::TILE + Z::MAT);
-    char* stage = sm + 4 * Z::TILE + 2 * Z::MAT + (threadIdx.x >> 5) * Z::STAGE;
-    float* pw = reinterpret_cast<float*>(sm + (LOCAL ? 2 * Z::TILE : 4 * Z::TILE + 2 * Z::MAT + Z::NW * Z::STAGE));
+    char* stage = sm + 4 * Z::TILE + 2 * Z::MAT + (threadIdx.x >> 5) * Z::BWD_STAGE;
+    float* pw = reinterpret_cast<float*>(sm + (LOCAL ? 2 * Z::TILE : 4 * Z::TILE + 2 * Z::MAT + Z::NW * Z::BWD_STAGE));
     float *pw1 = pw + 72, *a = pw + 144;
     const int warp = threadIdx.x >> 5, l = threadIdx.x & 31, g = l >> 2;
-    const uint32_t across = LOCAL ? W.segs - 1 : W.segs, pair32 = across == 1 ? blockIdx.x : blockIdx.x / across, n32 = pair32 / (uint32_t)A.h;
-    const int64_t pair = pair32;
-    const int rseg = blockIdx.x - pair32 * across, seg = W.segs - 1 - rseg, n = n32, h = pair32 - n32 * A.h;   // rseg 0: the last in time
-    const T *q = at<T>(A.q, n, h), *k = at<T>(A.k, n, h), *v = at<T>(A.v, n, h), *go = at<T>(A.d_o, n, h);
-    T *dq = at<T>(A.dq, n, h), *dk = at<T>(A.dk, n, h), *dv = at<T>(A.dv, n, h);
-    const uint8_t* reset = A.reset ? A.reset + n * A.reset_sn : nullptr;
+    const Spot P(A, LOCAL ? W.segs - 1 : W.segs);
+    const int rseg = P.seg, seg = W.segs - 1 - rseg, h = P.h, n = P.n;   // rseg 0: the last in time
+    const bool fine = A.ds_in != nullptr;
     const int c0 = seg * W.per, c1 = min(c0 + W.per, W.chunks);
     const int row0 = 16 * (warp % Z::RB), col0 = NC * (warp / Z::RB), m0 = 16 * warp;
     const float g2 = A.log_decay[h] * LOG2E;
     float u[D / 8][4];
-    bool some = true;   // whether the gradient of the state after the chunk may be other than zero
+    bool some;   // whether the gradient of the state after the chunk may be other than zero
     ResetBytes rb;
-    auto fetch = [&](int c) {
+    auto fetch_rows = [&](int c) {   // q and do
         const int t0 = c * C, nv = min(C, A.t - t0);
-        load_tile<T, D, C, NT>(tq, q, A.q.st, t0, nv);
-        load_tile<T, D, C, NT>(tg, go, A.d_o.st, t0, nv);
-        if (!LOCAL) {
-            load_tile<T, D, C, NT>(tk, k, A.k.st, t0, nv);
-            load_tile<T, D, C, NT>(tv, v, A.v.st, t0, nv);
-            if (c > 0) load_tile<T, D, D, NT>(ts, reinterpret_cast<const T*>(A.saved) + (pair * (W.chunks - 1) + c - 1) * D * D, D, 0, D);
-            else if (A.s_in) {
-                for (int i = threadIdx.x; i < D * D; i += NT) ts.at(i % D, i / D) = from_f<T>(A.s_in[pair * D * D + i]);
-            }
+        load_tile<T, D, C, NT>(tq, at<T>(A.q, n, h), A.q.st, t0, nv);
+        load_tile<T, D, C, NT>(tg, at<T>(A.d_o, n, h), A.d_o.st, t0, nv);
+        cp_commit();
+        rb.load(A.reset ? A.reset + n * A.reset_sn : nullptr, A.reset_st, t0, nv);
+    };
+    auto fetch_keys = [&](int c) {   // k, v and the state before the chunk
+        const int t0 = c * C, nv = min(C, A.t - t0);
+        const int64_t pair = (int64_t)n * A.h + h;
+        load_tile<T, D, C, NT>(tk, at<T>(A.k, n, h), A.k.st, t0, nv);
+        load_tile<T, D, C, NT>(tv, at<T>(A.v, n, h), A.v.st, t0, nv);
+        if (c > 0) load_tile<T, D, D, NT>(ts, reinterpret_cast<const T*>(A.saved) + (pair * (W.chunks - 1) + c - 1) * D * D, D, 0, D);
+        else if (A.s_in) {
+            for (int i = threadIdx.x; i < D * D; i += NT) ts.at(i % D, i / D) = from_f<T>(A.s_in[pair * D * D + i]);
         }
         cp_commit();
-        rb.load(reset, A.reset_st, t0, nv);
+    };
+    auto fetch = [&](int c) {
+        fetch_rows(c);
+        if (!LOCAL) fetch_keys(c);
     };
     if (c0 < c1) fetch(c1 - 1);
     powers(pw, pw1, C + 1, g2);
+    const int64_t pair = (int64_t)n * A.h + h;
+    some = true;
     if (rseg > 0 && !LOCAL) move_part<D, NT, false>(u, W.parts, pair * (W.segs - 1) + rseg - 1);
     else if (rseg == 0 && A.ds_out) move_state<D, false, false>(u, A.ds_out + pair * D * D, m0);
     else { zero(u); some = false; }
-    __syncthreads();
-    const Decay<false> down(pw, A.scale);
-    const Decay<true> up(pw, A.scale);
     uint64_t any_cut = 0;
     for (int c = c1 - 1; c >= c0; c--) {
         const int t0 = c * C;
@@ -541,35 +578,43 @@ __global__ void __launch_bounds__(Shape<T, D>::NT, MINB) k_attn_bwd(const FmeDec
         bool again = false;
         if constexpr (!LOCAL) {
             const int r0 = row0 + g, r1 = r0 + 8;
+            auto put = [&](const float (&acc)[NC / 8][4], const FmeAttnTensor& x) {
+                again |= not_finite(acc);
+                if constexpr (sizeof(T) == 2) put_rows<NC>(acc, at<T>(x, n, h), x.st, row0, col0, t0, cuts.n);
+                else store_rows<T, NC>(stage, acc, at<T>(x, n, h), x.st, row0, col0, t0, cuts.n);
+            };
+            float acc[NC / 8][4];
             {
                 const bool z0 = r0 >= last && r0 < cuts.n, z1 = r1 >= last && r1 < cuts.n;
-                const float w0 = pw[z0 ? cuts.n - 1 - r0 : 0], w1 = pw[z1 ? cuts.n - 1 - r1 : 0];
+                const float w0 = z0 ? pw[cuts.n - 1 - r0] : 0.f, w1 = z1 ? pw[cuts.n - 1 - r1] : 0.f;
+                const Decay<false> down(pw, A.scale);
                 const Mask<false> mask(cuts, row0, down);
-                float av[NC / 8][4], ak[NC / 8][4];
-                const Left<T, D> lk(tk, row0), lv(tv, row0);
-                if (some) {
-                    product<T, NC / 8, D, true>(av, lk, tu, col0); weigh(av, z0, z1, w0, w1);
-                    product<T, NC / 8, D, false>(ak, lv, tu, col0); weigh(ak, z0, z1, w0, w1);
-                } else { zero(av); zero(ak); }
+                // dv, then dk: the same with k and v, q and do in each other's place
+#pragma unroll
+                for (int which = 0; which < 2; which++) {
+                    const Ti &rows = which ? tv : tk, &cols = which ? tg : tq, &other = which ? tq : tg;
+                    const Left<T, D> left(rows, row0);
+                    if (some) {
+                        if (which) product<T, NC / 8, D, false>(acc, left, tu, col0);
+                        else product<T, NC / 8, D, true>(acc, left, tu, col0);
+                        weigh(acc, w0, w1);
+                    } else zero(acc);
 #pragma unroll 1
-                for (int i = row0; i < C; i += 16) {
-                    float p[2][4], f[2][4];
-                    mask.factors(f, i, pw1, down);
-                    block_scores<T, D>(p, lk, tq, i, f);
-                    block_apply<T, D>(av, p, tg, i, col0);
-                    block_scores<T, D>(p, lv, tg, i, f);
-                    block_apply<T, D>(ak, p, tq, i, col0);
+                    for (int i = row0; i < C; i += 16) {
+                        float p[2][4], f[2][4];
+                        mask.factors(f, i, pw1, down);
+                        block_scores<T, D>(p, left, cols, i, f);
+                        block_apply<T, D>(acc, p, other, i, col0);
+                    }
+                    put(acc, which ? A.dk : A.dv);
                 }
-                again |= not_finite(av) || not_finite(ak);
-                store_rows<T, NC>(stage, av, dv, A.dv.st, row0, col0, t0, cuts.n);
-                store_rows<T, NC>(stage, ak, dk, A.dk.st, row0, col0, t0, cuts.n);
             }
+            const Decay<true> up(pw, A.scale);
             const Mask<true> mask(cuts, row0, up);
-            float acc[NC / 8][4];
             const Left<T, D> lg(tg, row0);
             if (before) {
                 product<T, NC / 8, D, true>(acc, lg, ts, col0);
-                weigh(acc, cuts.last_up_to(r0) < 0, cuts.last_up_to(r1) < 0, pw[r0 + 1] * A.scale, pw[r1 + 1] * A.scale);
+                weigh(acc, cuts.last_up_to(r0) < 0 ? pw[r0 + 1] * A.scale : 0.f, cuts.last_up_to(r1) < 0 ? pw[r1 + 1] * A.scale : 0.f);
             } else zero(acc);
 #pragma unroll 1
             for (int j = 0; j <= row0; j += 16) {
@@ -578,22 +623,22 @@ __global__ void __launch_bounds__(Shape<T, D>::NT, MINB) k_attn_bwd(const FmeDec
                 block_scores<T, D>(p, lg, tv, j, f);
                 block_apply<T, D>(acc, p, tk, j, col0);
             }
-            again |= not_finite(acc);
-            store_rows<T, NC>(stage, acc, dq, A.dq.st, row0, col0, t0, cuts.n);
+            put(acc, A.dq);
         }
         const bool more = c > c0;
         const int j = threadIdx.x;
         if (j < C) a[j] = j < cuts.n && cuts.last_up_to(j) < 0 ? pw[j + 1] * A.scale : 0.f;
         again = __syncthreads_or(again);
+        if (!LOCAL && more && !again) fetch_keys(c - 1);   // k, v and the state before have been read by all
         if (LOCAL || again || more || TWO) {
             if (LOCAL) {
                 keep_state<D>(u, cuts, pw);
-                outer<T, D, C, true>(u, tq, m0, a, tg);
+                outer<T, D, C, 4>(u, tq, m0, a, tg, fine);
                 if (cuts.m && __any_sync(0xffffffffu, not_finite(u)))   // as in the forward pass: the walk starts over
                     walk<T, D, true>(u, tq, tg, tg, A.scale, 1.f, m0, cuts, pw[1], (T*)nullptr, 0, t0);
             } else if (!again) {
                 keep_state<D>(u, cuts, pw);
-                outer<T, D, C, true>(u, tq, m0, a, tg);
+                outer<T, D, C, 2>(u, tq, m0, a, tg, fine);
             } else {
                 float s[D / 8][4];
                 const int cc = l & 3;
@@ -602,20 +647,23 @@ __global__ void __launch_bounds__(Shape<T, D>::NT, MINB) k_attn_bwd(const FmeDec
                 for (int i = 0; i < D / 8; i++)
 #pragma unroll
                     for (int j = 0; j < 4; j++) s[i][j] = before ? to_f(ts.at(8 * i + 2 * cc + (j & 1), m0 + g + 8 * (j >> 1))) : 0.f;
-                walk<T, D, false>(s, tk, tv, tg, 1.f, A.scale, m0, cuts, pw[1], dq, A.dq.st, t0);
+                walk<T, D, false>(s, tk, tv, tg, 1.f, A.scale, m0, cuts, pw[1], at<T>(A.dq, n, h), A.dq.st, t0);
                 // dv: backward, the transposed gradient (rows: features of v)
 #pragma unroll
                 for (int i = 0; i < D / 8; i++)
 #pragma unroll
                     for (int j = 0; j < 4; j++) s[i][j] = some ? to_f(tu.at(8 * i + 2 * cc + (j & 1), m0 + g + 8 * (j >> 1))) : 0.f;
-                walk<T, D, true>(s, tg, tq, tk, A.scale, 1.f, m0, cuts, pw[1], dv, A.dv.st, t0);
+                walk<T, D, true>(s, tg, tq, tk, A.scale, 1.f, m0, cuts, pw[1], at<T>(A.dv, n, h), A.dv.st, t0);
                 // dk, and the gradient itself
-                walk<T, D, true>(u, tq, tg, tv, A.scale, 1.f, m0, cuts, pw[1], dk, A.dk.st, t0);
+                walk<T, D, true>(u, tq, tg, tv, A.scale, 1.f, m0, cuts, pw[1], at<T>(A.dk, n, h), A.dk.st, t0);
             }
         }
         some = true;
-        __syncthreads();   // the tiles and the gradient have been read by all
-        if (more) fetch(c - 1);
+        if (more) {
+            __syncthreads();   // the tiles and the gradient have been read by all
+            fetch_rows(c - 1);
+            if (!LOCAL && again) fetch_keys(c - 1);
+        }
     }
     if (LOCAL) {
         move_part<D, NT, true>(u, W.parts, blockIdx.x);
@@ -752,13 +800,13 @@ template <typename T, int D> struct Plan {
     int64_t ws_bytes() const { return W.segs > 1 ? pairs * (W.segs - 1) * (4 * D * D + 4) : 0; }
     int64_t saved_bytes() const { return W.chunks > 1 ? pairs * (W.chunks - 1) * D * D * (int64_t)sizeof(T) : 0; }
     static constexpr int FLOAT_BYTES = Z::FLOATS * 4;
-    static constexpr int FWD = 3 * Z::TILE + Z::MAT + FLOAT_BYTES, FWD2 = FWD + 3 * Z::TILE, BWD = 4 * Z::TILE + 2 * Z::MAT + Z::NW * Z::STAGE + FLOAT_BYTES;
+    static constexpr int FWD = 3 * Z::TILE + Z::MAT + FLOAT_BYTES, BWD = 4 * Z::TILE + 2 * Z::MAT + Z::NW * Z::BWD_STAGE + FLOAT_BYTES;
     static constexpr int LOCAL_FWD = 4 * Z::TILE + FLOAT_BYTES, LOCAL_BWD = 2 * Z::TILE + FLOAT_BYTES;
 };
 // CTAs an SM that the registers are bounded for: what shared memory allows, and no more than keeps the accumulators in registers
 template <typename T, int D> constexpr int fwd_ctas() { return D == 128 ? 1 : sizeof(T) == 4 ? 3 : D == 64 ? 4 : 8; }
-template <typename T, int D> constexpr int bwd_ctas() { return D == 128 ? 1 : sizeof(T) == 4 ? 2 : D == 64 ? 3 : 6; }
-template <typename T, int D> constexpr int local_ctas() { return D == 128 ? 2 : sizeof(T) == 4 ? 2 : 4; }
+template <typename T, int D> constexpr int bwd_ctas() { return D == 128 ? 1 : sizeof(T) == 4 ? 2 : D == 64 ? 4 : 8; }
+template <typename T, int D> constexpr int local_ctas() { return D == 128 ? 1 : sizeof(T) == 4 ? 2 : 4; }
 
 template <typename K> int go(const char* what, K kernel, int64_t grid, int threads, int smem, cudaStream_t st, const FmeDecayAttn& a, const Walkers& W) {
     if (smem > 48 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
@@ -786,7 +834,7 @@ template <typename T, int D> int launch_fwd(const FmeDecayAttn& a, cudaStream_t 
     if (P.W.segs > 1) {
         int rc = go(what, k_attn_fwd<T, D, true, 2, local_ctas<T, D>()>, P.pairs * (P.W.segs - 1), NT, Plan<T, D>::LOCAL_FWD, st, a, P.W);
         if (rc || (rc = join(what, P.W, P.pairs, D * D, st))) return rc;
-        if constexpr (D == 128) return go(what, k_attn_fwd<T, D, false, 2, 1>, P.pairs * P.W.segs, NT, Plan<T, D>::FWD2, st, a, P.W);
+        if constexpr (D == 128) return go(what, k_attn_fwd<T, D, false, 2, 1>, P.pairs * P.W.segs, NT, Plan<T, D>::FWD + 3 * Shape<T, D>::TILE, st, a, P.W);
     }
     return go(what, k_attn_fwd<T, D, false, 1, fwd_ctas<T, D>()>, P.pairs * P.W.segs, NT, Plan<T, D>::FWD, st, a, P.W);
 }

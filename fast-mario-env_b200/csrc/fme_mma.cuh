@@ -65,6 +65,9 @@ __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
 __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
 }
+__device__ __forceinline__ void stsm4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
 __device__ __forceinline__ float lds(uint32_t addr) {
     float x;
     asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(addr));
@@ -86,7 +89,12 @@ template <> struct Frag<bf16> {
     static constexpr int KS = 16, UNROLL = 8;   // steps of a product in one piece of code
     struct A { uint32_t r[4]; };
     struct B { uint32_t r[2]; };
-    struct A2 { A hi, lo; };    // a scaled operand in two bfloat16 numbers: 16 bits of it count
+    struct A2 { A hi, lo, rest; };    // a scaled operand in two bfloat16 numbers (16 bits of it count) or three (24)
+    // 16 x 16 accumulators to a tile
+    template <int COLS> static __device__ __forceinline__ void put16(const Tile<bf16, COLS>& s, int row, int col, const float* u, const float* v) {
+        const int l = threadIdx.x & 31;
+        stsm4(s.along(s.lane(row + (l & 15), l >> 4), 2 * col), pack2(u[0], u[1]), pack2(u[2], u[3]), pack2(v[0], v[1]), pack2(v[2], v[3]));
+    }
     static __device__ __forceinline__ void mma(float (&d)[4], const A& a, const B& b) {
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a.r[0]), "r"(a.r[1]), "r"(a.r[2]), "r"(a.r[3]), "r"(b.r[0]), "r"(b.r[1]));
@@ -118,7 +126,7 @@ template <> struct Frag<bf16> {
         b0.r[0] = r[0]; b0.r[1] = r[1]; b1.r[0] = r[2]; b1.r[1] = r[3];
     }
     // A[m][k] = weight[k] * tile[k][m], weights in shared memory
-    template <bool TWO, int COLS> static __device__ __forceinline__ A2 ldAt(const Tile<bf16, COLS>& s, int k, int m, const float* w) {
+    template <int COLS> static __device__ __forceinline__ A2 ldAt(const Tile<bf16, COLS>& s, int k, int m, const float* w, bool fine) {
         const int l = threadIdx.x & 31;
         A2 a;
         ldsm4t(a.hi.r, s.along(s.lane(k + (l & 7) + ((l >> 4) << 3), (l >> 3) & 1), 2 * m));
@@ -127,16 +135,19 @@ template <> struct Frag<bf16> {
             const float2 v = unpack2(a.hi.r[i]), f = *reinterpret_cast<const float2*>(w + k + ((i >> 1) << 3) + 2 * (l & 3));
             const float x = v.x * f.x, y = v.y * f.y;
             a.hi.r[i] = pack2(x, y);
-            if (TWO) {
-                const float2 h = unpack2(a.hi.r[i]);
-                a.lo.r[i] = pack2(x - h.x, y - h.y);
+            const float2 h = unpack2(a.hi.r[i]);
+            a.lo.r[i] = pack2(x - h.x, y - h.y);
+            if (fine) {
+                const float2 g = unpack2(a.lo.r[i]);
+                a.rest.r[i] = pack2(x - h.x - g.x, y - h.y - g.y);
             }
         }
         return a;
     }
-    template <bool TWO> static __device__ __forceinline__ void mma2(float (&d)[4], const A2& a, const B& b) {
+    static __device__ __forceinline__ void mma2(float (&d)[4], const A2& a, const B& b, bool fine) {
+        if (fine) mma(d, a.rest, b);
+        mma(d, a.lo, b);
         mma(d, a.hi, b);
-        if (TWO) mma(d, a.lo, b);
     }
     // The accumulators of 16 columns as an operand whose k runs over them
     static __device__ __forceinline__ A chain(const float (*acc)[4], int ks) {
@@ -150,6 +161,20 @@ template <> struct Frag<float> {
     struct A { uint32_t hi[4], lo[4]; };
     struct B { uint32_t hi[2], lo[2]; };
     using A2 = A;
+    template <int COLS> static __device__ __forceinline__ void put16(const Tile<float, COLS>& s, int row, int col, const float* u, const float* v) {
+        const int g = (threadIdx.x & 31) >> 2, c = 2 * (threadIdx.x & 3);
+        s.put2(row + g, col + c, u[0], u[1]);
+        s.put2(row + g + 8, col + c, u[2], u[3]);
+        s.put2(row + g, col + 8 + c, v[0], v[1]);
+        s.put2(row + g + 8, col + 8 + c, v[2], v[3]);
+    }
+    // d = a b
+    static __device__ __forceinline__ void mma0(float (&d)[4], const A& a, const B& b) {
+        asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                     : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a.lo[0]), "r"(a.lo[1]), "r"(a.lo[2]), "r"(a.lo[3]), "r"(b.hi[0]), "r"(b.hi[1]), "f"(0.f));
+        one(d, a.hi, b.lo);
+        one(d, a.hi, b.hi);
+    }
     static __device__ __forceinline__ void one(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
         asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
@@ -193,7 +218,7 @@ template <> struct Frag<float> {
             split_tf32(lds(s.along(at, 4 * n + 32)), b1.hi[i], b1.lo[i]);
         }
     }
-    template <bool TWO, int COLS> static __device__ __forceinline__ A2 ldAt(const Tile<float, COLS>& s, int k, int m, const float* w) {
+    template <int COLS> static __device__ __forceinline__ A2 ldAt(const Tile<float, COLS>& s, int k, int m, const float* w, bool) {
         const int g = (threadIdx.x & 31) >> 2;
         A a;
 #pragma unroll
@@ -203,7 +228,7 @@ template <> struct Frag<float> {
         }
         return a;
     }
-    template <bool TWO> static __device__ __forceinline__ void mma2(float (&d)[4], const A2& a, const B& b) { mma(d, a, b); }
+    static __device__ __forceinline__ void mma2(float (&d)[4], const A2& a, const B& b, bool) { mma(d, a, b); }
     static __device__ __forceinline__ A chain(const float (*acc)[4], int ks) {
         const float* u = acc[ks];
         A a;
