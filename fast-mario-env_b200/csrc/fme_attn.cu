@@ -434,6 +434,8 @@ __global__ void __launch_bounds__(Shape<T, D>::NT, MINB) k_attn_fwd(const FmeDec
     const Decay<true> dec(pw, A.scale);
     const int64_t pair = (int64_t)n * A.h + h;
     some = true;
+    if (LOCAL) let_next_start();
+    else await_previous();   // the parts
     if (seg > 0 && !LOCAL) move_part<D, NT, false>(s, W.parts, pair * (W.segs - 1) + seg - 1);
     else if (seg == 0 && A.s_in) move_state<D, true, false>(s, A.s_in + pair * D * D, m0);
     else { zero(s); some = false; }
@@ -562,6 +564,8 @@ __global__ void __launch_bounds__(Shape<T, D>::NT, MINB) k_attn_bwd(const FmeDec
     powers(pw, pw1, C + 1, g2);
     const int64_t pair = (int64_t)n * A.h + h;
     some = true;
+    if (LOCAL) let_next_start();
+    else await_previous();   // the parts
     if (rseg > 0 && !LOCAL) move_part<D, NT, false>(u, W.parts, pair * (W.segs - 1) + rseg - 1);
     else if (rseg == 0 && A.ds_out) move_state<D, false, false>(u, A.ds_out + pair * D * D, m0);
     else { zero(u); some = false; }
@@ -681,6 +685,8 @@ __global__ void __launch_bounds__(Shape<T, D>::NT, MINB) k_attn_bwd(const FmeDec
 constexpr int JOIN = 16;
 __global__ void __launch_bounds__(128) k_attn_join(float* parts, int64_t pairs, int segs, int dd) {
     const int64_t i = (int64_t)blockIdx.x * 128 + threadIdx.x;
+    let_next_start();
+    await_previous();
     if (i >= pairs * dd) return;
     const int64_t pair = i / dd;
     float* p = parts + pair * segs * dd + i % dd;
@@ -805,18 +811,18 @@ template <typename T, int D> struct Plan {
 };
 // CTAs an SM that the registers are bounded for: what shared memory allows, and no more than keeps the accumulators in registers
 template <typename T, int D> constexpr int fwd_ctas() { return D == 128 ? 1 : sizeof(T) == 4 ? 3 : D == 64 ? 4 : 8; }
-template <typename T, int D> constexpr int bwd_ctas() { return D == 128 ? 1 : sizeof(T) == 4 ? 2 : D == 64 ? 4 : 8; }
+template <typename T, int D> constexpr int bwd_ctas() { return D == 128 ? 1 : sizeof(T) == 4 ? 2 : D == 64 ? 3 : 6; }
 template <typename T, int D> constexpr int local_ctas() { return D == 128 ? 1 : sizeof(T) == 4 ? 2 : 4; }
 
-template <typename K> int go(const char* what, K kernel, int64_t grid, int threads, int smem, cudaStream_t st, const FmeDecayAttn& a, const Walkers& W) {
+template <typename K> int go(const char* what, K kernel, int64_t grid, int threads, int smem, cudaStream_t st, const FmeDecayAttn& a, const Walkers& W, bool behind = false) {
     if (smem > 48 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (behind) return launch_behind(what, kernel, dim3((unsigned)grid), dim3(threads), smem, st, a, W);
     kernel<<<(unsigned)grid, threads, smem, st>>>(a, W);
     return launch_status(what);
 }
 int join(const char* what, const Walkers& W, int64_t pairs, int dd, cudaStream_t st) {
     if (W.segs == 2) return FME_OK;   // one part: nothing to add
-    k_attn_join<<<(unsigned)((pairs * dd + 127) / 128), 128, 0, st>>>(W.parts, pairs, W.segs - 1, dd);
-    return launch_status(what);
+    return launch_behind(what, k_attn_join, dim3((unsigned)((pairs * dd + 127) / 128)), dim3(128), 0, st, W.parts, pairs, W.segs - 1, dd);
 }
 bool has_ws(const FmeDecayAttn& a, int64_t need) { return need == 0 || (a.ws && !((uintptr_t)a.ws & 255) && a.ws_bytes >= need); }
 int pass_on(const char* what, const FmeDecayAttn& a, const float* from, float* to, cudaStream_t st) {
@@ -834,9 +840,9 @@ template <typename T, int D> int launch_fwd(const FmeDecayAttn& a, cudaStream_t 
     if (P.W.segs > 1) {
         int rc = go(what, k_attn_fwd<T, D, true, 2, local_ctas<T, D>()>, P.pairs * (P.W.segs - 1), NT, Plan<T, D>::LOCAL_FWD, st, a, P.W);
         if (rc || (rc = join(what, P.W, P.pairs, D * D, st))) return rc;
-        if constexpr (D == 128) return go(what, k_attn_fwd<T, D, false, 2, 1>, P.pairs * P.W.segs, NT, Plan<T, D>::FWD + 3 * Shape<T, D>::TILE, st, a, P.W);
+        if constexpr (D == 128) return go(what, k_attn_fwd<T, D, false, 2, 1>, P.pairs * P.W.segs, NT, Plan<T, D>::FWD + 3 * Shape<T, D>::TILE, st, a, P.W, true);
     }
-    return go(what, k_attn_fwd<T, D, false, 1, fwd_ctas<T, D>()>, P.pairs * P.W.segs, NT, Plan<T, D>::FWD, st, a, P.W);
+    return go(what, k_attn_fwd<T, D, false, 1, fwd_ctas<T, D>()>, P.pairs * P.W.segs, NT, Plan<T, D>::FWD, st, a, P.W, P.W.segs > 1);
 }
 template <typename T, int D> int launch_bwd(const FmeDecayAttn& a, cudaStream_t st) {
     const char* what = "fme_decay_attn_bwd";
@@ -850,8 +856,8 @@ template <typename T, int D> int launch_bwd(const FmeDecayAttn& a, cudaStream_t 
         int rc = go(what, k_attn_bwd<T, D, true, true, local_ctas<T, D>()>, P.pairs * (P.W.segs - 1), NT, Plan<T, D>::LOCAL_BWD, st, a, P.W);
         if (rc || (rc = join(what, P.W, P.pairs, D * D, st))) return rc;
     }
-    if (a.ds_in) return go(what, k_attn_bwd<T, D, false, true, bwd_ctas<T, D>()>, P.pairs * P.W.segs, NT, Plan<T, D>::BWD, st, a, P.W);
-    return go(what, k_attn_bwd<T, D, false, false, bwd_ctas<T, D>()>, P.pairs * P.W.segs, NT, Plan<T, D>::BWD, st, a, P.W);
+    if (a.ds_in) return go(what, k_attn_bwd<T, D, false, true, bwd_ctas<T, D>()>, P.pairs * P.W.segs, NT, Plan<T, D>::BWD, st, a, P.W, P.W.segs > 1);
+    return go(what, k_attn_bwd<T, D, false, false, bwd_ctas<T, D>()>, P.pairs * P.W.segs, NT, Plan<T, D>::BWD, st, a, P.W, P.W.segs > 1);
 }
 template <typename T, int D> int launch_step(const FmeDecayAttn& a, cudaStream_t st) {
     k_attn_step<T, D><<<a.n * a.h, STEP_THREADS, 0, st>>>(a);

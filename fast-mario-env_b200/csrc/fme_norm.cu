@@ -576,6 +576,7 @@ __global__ void __launch_bounds__(MAX_THREADS, 2) k_norm_bwd(const FmeGroupNorm 
     }
     if (PH == APPLY || !A.dw) return;
     // dw and db of this CTA: slots c, c + C, ... hold channel c
+    let_next_start();
     __syncthreads();
     float* rw = reinterpret_cast<float*>(sm);
     const int slots = P.R * P.M * VEC;
@@ -812,6 +813,7 @@ __global__ void __launch_bounds__(NT, KV == 4 ? 1 : 2) k_norm_rows_bwd(const Fme
         }
     }
     if (!A.dw) return;
+    let_next_start();
     // the CTA's row of dw and db: c of each, with zeros where another grid.y has the channels
     float* row = (float*)A.ws + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 2 * A.c;
     const int tall = W.tall ? W.tall : 1, k0 = W.tall ? (S.first - (int)blockIdx.x * W.tall) : 0;
@@ -944,6 +946,7 @@ __global__ void __launch_bounds__(1024) k_norm_params(const float* __restrict__ 
     __shared__ float sm[32][33];
     const int i = blockIdx.x * 32 + threadIdx.x;
     float s = 0.f;
+    await_previous();
     if (i < 2 * c) {
         const float* p = ws + i;
         int r = threadIdx.y;
@@ -1232,8 +1235,7 @@ int fme_group_norm_bwd(const FmeGroupNorm* a, void* stream) {
         else rc = u8 ? run_bwd<__nv_bfloat16, true>(*a, P, st) : run_bwd<__nv_bfloat16, false>(*a, P, st);
     }
     if (rc || !a->dw) return rc;
-    k_norm_params<<<(2 * a->c + 31) / 32, dim3(32, 32), 0, st>>>((const float*)a->ws + skip, rows, a->c, a->dw, a->db);
-    return launch_status("fme_group_norm_bwd");
+    return launch_behind("fme_group_norm_bwd", k_norm_params, dim3((2 * a->c + 31) / 32), dim3(32, 32), 0, st, (const float*)a->ws + skip, rows, a->c, a->dw, a->db);
 }
 
 }  // extern "C"
