@@ -32,7 +32,6 @@ template <typename T, int D> struct Shape {
     static constexpr int NW = D / 16, NT = 32 * NW, RB = C / 16, CG = NW / RB, NC = D / CG;
     static constexpr int TILE = C * D * (int)sizeof(T), MAT = D * D * (int)sizeof(T);
     static constexpr int STAGE = 16 * NC * (int)sizeof(T);   // a warp's outputs on their way out
-    static constexpr int BWD_STAGE = sizeof(T) == 2 ? 0 : STAGE;
     static constexpr int FLOATS = 3 * 72;                    // powers, powers one place on, weights
 };
 
@@ -70,14 +69,16 @@ __device__ __forceinline__ void load_tile(const Tile<T, D>& dst, const T* src, i
     const int row = threadIdx.x / PIECES, col = (threadIdx.x % PIECES) * Tile<T, D>::PER;
     const char* p = reinterpret_cast<const char*>(src + (t0 + row) * st + col);
     const int64_t step = STEP * st * (int64_t)sizeof(T);
+    static_assert(STEP % 8 == 0, "the permutation repeats after eight rows");
+    const uint32_t to = dst.base + dst.off(row, col);
     if (n == C) {
 #pragma unroll
-        for (int i = 0; i < C / STEP; i++) cp16(dst.base + dst.off(row + i * STEP, col), p + i * step, true);
+        for (int i = 0; i < C / STEP; i++) cp16(to + i * STEP * Tile<T, D>::ROW, p + i * step, true);
     } else {
 #pragma unroll
         for (int i = 0; i < C / STEP; i++) {
             const bool in = row + i * STEP < n;
-            cp16(dst.base + dst.off(row + i * STEP, col), in ? p + i * step : reinterpret_cast<const char*>(src), in);
+            cp16(to + i * STEP * Tile<T, D>::ROW, in ? p + i * step : reinterpret_cast<const char*>(src), in);
         }
     }
 }
@@ -103,7 +104,20 @@ __device__ __forceinline__ void store_rows(char* stage, const float (&acc)[NC / 
     __syncwarp();
 }
 
-// The same without shared memory, for bf16: lanes 2x and 2x + 1 hold two words each of two neighbouring blocks of 8 columns and
+// The same without shared memory. fp32: four lanes write a row's 32 bytes
+template <int NC>
+__device__ __forceinline__ void put_rows(const float (&acc)[NC / 8][4], float* dst, int64_t st, int row0, int col0, int t0, int n) {
+    const int l = threadIdx.x & 31, g = l >> 2;
+    float* p = dst + (int64_t)(t0 + row0 + g) * st + col0 + 2 * (l & 3);
+    const int64_t down = 8 * st;
+    const bool in0 = row0 + g < n, in1 = row0 + g + 8 < n;
+#pragma unroll
+    for (int i = 0; i < NC / 8; i++) {
+        if (in0) *reinterpret_cast<float2*>(p + 8 * i) = make_float2(acc[i][0], acc[i][1]);
+        if (in1) *reinterpret_cast<float2*>(p + down + 8 * i) = make_float2(acc[i][2], acc[i][3]);
+    }
+}
+// bf16: lanes 2x and 2x + 1 hold two words each of two neighbouring blocks of 8 columns and
 // trade one, so that each has 8 bytes in a row and four lanes write a row's 32 bytes
 template <int NC>
 __device__ __forceinline__ void put_rows(const float (&acc)[NC / 8][4], bf16* dst, int64_t st, int row0, int col0, int t0, int n) {
@@ -213,12 +227,27 @@ template <bool UP> struct Mask {
     int row0, lim0, lim1, lim;
     float r0, r1;
     __device__ __forceinline__ Mask(const Cuts& cuts, int row0_, const Decay<UP>& dec) : row0(row0_) {
-        const int g = (threadIdx.x & 31) >> 2, edge = UP ? row0 : row0 + 15;
-        lim0 = UP ? cuts.last_up_to(row0 + g) : cuts.next_after(row0 + g);
-        lim1 = UP ? cuts.last_up_to(row0 + g + 8) : cuts.next_after(row0 + g + 8);
-        lim = UP ? cuts.last_up_to(edge) : cuts.next_after(edge);
-        r0 = (UP ? lim0 <= edge : lim0 > edge) ? dec.row[0] : 0.f;
-        r1 = (UP ? lim1 <= edge : lim1 > edge) ? dec.row[1] : 0.f;
+        // restarts within the sixteen rows, and the nearest one outside them
+        const int g = (threadIdx.x & 31) >> 2;
+        const uint32_t own = (uint32_t)(cuts.m >> row0) & 0xffffu;
+        if (UP) {
+            const uint64_t below = cuts.m & ~(~0ull << row0);
+            const int out = 63 - __clzll((long long)below);
+            const uint32_t x0 = own & (0x1ffu >> (8 - g)), x1 = own & (0x1ffffu >> (8 - g));
+            lim = own & 1 ? row0 : out;
+            lim0 = x0 ? row0 + 31 - __clz(x0) : out;
+            lim1 = x1 ? row0 + 31 - __clz(x1) : out;
+            r0 = lim0 <= row0 ? dec.row[0] : 0.f;
+            r1 = lim1 <= row0 ? dec.row[1] : 0.f;
+        } else {
+            const uint64_t above = row0 + 16 >= 64 ? 0ull : cuts.m >> (row0 + 16);
+            const uint32_t x0 = own >> (g + 1), x1 = own >> (g + 9);
+            lim = above ? row0 + 15 + __ffsll((long long)above) : 64;
+            lim0 = x0 ? row0 + g + __ffs(x0) : lim;
+            lim1 = x1 ? row0 + g + 8 + __ffs(x1) : lim;
+            r0 = x0 ? 0.f : dec.row[0];
+            r1 = x1 ? 0.f : dec.row[1];
+        }
     }
     // L * scale of the rows against columns col0..col0+15. pw1: the powers, one place on, so that pairs stand on 8 bytes
     __device__ __forceinline__ void factors(float (&f)[2][4], int col0, const float* pw1, const Decay<UP>& dec) const {
@@ -525,8 +554,7 @@ __global__ void __launch_bounds__(Shape<T, D>::NT, MINB) k_attn_bwd(const FmeDec
     constexpr int C = Z::C, NT = Z::NT, NC = Z::NC;
     extern __shared__ __align__(1024) char sm[];
     const Ti tq(sm), tg(sm + Z::TILE), tk(sm + 2 * Z::TILE), tv(sm + 3 * Z::TILE), ts(sm + 4 * Z::TILE), tu(sm + 4 * Z::TILE + Z::MAT);
-    char* stage = sm + 4 * Z::TILE + 2 * Z::MAT + (threadIdx.x >> 5) * Z::BWD_STAGE;
-    float* pw = reinterpret_cast<float*>(sm + (LOCAL ? 2 * Z::TILE : 4 * Z::TILE + 2 * Z::MAT + Z::NW * Z::BWD_STAGE));
+    float* pw = reinterpret_cast<float*>(sm + (LOCAL ? 2 * Z::TILE : 4 * Z::TILE + 2 * Z::MAT));
     float *pw1 = pw + 72, *a = pw + 144;
     const int warp = threadIdx.x >> 5, l = threadIdx.x & 31, g = l >> 2;
     const Spot P(A, LOCAL ? W.segs - 1 : W.segs);
@@ -584,8 +612,7 @@ __global__ void __launch_bounds__(Shape<T, D>::NT, MINB) k_attn_bwd(const FmeDec
             const int r0 = row0 + g, r1 = r0 + 8;
             auto put = [&](const float (&acc)[NC / 8][4], const FmeAttnTensor& x) {
                 again |= not_finite(acc);
-                if constexpr (sizeof(T) == 2) put_rows<NC>(acc, at<T>(x, n, h), x.st, row0, col0, t0, cuts.n);
-                else store_rows<T, NC>(stage, acc, at<T>(x, n, h), x.st, row0, col0, t0, cuts.n);
+                put_rows<NC>(acc, at<T>(x, n, h), x.st, row0, col0, t0, cuts.n);
             };
             float acc[NC / 8][4];
             {
@@ -806,7 +833,7 @@ template <typename T, int D> struct Plan {
     int64_t ws_bytes() const { return W.segs > 1 ? pairs * (W.segs - 1) * (4 * D * D + 4) : 0; }
     int64_t saved_bytes() const { return W.chunks > 1 ? pairs * (W.chunks - 1) * D * D * (int64_t)sizeof(T) : 0; }
     static constexpr int FLOAT_BYTES = Z::FLOATS * 4;
-    static constexpr int FWD = 3 * Z::TILE + Z::MAT + FLOAT_BYTES, BWD = 4 * Z::TILE + 2 * Z::MAT + Z::NW * Z::BWD_STAGE + FLOAT_BYTES;
+    static constexpr int FWD = 3 * Z::TILE + Z::MAT + FLOAT_BYTES, BWD = 4 * Z::TILE + 2 * Z::MAT + FLOAT_BYTES;
     static constexpr int LOCAL_FWD = 4 * Z::TILE + FLOAT_BYTES, LOCAL_BWD = 2 * Z::TILE + FLOAT_BYTES;
 };
 // CTAs an SM that the registers are bounded for: what shared memory allows, and no more than keeps the accumulators in registers

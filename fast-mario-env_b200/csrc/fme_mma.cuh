@@ -41,11 +41,11 @@ template <typename T, int COLS> struct Tile {
         const uint32_t sw = ROW >= 128 ? (uint32_t)(row & 7) : (uint32_t)((row >> 1) & 3);
         return (uint32_t)row * ROW + ((piece ^ sw) << 4) + in;
     }
-    // A lane's address of piece x (0 or 1) of a row, and from there the same piece `bytes` (a multiple of 32) further along the
-    // row: the permutation is an exclusive or within 128 bytes, so that one instruction moves on
-    __device__ __forceinline__ uint32_t lane(int row, int x) const {
-        const uint32_t sw = ROW >= 128 ? (uint32_t)(row & 7) : (uint32_t)((row >> 1) & 3);
-        return base + (uint32_t)row * ROW + (((uint32_t)x ^ sw) << 4);
+    // A lane's address of piece x (0 or 1) of row + its own row (row a multiple of 8, so that the permutation does not depend on
+    // it), and from there the same piece `bytes` (a multiple of 32) further along the row: an exclusive or within 128 bytes
+    __device__ __forceinline__ uint32_t lane(int row, int own, int x) const {
+        const uint32_t sw = ROW >= 128 ? (uint32_t)(own & 7) : (uint32_t)((own >> 1) & 3);
+        return base + (uint32_t)row * ROW + ((uint32_t)own * ROW + (((uint32_t)x ^ sw) << 4));
     }
     static __device__ __forceinline__ uint32_t along(uint32_t lane, int bytes) { return (lane ^ ((uint32_t)bytes & 127u)) + ((uint32_t)bytes & ~127u); }
     __device__ __forceinline__ T& at(int row, int col) const { return *reinterpret_cast<T*>(gen + off(row, col)); }
@@ -93,7 +93,7 @@ template <> struct Frag<bf16> {
     // 16 x 16 accumulators to a tile
     template <int COLS> static __device__ __forceinline__ void put16(const Tile<bf16, COLS>& s, int row, int col, const float* u, const float* v) {
         const int l = threadIdx.x & 31;
-        stsm4(s.along(s.lane(row + (l & 15), l >> 4), 2 * col), pack2(u[0], u[1]), pack2(u[2], u[3]), pack2(v[0], v[1]), pack2(v[2], v[3]));
+        stsm4(s.along(s.lane(row, l & 15, l >> 4), 2 * col), pack2(u[0], u[1]), pack2(u[2], u[3]), pack2(v[0], v[1]), pack2(v[2], v[3]));
     }
     static __device__ __forceinline__ void mma(float (&d)[4], const A& a, const B& b) {
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -108,28 +108,28 @@ template <> struct Frag<bf16> {
     template <int COLS> static __device__ __forceinline__ A ldA(const Tile<bf16, COLS>& s, int m, int k) {
         const int l = threadIdx.x & 31;
         A a;
-        ldsm4(a.r, s.along(s.lane(m + (l & 15), l >> 4), 2 * k));
+        ldsm4(a.r, s.along(s.lane(m, l & 15, l >> 4), 2 * k));
         return a;
     }
     // B[k][n] = tile[n][k], 16 columns n
     template <int COLS> static __device__ __forceinline__ void ldB(const Tile<bf16, COLS>& s, int n, int k, B& b0, B& b1) {
         const int l = threadIdx.x & 31;
         uint32_t r[4];
-        ldsm4(r, s.along(s.lane(n + (l & 7) + ((l >> 4) << 3), (l >> 3) & 1), 2 * k));
+        ldsm4(r, s.along(s.lane(n, (l & 7) + ((l >> 4) << 3), (l >> 3) & 1), 2 * k));
         b0.r[0] = r[0]; b0.r[1] = r[1]; b1.r[0] = r[2]; b1.r[1] = r[3];
     }
     // B[k][n] = tile[k][n], 16 columns n
     template <bool NAT, int COLS> static __device__ __forceinline__ void ldBt(const Tile<bf16, COLS>& s, int k, int n, B& b0, B& b1) {
         const int l = threadIdx.x & 31;
         uint32_t r[4];
-        ldsm4t(r, s.along(s.lane(k + (l & 15), l >> 4), 2 * n));
+        ldsm4t(r, s.along(s.lane(k, l & 15, l >> 4), 2 * n));
         b0.r[0] = r[0]; b0.r[1] = r[1]; b1.r[0] = r[2]; b1.r[1] = r[3];
     }
     // A[m][k] = weight[k] * tile[k][m], weights in shared memory
     template <int COLS> static __device__ __forceinline__ A2 ldAt(const Tile<bf16, COLS>& s, int k, int m, const float* w, bool fine) {
         const int l = threadIdx.x & 31;
         A2 a;
-        ldsm4t(a.hi.r, s.along(s.lane(k + (l & 7) + ((l >> 4) << 3), (l >> 3) & 1), 2 * m));
+        ldsm4t(a.hi.r, s.along(s.lane(k, (l & 7) + ((l >> 4) << 3), (l >> 3) & 1), 2 * m));
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const float2 v = unpack2(a.hi.r[i]), f = *reinterpret_cast<const float2*>(w + k + ((i >> 1) << 3) + 2 * (l & 3));
@@ -187,7 +187,7 @@ template <> struct Frag<float> {
     template <int COLS> static __device__ __forceinline__ A ldA(const Tile<float, COLS>& s, int m, int k) {
         const int l = threadIdx.x & 31;
         uint32_t r[4];
-        ldsm4(r, s.along(s.lane(m + (l & 15), l >> 4), 4 * k));
+        ldsm4(r, s.along(s.lane(m, l & 15, l >> 4), 4 * k));
         A a;
 #pragma unroll
         for (int i = 0; i < 4; i++) split_tf32(__uint_as_float(r[i]), a.hi[i], a.lo[i]);
@@ -196,7 +196,7 @@ template <> struct Frag<float> {
     template <int COLS> static __device__ __forceinline__ void ldB(const Tile<float, COLS>& s, int n, int k, B& b0, B& b1) {
         const int l = threadIdx.x & 31;
         uint32_t r[4];
-        ldsm4(r, s.along(s.lane(n + (l & 7) + ((l >> 4) << 3), (l >> 3) & 1), 4 * k));
+        ldsm4(r, s.along(s.lane(n, (l & 7) + ((l >> 4) << 3), (l >> 3) & 1), 4 * k));
 #pragma unroll
         for (int i = 0; i < 2; i++) {
             split_tf32(__uint_as_float(r[i]), b0.hi[i], b0.lo[i]);
@@ -213,7 +213,7 @@ template <> struct Frag<float> {
         const int g = (threadIdx.x & 31) >> 2;
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-            const uint32_t at = s.lane(k + row_of<NAT>(i), g >> 2) + 4 * (g & 3);
+            const uint32_t at = s.lane(k, row_of<NAT>(i), g >> 2) + 4 * (g & 3);
             split_tf32(lds(s.along(at, 4 * n)), b0.hi[i], b0.lo[i]);
             split_tf32(lds(s.along(at, 4 * n + 32)), b1.hi[i], b1.lo[i]);
         }
@@ -223,8 +223,8 @@ template <> struct Frag<float> {
         A a;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const int row = k + row_of<false>(i >> 1);
-            split_tf32(lds(s.along(s.lane(row, g >> 2) + 4 * (g & 3), 4 * (m + 8 * (i & 1)))) * w[row], a.hi[i], a.lo[i]);
+            const int own = row_of<false>(i >> 1);
+            split_tf32(lds(s.along(s.lane(k, own, g >> 2) + 4 * (g & 3), 4 * (m + 8 * (i & 1)))) * w[k + own], a.hi[i], a.lo[i]);
         }
         return a;
     }
