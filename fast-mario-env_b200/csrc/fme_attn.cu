@@ -32,7 +32,7 @@ template <typename T, int D> struct Shape {
     static constexpr int NW = D / 16, NT = 32 * NW, RB = C / 16, CG = NW / RB, NC = D / CG;
     static constexpr int TILE = C * D * (int)sizeof(T), MAT = D * D * (int)sizeof(T);
     static constexpr int STAGE = 16 * NC * (int)sizeof(T);   // a warp's outputs on their way out
-    static constexpr int FLOATS = 3 * 72;                    // powers, powers one place on, weights
+    static constexpr int FLOATS = 2 * 72;                    // powers and weights
 };
 
 // Where a chunk restarts. Bit i: token i does; valid tokens only.
@@ -42,10 +42,6 @@ struct Cuts {
     __device__ __forceinline__ int last_up_to(int i) const {   // latest restart at or before i, -1: none
         const uint64_t x = m & (~0ull >> (63 - i));
         return 63 - __clzll((long long)x);
-    }
-    __device__ __forceinline__ int next_after(int j) const {   // earliest restart after j, 64: none
-        const uint64_t x = j >= 63 ? 0ull : m & (~0ull << (j + 1));
-        return x ? __ffsll((long long)x) - 1 : 64;
     }
 };
 
@@ -94,12 +90,12 @@ __device__ __forceinline__ void store_rows(char* stage, const float (&acc)[NC / 
 #pragma unroll
     for (int i = 0; i < NC / 8; i += 2) Frag<T>::put16(s, 0, 8 * i, acc[i], acc[i + 1]);
     __syncwarp();
-    constexpr int PIECES = NC / Tile<T, PW>::PER;
+    constexpr int PIECES = NC / Tile<T, PW>::PER, STEP = 32 / PIECES;   // STEP: rows between a lane's pieces
+    const int row = l / PIECES, col = (l % PIECES) * Tile<T, PW>::PER;
+    T* p = dst + (t0 + row0 + row) * st + col0 + col;
 #pragma unroll
-    for (int i = 0; i < 16 * PIECES / 32; i++) {
-        const int e = i * 32 + l, row = e / PIECES, col = (e % PIECES) * Tile<T, PW>::PER;
-        if (row0 + row < n)
-            *reinterpret_cast<uint4*>(dst + (t0 + row0 + row) * st + col0 + col) = *reinterpret_cast<const uint4*>(s.gen + s.off(row, col));
+    for (int i = 0; i < 16 / STEP; i++) {
+        if (row0 + row + i * STEP < n) *reinterpret_cast<uint4*>(p + i * STEP * st) = *reinterpret_cast<const uint4*>(s.gen + s.off(row + i * STEP, col));
     }
     __syncwarp();
 }
@@ -200,73 +196,91 @@ __device__ __forceinline__ void product(float (&acc)[NB][4], const Left<T, D>& a
     for (int k = sizeof(T) == 2 ? F::KS : 0; k < D; k += F::KS) step(k, std::false_type{});
 }
 
-// A warp's factors of L * scale: within the 16 x 16 block on the diagonal as they are (0 above it), elsewhere
-// lambda^(i-j) = lambda^(i-edge) lambda^(edge-j) with the edge between the block's rows and the column: neither power grows.
-// UP: rows are i, columns j; otherwise rows are j and columns i.
-template <bool UP> struct Decay {
-    float diag[2][4], row[2];
-    __device__ __forceinline__ Decay(const float* pw, float scale) {
-        const int l = threadIdx.x & 31, g = l >> 2, c = l & 3;
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            row[h] = pw[UP ? g + 8 * h : 15 - g - 8 * h] * scale;
-#pragma unroll
-            for (int i = 0; i < 2; i++)
-#pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    const int far = (g + 8 * h) - (8 * i + 2 * c + e), d = UP ? far : -far;
-                    diag[i][2 * h + e] = d >= 0 ? pw[d < 0 ? 0 : d] * scale : 0.f;
-                }
-        }
-    }
-};
-
-// What a warp's rows row0..row0+15 of a chunk's L come from: the latest restart up to each row (UP) or the next one after it.
-// No restart in (j, i] means none in (j, edge] and none in (edge, i]: outside the diagonal's block the mask is a product too.
-template <bool UP> struct Mask {
-    int row0, lim0, lim1, lim;
-    float r0, r1;
-    __device__ __forceinline__ Mask(const Cuts& cuts, int row0_, const Decay<UP>& dec) : row0(row0_) {
-        // restarts within the sixteen rows, and the nearest one outside them
+// A warp's factors of L * scale for rows row0..row0+15 of a chunk, block of 16 columns by block. UP: rows are i, columns j, from the
+// diagonal down to column 0; otherwise rows are j and columns i, from the diagonal up. On the diagonal the factors are as they are.
+// Elsewhere lambda^(i-j) = lambda^(i-edge) lambda^(edge-j) with the edge between rows and column, so that neither power grows, and
+// from one block to the next the column's part takes lambda^16. No restart in (j, i] means none in (j, edge] and none in
+// (edge, i]: the mask is a product too, and blocks beyond the nearest restart outside the sixteen rows are not visited.
+template <bool UP, int C> struct Decay {
+    int row0, lim0, lim1, lim;   // lim: the nearest restart outside the rows, lim0 and lim1 for rows g and g + 8
+    uint32_t own;                // restarts within the rows
+    __device__ __forceinline__ Decay(const Cuts& cuts, int row0_) : row0(row0_) {
         const int g = (threadIdx.x & 31) >> 2;
-        const uint32_t own = (uint32_t)(cuts.m >> row0) & 0xffffu;
+        own = (uint32_t)(cuts.m >> row0) & 0xffffu;
         if (UP) {
             const uint64_t below = cuts.m & ~(~0ull << row0);
-            const int out = 63 - __clzll((long long)below);
             const uint32_t x0 = own & (0x1ffu >> (8 - g)), x1 = own & (0x1ffffu >> (8 - g));
-            lim = own & 1 ? row0 : out;
-            lim0 = x0 ? row0 + 31 - __clz(x0) : out;
-            lim1 = x1 ? row0 + 31 - __clz(x1) : out;
-            r0 = lim0 <= row0 ? dec.row[0] : 0.f;
-            r1 = lim1 <= row0 ? dec.row[1] : 0.f;
+            lim = 63 - __clzll((long long)below);
+            lim0 = x0 ? row0 + 31 - __clz(x0) : lim;
+            lim1 = x1 ? row0 + 31 - __clz(x1) : lim;
         } else {
             const uint64_t above = row0 + 16 >= 64 ? 0ull : cuts.m >> (row0 + 16);
             const uint32_t x0 = own >> (g + 1), x1 = own >> (g + 9);
             lim = above ? row0 + 15 + __ffsll((long long)above) : 64;
             lim0 = x0 ? row0 + g + __ffs(x0) : lim;
             lim1 = x1 ? row0 + g + 8 + __ffs(x1) : lim;
-            r0 = x0 ? 0.f : dec.row[0];
-            r1 = x1 ? 0.f : dec.row[1];
         }
     }
-    // L * scale of the rows against columns col0..col0+15. pw1: the powers, one place on, so that pairs stand on 8 bytes
-    __device__ __forceinline__ void factors(float (&f)[2][4], int col0, const float* pw1, const Decay<UP>& dec) const {
-        const int c = 2 * (threadIdx.x & 3);
-        if (col0 == row0) {
+    __device__ __forceinline__ void diagonal(float (&f)[2][4], const float* pw, float scale) const {
+        const int l = threadIdx.x & 31, g = l >> 2, c = 2 * (l & 3);
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int row = g + 8 * (j >> 1), col = 8 * i + c + (j & 1), d = UP ? row - col : col - row;
+                f[i][j] = d >= 0 ? pw[d < 0 ? 0 : d] * scale : 0.f;
+            }
+        if (own) {
 #pragma unroll
             for (int i = 0; i < 2; i++)
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    const int at = col0 + 8 * i + c + (j & 1), l = j < 2 ? lim0 : lim1;
-                    f[i][j] = (UP ? at >= l : at < l) ? dec.diag[i][j] : 0.f;
+                    const int at = row0 + 8 * i + c + (j & 1), l = j < 2 ? lim0 : lim1;
+                    f[i][j] = (UP ? at >= l : at < l) ? f[i][j] : 0.f;
                 }
-        } else {
+        }
+    }
+    // The rows' parts, and the columns' in the block next to the diagonal
+    __device__ __forceinline__ void beside(float (&rows)[2], float (&cols)[2][2], const float* pw, float scale) const {
+        const int l = threadIdx.x & 31, g = l >> 2, c = 2 * (l & 3);
+        const bool in0 = UP ? lim0 < row0 : lim0 > row0 + 15, in1 = UP ? lim1 < row0 : lim1 > row0 + 15;
+        rows[0] = in0 ? pw[UP ? g : 15 - g] * scale : 0.f;
+        rows[1] = in1 ? pw[UP ? g + 8 : 7 - g] * scale : 0.f;
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) cols[i][e] = pw[UP ? 16 - 8 * i - c - e : 1 + 8 * i + c + e];
+    }
+    // Columns beyond the nearest restart, in the block that holds it
+    __device__ __forceinline__ void cut(float (&x)[2][2], int col0) const {
+        const int c = 2 * (threadIdx.x & 3);
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const int at = col0 + 8 * i + c + e;
+                x[i][e] = (UP ? at >= lim : at < lim) ? x[i][e] : 0.f;
+            }
+    }
+    // f(col0, factors) for every block that the mask leaves
+    template <typename F> __device__ __forceinline__ void blocks(const float* pw, float scale, F f) const {
+        float w[2][4], rows[2], cols[2][2];
+        diagonal(w, pw, scale);
+        beside(rows, cols, pw, scale);
+        const float step = pw[16];
+        const int last = UP ? (lim < 0 ? 0 : lim & ~15) : (lim > C ? C : lim) - 1;   // a column of the last block
+#pragma unroll 1
+        for (int col0 = row0;;) {   // one copy of f: the code has to stay in the instruction cache
+            f(col0, w);
+            col0 += UP ? -16 : 16;
+            if (UP ? col0 < last : col0 > last) break;
+            float x[2][2] = {{cols[0][0], cols[0][1]}, {cols[1][0], cols[1][1]}};
+            if (UP ? col0 < lim : col0 + 16 > lim) cut(x, col0);
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                const int col = col0 + 8 * i + c;
-                const float2 e = *reinterpret_cast<const float2*>(pw1 + (UP ? row0 - col : col - row0 - 14));
-                const float x = (UP ? col >= lim : col < lim) ? (UP ? e.y : e.x) : 0.f, y = (UP ? col + 1 >= lim : col + 1 < lim) ? (UP ? e.x : e.y) : 0.f;
-                f[i][0] = x * r0; f[i][1] = y * r0; f[i][2] = x * r1; f[i][3] = y * r1;
+#pragma unroll
+                for (int j = 0; j < 4; j++) w[i][j] = x[i][j & 1] * rows[j >> 1];
+                cols[i][0] *= step; cols[i][1] *= step;
             }
         }
     }
@@ -420,8 +434,8 @@ struct Spot {
     }
 };
 
-__device__ __forceinline__ void powers(float* pw, float* pw1, int n, float log2_lam) {
-    for (int i = threadIdx.x; i < n; i += blockDim.x) pw[i] = pw1[i + 1] = i ? exp2f(log2_lam * (float)i) : 1.f;
+__device__ __forceinline__ void powers(float* pw, int n, float log2_lam) {
+    for (int i = threadIdx.x; i < n; i += blockDim.x) pw[i] = i ? exp2f(log2_lam * (float)i) : 1.f;
 }
 
 constexpr float LOG2E = 1.44269504088896340736f;
@@ -437,7 +451,7 @@ __global__ void __launch_bounds__(Shape<T, D>::NT, MINB) k_attn_fwd(const FmeDec
     constexpr int SET = (LOCAL ? 2 : 3) * Z::TILE;
     const Ti ts(sm + STAGES * SET);
     float* pw = reinterpret_cast<float*>(sm + STAGES * SET + (LOCAL ? 0 : Z::MAT));   // C + 1
-    float *pw1 = pw + 72, *z = pw + 144;                                                      // C + 2, C
+    float* z = pw + 72;                                                                       // C
     const int warp = threadIdx.x >> 5, l = threadIdx.x & 31, g = l >> 2;
     const Spot P(A, LOCAL ? W.segs - 1 : W.segs);
     const int seg = P.seg, h = P.h, n = P.n;
@@ -458,9 +472,8 @@ __global__ void __launch_bounds__(Shape<T, D>::NT, MINB) k_attn_fwd(const FmeDec
         rb.load(A.reset ? A.reset + n * A.reset_sn : nullptr, A.reset_st, t0, nv);
     };
     if (c0 < c1) fetch(c0);
-    powers(pw, pw1, C + 1, g2);
+    powers(pw, C + 1, g2);
     __syncthreads();
-    const Decay<true> dec(pw, A.scale);
     const int64_t pair = (int64_t)n * A.h + h;
     some = true;
     if (LOCAL) let_next_start();
@@ -493,14 +506,12 @@ __global__ void __launch_bounds__(Shape<T, D>::NT, MINB) k_attn_fwd(const FmeDec
                 const bool in0 = cuts.last_up_to(row0 + g) < 0, in1 = cuts.last_up_to(row0 + g + 8) < 0;
                 weigh(acc, in0 ? pw[row0 + g + 1] * A.scale : 0.f, in1 ? pw[row0 + g + 9] * A.scale : 0.f);
             } else zero(acc);
-            const Mask<true> mask(cuts, row0, dec);
-#pragma unroll 1
-            for (int j = 0; j <= row0; j += 16) {
-                float p[2][4], f[2][4];
-                mask.factors(f, j, pw1, dec);
+            const Decay<true, C> decay(cuts, row0);
+            decay.blocks(pw, A.scale, [&](int j, const float (&f)[2][4]) {
+                float p[2][4];
                 block_scores<T, D>(p, lq, tk, j, f);
                 block_apply<T, D>(acc, p, tv, j, col0);
-            }
+            });
             again = __syncthreads_or(not_finite(acc));
             // q and the old state have been read by all: the q tile takes the outputs
             if (!again) store_rows<T, NC>(set + 2 * Z::TILE + warp * Z::STAGE, acc, at<T>(A.o, n, h), A.o.st, row0, col0, t0, cuts.n);
@@ -555,7 +566,7 @@ __global__ void __launch_bounds__(Shape<T, D>::NT, MINB) k_attn_bwd(const FmeDec
     extern __shared__ __align__(1024) char sm[];
     const Ti tq(sm), tg(sm + Z::TILE), tk(sm + 2 * Z::TILE), tv(sm + 3 * Z::TILE), ts(sm + 4 * Z::TILE), tu(sm + 4 * Z::TILE + Z::MAT);
     float* pw = reinterpret_cast<float*>(sm + (LOCAL ? 2 * Z::TILE : 4 * Z::TILE + 2 * Z::MAT));
-    float *pw1 = pw + 72, *a = pw + 144;
+    float* a = pw + 72;
     const int warp = threadIdx.x >> 5, l = threadIdx.x & 31, g = l >> 2;
     const Spot P(A, LOCAL ? W.segs - 1 : W.segs);
     const int rseg = P.seg, seg = W.segs - 1 - rseg, h = P.h, n = P.n;   // rseg 0: the last in time
@@ -589,7 +600,7 @@ __global__ void __launch_bounds__(Shape<T, D>::NT, MINB) k_attn_bwd(const FmeDec
         if (!LOCAL) fetch_keys(c);
     };
     if (c0 < c1) fetch(c1 - 1);
-    powers(pw, pw1, C + 1, g2);
+    powers(pw, C + 1, g2);
     const int64_t pair = (int64_t)n * A.h + h;
     some = true;
     if (LOCAL) let_next_start();
@@ -618,42 +629,36 @@ __global__ void __launch_bounds__(Shape<T, D>::NT, MINB) k_attn_bwd(const FmeDec
             {
                 const bool z0 = r0 >= last && r0 < cuts.n, z1 = r1 >= last && r1 < cuts.n;
                 const float w0 = z0 ? pw[cuts.n - 1 - r0] : 0.f, w1 = z1 ? pw[cuts.n - 1 - r1] : 0.f;
-                const Decay<false> down(pw, A.scale);
-                const Mask<false> mask(cuts, row0, down);
+                const Decay<false, C> down(cuts, row0);
                 // dv, then dk: the same with k and v, q and do in each other's place
-#pragma unroll
+#pragma unroll(sizeof(T) == 2 ? 2 : 1)
                 for (int which = 0; which < 2; which++) {
-                    const Ti &rows = which ? tv : tk, &cols = which ? tg : tq, &other = which ? tq : tg;
+                    const Ti rows = which ? tv : tk, cols = which ? tg : tq, other = which ? tq : tg;
                     const Left<T, D> left(rows, row0);
                     if (some) {
                         if (which) product<T, NC / 8, D, false>(acc, left, tu, col0);
                         else product<T, NC / 8, D, true>(acc, left, tu, col0);
                         weigh(acc, w0, w1);
                     } else zero(acc);
-#pragma unroll 1
-                    for (int i = row0; i < C; i += 16) {
-                        float p[2][4], f[2][4];
-                        mask.factors(f, i, pw1, down);
+                    down.blocks(pw, A.scale, [&](int i, const float (&f)[2][4]) {
+                        float p[2][4];
                         block_scores<T, D>(p, left, cols, i, f);
                         block_apply<T, D>(acc, p, other, i, col0);
-                    }
+                    });
                     put(acc, which ? A.dk : A.dv);
                 }
             }
-            const Decay<true> up(pw, A.scale);
-            const Mask<true> mask(cuts, row0, up);
+            const Decay<true, C> up(cuts, row0);
             const Left<T, D> lg(tg, row0);
             if (before) {
                 product<T, NC / 8, D, true>(acc, lg, ts, col0);
                 weigh(acc, cuts.last_up_to(r0) < 0 ? pw[r0 + 1] * A.scale : 0.f, cuts.last_up_to(r1) < 0 ? pw[r1 + 1] * A.scale : 0.f);
             } else zero(acc);
-#pragma unroll 1
-            for (int j = 0; j <= row0; j += 16) {
-                float p[2][4], f[2][4];
-                mask.factors(f, j, pw1, up);
+            up.blocks(pw, A.scale, [&](int j, const float (&f)[2][4]) {
+                float p[2][4];
                 block_scores<T, D>(p, lg, tv, j, f);
                 block_apply<T, D>(acc, p, tk, j, col0);
-            }
+            });
             put(acc, A.dq);
         }
         const bool more = c > c0;
