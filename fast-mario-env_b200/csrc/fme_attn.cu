@@ -79,6 +79,28 @@ __device__ __forceinline__ void load_tile(const Tile<T, D>& dst, const T* src, i
     }
 }
 
+// Sixteen rows (n of them valid) of a tile to global memory, a row's pieces as 16 bytes each
+template <typename TI, int COLS, typename T> __device__ __forceinline__ void copy_rows(const TI& s, int from, T* dst, int64_t st, int n) {
+    constexpr int PIECES = COLS / TI::PER, STEP = 32 / PIECES;   // STEP: rows between a lane's pieces
+    const int l = threadIdx.x & 31, row = l / PIECES, piece = l % PIECES;
+    const uint32_t a = s.lane(from, row, piece);
+    T* p = dst + row * st + piece * TI::PER;
+    auto one = [&](int i) {   // i * STEP further down the permutation differs in bits that row does not have
+        uint4 v;
+        const uint32_t at = (TI::ROW >= 128 ? a ^ (((i * STEP) & 7) << 4) : a) + i * STEP * TI::ROW;
+        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+        *reinterpret_cast<uint4*>(p + i * STEP * st) = v;
+    };
+    if (n >= 16) {
+#pragma unroll
+        for (int i = 0; i < 16 / STEP; i++) one(i);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16 / STEP; i++)
+            if (row + i * STEP < n) one(i);
+    }
+}
+
 // A warp's 16 x NC accumulators to rows row0.. and columns col0.. of a (t, h, d) output: through shared memory, so that a row's
 // pieces leave as 16 bytes each
 template <typename T, int NC>
@@ -86,17 +108,10 @@ __device__ __forceinline__ void store_rows(char* stage, const float (&acc)[NC / 
     constexpr int PW = NC < 32 ? 32 : NC;
     static_assert(NC >= 32, "");
     const Tile<T, PW> s(stage);
-    const int l = threadIdx.x & 31;
 #pragma unroll
     for (int i = 0; i < NC / 8; i += 2) Frag<T>::put16(s, 0, 8 * i, acc[i], acc[i + 1]);
     __syncwarp();
-    constexpr int PIECES = NC / Tile<T, PW>::PER, STEP = 32 / PIECES;   // STEP: rows between a lane's pieces
-    const int row = l / PIECES, col = (l % PIECES) * Tile<T, PW>::PER;
-    T* p = dst + (t0 + row0 + row) * st + col0 + col;
-#pragma unroll
-    for (int i = 0; i < 16 / STEP; i++) {
-        if (row0 + row + i * STEP < n) *reinterpret_cast<uint4*>(p + i * STEP * st) = *reinterpret_cast<const uint4*>(s.gen + s.off(row + i * STEP, col));
-    }
+    copy_rows<Tile<T, PW>, NC>(s, 0, dst + (t0 + row0) * st + col0, st, n - row0);
     __syncwarp();
 }
 
@@ -514,7 +529,10 @@ __global__ void __launch_bounds__(Shape<T, D>::NT, MINB) k_attn_fwd(const FmeDec
             });
             again = __syncthreads_or(not_finite(acc));
             // q and the old state have been read by all: the q tile takes the outputs
-            if (!again) store_rows<T, NC>(set + 2 * Z::TILE + warp * Z::STAGE, acc, at<T>(A.o, n, h), A.o.st, row0, col0, t0, cuts.n);
+            if (!again) {
+                if constexpr (sizeof(T) == 2) store_rows<T, NC>(set + 2 * Z::TILE + warp * Z::STAGE, acc, at<T>(A.o, n, h), A.o.st, row0, col0, t0, cuts.n);
+                else put_rows<NC>(acc, at<T>(A.o, n, h), A.o.st, row0, col0, t0, cuts.n);
+            }
         }
         const bool more = c + 1 < c1, save = A.saved && c + 1 < W.chunks;
         if (more || LOCAL || save || (A.s_out && c + 1 == W.chunks)) {
@@ -531,13 +549,7 @@ __global__ void __launch_bounds__(Shape<T, D>::NT, MINB) k_attn_fwd(const FmeDec
             if (more || save) put_state(ts, s, m0);
             if (save) {
                 __syncwarp();
-                T* dst = reinterpret_cast<T*>(A.saved) + ((pair * (W.chunks - 1) + c) * D + m0) * D;
-                constexpr int PIECES = D / Ti::PER;
-#pragma unroll
-                for (int i = 0; i < 16 * PIECES / 32; i++) {
-                    const int e = i * 32 + l, row = e / PIECES, col = (e % PIECES) * Ti::PER;
-                    *reinterpret_cast<uint4*>(dst + row * D + col) = *reinterpret_cast<const uint4*>(ts.gen + ts.off(m0 + row, col));
-                }
+                copy_rows<Ti, D>(ts, m0, reinterpret_cast<T*>(A.saved) + ((pair * (W.chunks - 1) + c) * D + m0) * D, (int64_t)D, 16);
             }
         }
         if (STAGES == 1 && more) {

@@ -285,6 +285,41 @@ def test_same_bits_again_and_on_another_stream():
         assert torch.equal(one[name], two[name]), name
 
 
+def test_operators_in_a_captured_graph():
+    """Acting and learning are captured by the trainers: the same bits as outside, on inputs that change between replays."""
+    n, t, h, d = 3, 600, 2, 64   # few rows: the joined segments are part of it
+    c = make(n, t, h, d, torch.bfloat16, 0.01, True, seed=18)
+    x, w, b, dy = norm_case((8, 16, 6, 6), 4, torch.float32, seed=18)
+    g, reset = c["g"].to(DEV), c["reset"].to(DEV)
+    q, k, v = (c[i].to(DEV).requires_grad_() for i in ("q", "k", "v"))
+    do, gx, gw, gb, gd = c["do"].to(DEV), last_dense(x.to(DEV)).requires_grad_(), w.to(DEV), b.to(DEV), last_dense(dy.to(DEV))
+    state = c["state"].to(DEV)
+
+    def work(s):
+        o, last = ops.decay_attention(q, k, v, g, reset=reset, state=c_state)
+        y = ops.group_norm_act(gx, 4, gw, gb, checkpoint="u8")
+        one = ops.decay_attention_step(q[:, 0].detach(), k[:, 0].detach(), v[:, 0].detach(), g, s, reset=reset[:, 0])
+        return (o, last, *torch.autograd.grad(o, (q, k, v), do), y, *torch.autograd.grad(y, gx, gd), one, s)
+
+    c_state, s = state.clone(), state.clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        work(s)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = work(s)
+    with torch.no_grad():
+        for i in (q, k, v, gx):
+            i.mul_(0.5)
+    s.copy_(state)
+    graph.replay()
+    got = [i.detach().clone() for i in out]
+    for a, b in zip(got, work(state.clone())):
+        assert torch.equal(a, b)
+
+
 def test_attention_refusals():
     q = torch.zeros(2, 4, 2, 64, device=DEV)
     g = torch.zeros(2, device=DEV)
