@@ -17,6 +17,7 @@ from functools import lru_cache
 
 import torch
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version
 
 from . import _native as N
 
@@ -196,8 +197,8 @@ def decay_attention_step(q, k, v, log_decay, state, *, reset=None, scale=None, o
     """One token of `decay_attention` for each of N envs, for acting: q, k, v (N, H, D), reset (N,), and state
     (N, H, D, D) float32 contiguous, which is updated in place. Returns o (N, H, D), in `out` where given. No gradient."""
     _check_qkv(q, k, v, log_decay, reset, state, 1)
-    if state is None or not state.is_contiguous():
-        raise ValueError("state must be contiguous: it is updated in place")
+    if state is None or not state.is_contiguous() or state.requires_grad:
+        raise ValueError("state must be contiguous and without a gradient: it is updated in place")
     n, h, d = q.shape
     if out is None:
         out = torch.empty((n, h, d), dtype=q.dtype, device=q.device)
@@ -209,6 +210,7 @@ def decay_attention_step(q, k, v, log_decay, state, *, reset=None, scale=None, o
     _call("fme_decay_attn_step",
           N.ATTN.pack(n, 1, h, d, _DTYPES[q.dtype], d ** -0.5 if scale is None else scale, *_t3(q), *_t3(k), *_t3(v), *_t3(out), log_decay.data_ptr(),
                       _ptr(reset), 0 if reset is None else reset.stride(0), 0, s, s, *_NO4, *_NO4, *_NO4, *_NO4, 0, 0, 0, 0, 0), q.get_device())
+    increment_version((state, out))   # a backward pass that kept either notices
     return out
 
 

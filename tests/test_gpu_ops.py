@@ -239,6 +239,16 @@ def test_step_with_strides_out_and_bad_values():
     assert state.isfinite().all()
 
 
+def test_a_state_that_a_backward_pass_needs_is_not_changed_unnoticed():
+    c = make(2, 5, 2, 64, torch.float32, None, True, seed=19)
+    q, k, v, g, s = (c[x].to(DEV) for x in ("q", "k", "v", "g", "state"))
+    q.requires_grad_()
+    o, _ = ops.decay_attention(q, k, v, g, state=s)
+    ops.decay_attention_step(q[:, 0].detach(), k[:, 0], v[:, 0], g, s)
+    with pytest.raises(RuntimeError, match="inplace"):
+        o.sum().backward()
+
+
 def test_empty_sequences():
     g = decays(2).to(DEV)
     z = torch.zeros(3, 0, 2, 64, device=DEV, requires_grad=True)
