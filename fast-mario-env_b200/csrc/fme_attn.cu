@@ -228,9 +228,9 @@ __device__ __forceinline__ void product(float (&acc)[NB][4], const Left<T, D>& a
 // from one block to the next the column's part takes lambda^16. No restart in (j, i] means none in (j, edge] and none in
 // (edge, i]: the mask is a product too, and blocks beyond the nearest restart outside the sixteen rows are not visited.
 template <bool UP, int C> struct Decay {
-    int row0, lim0, lim1, lim;   // lim: the nearest restart outside the rows, lim0 and lim1 for rows g and g + 8
+    int row0, n, lim0, lim1, lim;   // lim: the nearest restart outside the rows, lim0 and lim1 for rows g and g + 8
     uint32_t own;                // restarts within the rows
-    __device__ __forceinline__ Decay(const Cuts& cuts, int row0_) : row0(row0_) {
+    __device__ __forceinline__ Decay(const Cuts& cuts, int row0_) : row0(row0_), n(cuts.n) {
         const int g = (threadIdx.x & 31) >> 2;
         own = (uint32_t)(cuts.m >> row0) & 0xffffu;
         if (UP) {
@@ -294,7 +294,7 @@ template <bool UP, int C> struct Decay {
         diagonal(w, pw, scale);
         beside(rows, cols, pw, scale);
         const float step = pw[16];
-        const int last = UP ? (lim < 0 ? 0 : lim & ~15) : (lim > C ? C : lim) - 1;   // a column of the last block
+        const int last = UP ? (lim < 0 ? 0 : lim & ~15) : (lim > n ? n : lim) - 1;   // a column of the last block
 #pragma unroll 1
         for (int col0 = row0;;) {   // one copy of f: the code has to stay in the instruction cache
             f(col0, w);
@@ -529,21 +529,25 @@ __global__ void __launch_bounds__(Shape<T, D>::NT, MINB) k_attn_fwd(const FmeDec
         if constexpr (LOCAL) __syncthreads();
         if constexpr (!LOCAL) {
             float acc[NC / 8][4];
-            const Left<T, D> lq(tq, row0);
-            if (some) {
-                product<T, NC / 8, D, false>(acc, lq, ts, col0);
-                const bool in0 = cuts.last_up_to(row0 + g) < 0, in1 = cuts.last_up_to(row0 + g + 8) < 0;
-                weigh(acc, in0 ? pw[row0 + g + 1] * A.scale : 0.f, in1 ? pw[row0 + g + 9] * A.scale : 0.f);
-            } else zero(acc);
-            const Decay<true, C> decay(cuts, row0);
-            decay.blocks(pw, A.scale, [&](int j, const float (&f)[2][4]) {
-                float p[2][4];
-                block_scores<T, D>(p, lq, tk, j, f);
-                block_apply<T, D>(acc, p, tv, j, col0);
-            });
-            again = __syncthreads_or(not_finite(acc));
+            bool off = false;
+            if (row0 < cuts.n) {   // rows past the sequence's end have nothing to do
+                const Left<T, D> lq(tq, row0);
+                if (some) {
+                    product<T, NC / 8, D, false>(acc, lq, ts, col0);
+                    const bool in0 = cuts.last_up_to(row0 + g) < 0, in1 = cuts.last_up_to(row0 + g + 8) < 0;
+                    weigh(acc, in0 ? pw[row0 + g + 1] * A.scale : 0.f, in1 ? pw[row0 + g + 9] * A.scale : 0.f);
+                } else zero(acc);
+                const Decay<true, C> decay(cuts, row0);
+                decay.blocks(pw, A.scale, [&](int j, const float (&f)[2][4]) {
+                    float p[2][4];
+                    block_scores<T, D>(p, lq, tk, j, f);
+                    block_apply<T, D>(acc, p, tv, j, col0);
+                });
+                off = not_finite(acc);
+            }
+            again = __syncthreads_or(off);
             // q and the old state have been read by all: the q tile takes the outputs
-            if (!again) {
+            if (!again && row0 < cuts.n) {
                 if constexpr (sizeof(T) == 2) store_rows<T, NC>(set + 2 * Z::TILE + warp * Z::STAGE, acc, at<T>(A.o, n, h), A.o.st, row0, col0, t0, cuts.n);
                 else put_rows<NC>(acc, at<T>(A.o, n, h), A.o.st, row0, col0, t0, cuts.n);
             }
@@ -653,41 +657,43 @@ __global__ void __launch_bounds__(Shape<T, D>::NT, MINB) k_attn_bwd(const FmeDec
                 again |= not_finite(acc);
                 put_rows<NC>(acc, at<T>(x, n, h), x.st, row0, col0, t0, cuts.n);
             };
-            float acc[NC / 8][4];
-            {
-                const bool z0 = r0 >= last && r0 < cuts.n, z1 = r1 >= last && r1 < cuts.n;
-                const float w0 = z0 ? pw[cuts.n - 1 - r0] : 0.f, w1 = z1 ? pw[cuts.n - 1 - r1] : 0.f;
-                const Decay<false, C> down(cuts, row0);
-                // dv, then dk: the same with k and v, q and do in each other's place
+            if (row0 < cuts.n) {   // rows past the sequence's end have nothing to do
+                float acc[NC / 8][4];
+                {
+                    const bool z0 = r0 >= last && r0 < cuts.n, z1 = r1 >= last && r1 < cuts.n;
+                    const float w0 = z0 ? pw[cuts.n - 1 - r0] : 0.f, w1 = z1 ? pw[cuts.n - 1 - r1] : 0.f;
+                    const Decay<false, C> down(cuts, row0);
+                    // dv, then dk: the same with k and v, q and do in each other's place
 #pragma unroll(sizeof(T) == 2 ? 2 : 1)
-                for (int which = 0; which < 2; which++) {
-                    const Ti rows = which ? tv : tk, cols = which ? tg : tq, other = which ? tq : tg;
-                    const Left<T, D> left(rows, row0);
-                    if (some) {
-                        if (which) product<T, NC / 8, D, false>(acc, left, tu, col0);
-                        else product<T, NC / 8, D, true>(acc, left, tu, col0);
-                        weigh(acc, w0, w1);
-                    } else zero(acc);
-                    down.blocks(pw, A.scale, [&](int i, const float (&f)[2][4]) {
-                        float p[2][4];
-                        block_scores<T, D>(p, left, cols, i, f);
-                        block_apply<T, D>(acc, p, other, i, col0);
-                    });
-                    put(acc, which ? A.dk : A.dv);
+                    for (int which = 0; which < 2; which++) {
+                        const Ti rows = which ? tv : tk, cols = which ? tg : tq, other = which ? tq : tg;
+                        const Left<T, D> left(rows, row0);
+                        if (some) {
+                            if (which) product<T, NC / 8, D, false>(acc, left, tu, col0);
+                            else product<T, NC / 8, D, true>(acc, left, tu, col0);
+                            weigh(acc, w0, w1);
+                        } else zero(acc);
+                        down.blocks(pw, A.scale, [&](int i, const float (&f)[2][4]) {
+                            float p[2][4];
+                            block_scores<T, D>(p, left, cols, i, f);
+                            block_apply<T, D>(acc, p, other, i, col0);
+                        });
+                        put(acc, which ? A.dk : A.dv);
+                    }
                 }
+                const Decay<true, C> up(cuts, row0);
+                const Left<T, D> lg(tg, row0);
+                if (before) {
+                    product<T, NC / 8, D, true>(acc, lg, ts, col0);
+                    weigh(acc, cuts.last_up_to(r0) < 0 ? pw[r0 + 1] * A.scale : 0.f, cuts.last_up_to(r1) < 0 ? pw[r1 + 1] * A.scale : 0.f);
+                } else zero(acc);
+                up.blocks(pw, A.scale, [&](int j, const float (&f)[2][4]) {
+                    float p[2][4];
+                    block_scores<T, D>(p, lg, tv, j, f);
+                    block_apply<T, D>(acc, p, tk, j, col0);
+                });
+                put(acc, A.dq);
             }
-            const Decay<true, C> up(cuts, row0);
-            const Left<T, D> lg(tg, row0);
-            if (before) {
-                product<T, NC / 8, D, true>(acc, lg, ts, col0);
-                weigh(acc, cuts.last_up_to(r0) < 0 ? pw[r0 + 1] * A.scale : 0.f, cuts.last_up_to(r1) < 0 ? pw[r1 + 1] * A.scale : 0.f);
-            } else zero(acc);
-            up.blocks(pw, A.scale, [&](int j, const float (&f)[2][4]) {
-                float p[2][4];
-                block_scores<T, D>(p, lg, tv, j, f);
-                block_apply<T, D>(acc, p, tk, j, col0);
-            });
-            put(acc, A.dq);
         }
         const bool more = c > c0;
         const int j = threadIdx.x;
@@ -873,8 +879,8 @@ template <typename T, int D> struct Plan {
     static constexpr int LOCAL_FWD = 4 * Z::TILE + FLOAT_BYTES, LOCAL_BWD = 2 * Z::TILE + FLOAT_BYTES;
 };
 // CTAs an SM that the registers are bounded for: what shared memory allows, and no more than keeps the accumulators in registers
-template <typename T, int D> constexpr int fwd_ctas() { return D == 128 ? 1 : sizeof(T) == 4 ? 3 : D == 64 ? 4 : 8; }
-template <typename T, int D> constexpr int bwd_ctas() { return D == 128 ? 1 : sizeof(T) == 4 ? 2 : D == 64 ? 3 : 6; }
+template <typename T, int D> constexpr int fwd_ctas() { return D == 128 ? 1 : D == 32 ? 8 : sizeof(T) == 4 ? 3 : 4; }
+template <typename T, int D> constexpr int bwd_ctas() { return D == 128 ? 1 : D == 32 ? 6 : sizeof(T) == 4 ? 2 : 3; }
 template <typename T, int D> constexpr int local_ctas() { return D == 128 ? 1 : sizeof(T) == 4 ? 2 : 4; }
 
 template <typename K> int go(const char* what, K kernel, int64_t grid, int threads, int smem, cudaStream_t st, const FmeDecayAttn& a, const Walkers& W, bool behind = false) {
