@@ -16,8 +16,8 @@
 // thousand flops, so HBM is the floor and warp-level mma is enough for it: the tensor pipe is busy for 38 % of the time. What bounds the
 // kernels now is the rest of the instruction stream (issue slots 45 to 50 % used by 12 to 16 warps an SM, shared memory 52 to 65 %):
 // masks, rounding to operands, stores. Measured on a B200 (HBM copy 6441 GB/s), 1024 x 128 tokens of 8 heads of 64, restarts at 2 %:
-// bf16 forward 133 us (4.0 TB/s of the tensors above), backward 263 us (3.6 TB/s); fp32, 257 x 127 with states in and out: 185 and
-// 457 us, bound by its three tf32 products and the splitting of their operands (ALU 45 %, tensor 39 %).
+// bf16 forward 133 us (4.0 TB/s of the tensors above), backward 263 us (3.6 TB/s); fp32, 257 x 127 with states in and out: 640 us
+// both, backward 70 % of it, bound by its three tf32 products and the splitting of their operands (ALU 46 %, tensor 39 %).
 // Chunks of 64: with 128 (no state between two chunks of a 128-token rollout, more products within one) the same pass took 486
 // against 441 us. One CTA for each sequence and head: CTAs that walk several with the powers kept took 171 against 153 us forward.
 #include <math.h>
@@ -41,7 +41,6 @@ template <typename T, int D> struct Shape {
     static constexpr int C = D == 32 || (D == 128 && sizeof(T) == 4) ? 32 : 64;
     static constexpr int NW = D / 16, NT = 32 * NW, RB = C / 16, CG = NW / RB, NC = D / CG;
     static constexpr int TILE = C * D * (int)sizeof(T), MAT = D * D * (int)sizeof(T);
-    static constexpr int STAGE = 16 * NC * (int)sizeof(T);   // a warp's outputs on their way out
     static constexpr int FLOATS = 2 * 72;                    // powers and weights
 };
 
@@ -212,8 +211,8 @@ __device__ __forceinline__ void product(float (&acc)[NB][4], const Left<T, D>& a
             typename F::B b0, b1;
             if (TR) F::template ldBt<true>(b, k, n + 8 * i, b0, b1);
             else F::ldB(b, n + 8 * i, k, b0, b1);
-            if (decltype(first)::value) { F::mma0(acc[i], fa, b0); F::mma0(acc[i + 1], fa, b1); }
-            else { F::mma(acc[i], fa, b0); F::mma(acc[i + 1], fa, b1); }
+            F::template begin<decltype(first)::value>(acc[i], fa, b0);
+            F::template begin<decltype(first)::value>(acc[i + 1], fa, b1);
         }
     };
     if constexpr (sizeof(T) == 2) step(0, std::true_type{});
@@ -320,16 +319,34 @@ __device__ __forceinline__ void block_scores(float (&p)[2][4], const Left<T, D>&
         const typename F::A fa = a.get(0);
         typename F::B b0, b1;
         F::ldB(b, col0, 0, b0, b1);
-        F::mma0(p[0], fa, b0);
-        F::mma0(p[1], fa, b1);
+        F::template begin<true>(p[0], fa, b0);
+        F::template begin<true>(p[1], fa, b1);
     } else zero(p);
-#pragma unroll(sizeof(T) == 2 ? 8 : 2)
-    for (int k = sizeof(T) == 2 ? F::KS : 0; k < D; k += F::KS) {
-        const typename F::A fa = a.get(k);
-        typename F::B b0, b1;
-        F::ldB(b, col0, k, b0, b1);
-        F::mma(p[0], fa, b0);
-        F::mma(p[1], fa, b1);
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int k = F::KS; k < D; k += F::KS) {
+            const typename F::A fa = a.get(k);
+            typename F::B b0, b1;
+            F::ldB(b, col0, k, b0, b1);
+            F::mma(p[0], fa, b0);
+            F::mma(p[1], fa, b1);
+        }
+    } else {   // the products with a remainder are summed apart: an accumulator drops bits at its own size with each addition
+               // (error against 64 bits 6.7e-7 and not 8.3e-7, and the sums wait less for one another: 640 against 646 us, 257 x 127)
+        float r[2][4];
+        zero(r);
+#pragma unroll 2
+        for (int k = 0; k < D; k += F::KS) {
+            const typename F::A fa = a.get(k);
+            typename F::B b0, b1;
+            F::ldB(b, col0, k, b0, b1);
+            F::mma_apart(p[0], r[0], fa, b0);
+            F::mma_apart(p[1], r[1], fa, b1);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) p[i][j] += r[i][j];
     }
 #pragma unroll
     for (int i = 0; i < 2; i++)
@@ -548,7 +565,7 @@ __global__ void __launch_bounds__(Shape<T, D>::NT, MINB) k_attn_fwd(const FmeDec
             again = __syncthreads_or(off);
             // q and the old state have been read by all: the q tile takes the outputs
             if (!again && row0 < cuts.n) {
-                if constexpr (sizeof(T) == 2) store_rows<T, NC>(set + 2 * Z::TILE + warp * Z::STAGE, acc, at<T>(A.o, n, h), A.o.st, row0, col0, t0, cuts.n);
+                if constexpr (sizeof(T) == 2) store_rows<T, NC>(set + 2 * Z::TILE + warp * (16 * NC * (int)sizeof(T)), acc, at<T>(A.o, n, h), A.o.st, row0, col0, t0, cuts.n);
                 else put_rows<NC>(acc, at<T>(A.o, n, h), A.o.st, row0, col0, t0, cuts.n);
             }
         }

@@ -99,10 +99,12 @@ template <> struct Frag<bf16> {
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a.r[0]), "r"(a.r[1]), "r"(a.r[2]), "r"(a.r[3]), "r"(b.r[0]), "r"(b.r[1]));
     }
-    // d = a b
-    static __device__ __forceinline__ void mma0(float (&d)[4], const A& a, const B& b) {
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-                     : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a.r[0]), "r"(a.r[1]), "r"(a.r[2]), "r"(a.r[3]), "r"(b.r[0]), "r"(b.r[1]), "f"(0.f));
+    // d = a b where FIRST, else d += a b
+    template <bool FIRST> static __device__ __forceinline__ void begin(float (&d)[4], const A& a, const B& b) {
+        if constexpr (FIRST)
+            asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a.r[0]), "r"(a.r[1]), "r"(a.r[2]), "r"(a.r[3]), "r"(b.r[0]), "r"(b.r[1]), "f"(0.f));
+        else mma(d, a, b);
     }
     // A[m][k] = tile[m][k]
     template <int COLS> static __device__ __forceinline__ A ldA(const Tile<bf16, COLS>& s, int m, int k) {
@@ -168,13 +170,6 @@ template <> struct Frag<float> {
         s.put2(row + g, col + 8 + c, v[0], v[1]);
         s.put2(row + g + 8, col + 8 + c, v[2], v[3]);
     }
-    // d = a b
-    static __device__ __forceinline__ void mma0(float (&d)[4], const A& a, const B& b) {
-        asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-                     : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a.lo[0]), "r"(a.lo[1]), "r"(a.lo[2]), "r"(a.lo[3]), "r"(b.hi[0]), "r"(b.hi[1]), "f"(0.f));
-        one(d, a.hi, b.lo);
-        one(d, a.hi, b.hi);
-    }
     static __device__ __forceinline__ void one(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
         asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
@@ -182,6 +177,13 @@ template <> struct Frag<float> {
     static __device__ __forceinline__ void mma(float (&d)[4], const A& a, const B& b) {
         one(d, a.lo, b.hi);
         one(d, a.hi, b.lo);
+        one(d, a.hi, b.hi);
+    }
+    template <bool> static __device__ __forceinline__ void begin(float (&d)[4], const A& a, const B& b) { mma(d, a, b); }   // d is zero at first
+    // the same with the products of a remainder in sums of their own
+    static __device__ __forceinline__ void mma_apart(float (&d)[4], float (&r)[4], const A& a, const B& b) {
+        one(r, a.lo, b.hi);
+        one(r, a.hi, b.lo);
         one(d, a.hi, b.hi);
     }
     template <int COLS> static __device__ __forceinline__ A ldA(const Tile<float, COLS>& s, int m, int k) {
