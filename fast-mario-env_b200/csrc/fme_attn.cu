@@ -16,7 +16,7 @@
 // thousand flops, so HBM is the floor and warp-level mma is enough for it: the tensor pipe is busy for 38 % of the time. What bounds the
 // kernels now is the rest of the instruction stream (issue slots 45 to 50 % used by 12 to 16 warps an SM, shared memory 52 to 65 %):
 // masks, rounding to operands, stores. Measured on a B200 (HBM copy 6441 GB/s), 1024 x 128 tokens of 8 heads of 64, restarts at 2 %:
-// bf16 forward 133 us (4.0 TB/s of the tensors above), backward 263 us (3.6 TB/s); fp32, 257 x 127 with states in and out: 640 us
+// bf16 forward 133 us (4.0 TB/s of the tensors above), backward 263 us (3.6 TB/s); fp32, 257 x 127 with states in and out: 650 us
 // both, backward 70 % of it, bound by its three tf32 products and the splitting of their operands (ALU 46 %, tensor 39 %).
 // Chunks of 64: with 128 (no state between two chunks of a 128-token rollout, more products within one) the same pass took 486
 // against 441 us. One CTA for each sequence and head: CTAs that walk several with the powers kept took 171 against 153 us forward.
@@ -372,21 +372,30 @@ __device__ __forceinline__ void block_apply(float (&acc)[NB][4], const float (&p
 }
 
 // state (rows m0..m0+15 of the D x D matrix) += (w a)^T b over the chunk's tokens. The scaled rows of bf16 are taken in 16 bits,
-// fine: in 24, where the state itself is asked for, in fp32.
+// fine: in 24, where the state itself is asked for, in fp32. Two loops, the choice outside: with it at each product 3 x 5000 tokens
+// of 4 heads of 128 took 168 and not 153 us, forward and backward, and 1024 x 128 of 8 heads of 64 425 and not 411 us.
 template <typename T, int D, int C, int UNROLL>
 __device__ __forceinline__ void outer(float (&s)[D / 8][4], const Tile<T, D>& a, int m0, const float* w, const Tile<T, D>& b, bool fine) {
     using F = Frag<T>;
-#pragma unroll(sizeof(T) == 2 ? UNROLL : 1)
-    for (int k = 0; k < C; k += F::KS) {
-        const typename F::A2 fa = F::ldAt(a, k, m0, w, fine);
+    auto step = [&](int k, auto all) {
+        const typename F::A2 fa = F::ldAt(a, k, m0, w, decltype(all)::value);
 #pragma unroll
         for (int i = 0; i < D / 8; i += 2) {
             typename F::B b0, b1;
             F::template ldBt<false>(b, k, 8 * i, b0, b1);
-            F::mma2(s[i], fa, b0, fine);
-            F::mma2(s[i + 1], fa, b1, fine);
+            F::template add<decltype(all)::value>(s[i], fa, b0);
+            F::template add<decltype(all)::value>(s[i + 1], fa, b1);
+        }
+    };
+    if constexpr (sizeof(T) == 2) {
+        if (!fine) {
+#pragma unroll(UNROLL)
+            for (int k = 0; k < C; k += F::KS) step(k, std::false_type{});
+            return;
         }
     }
+#pragma unroll 1
+    for (int k = 0; k < C; k += F::KS) step(k, std::true_type{});
 }
 
 template <int D> __device__ __forceinline__ void keep_state(float (&s)[D / 8][4], const Cuts& cuts, const float* pw) {
@@ -486,7 +495,7 @@ constexpr float LOG2E = 1.44269504088896340736f;
 // The forward pass of a segment (state rows: features of v). LOCAL: only its part of the state, from zero (the first: from s_in).
 // P = q k^T goes from accumulators straight to operands; the state's transpose is kept, so that its accumulators, rounded to the
 // operands' type, are the rows that q S reads. Rounded to bf16: P, S as q reads it; o is off by 0.0023 of its norm against 0.0017 by
-// its own rounding alone. One env's 16384 tokens, 8 heads of 64, bf16: 18 us (parts) + 8 (join) + 31, started behind each other 47.
+// its own rounding alone. One env's 16384 tokens, 8 heads of 64, bf16: parts, join and outputs, started behind each other, 49 us.
 // STAGES: 2 loads the next chunk while this one is computed, for CTAs that have an SM to themselves or nearly so.
 template <typename T, int D, bool LOCAL, int STAGES, int MINB>
 __global__ void __launch_bounds__(Shape<T, D>::NT, MINB) k_attn_fwd(const FmeDecayAttn A, const Walkers W) {
@@ -606,7 +615,7 @@ __global__ void __launch_bounds__(Shape<T, D>::NT, MINB) k_attn_fwd(const FmeDec
 // The backward pass of a segment, from its last chunk to its first (state rows: features of k). LOCAL: only its part of the
 // state's gradient, from zero (the last: from ds_out); segments then count from the end. TWO: ds_in is wanted.
 // A warp finds do v^T twice, once by rows and once by columns: two products more, no exchange through shared memory and no barrier.
-// 3 x 5000 tokens, 4 heads of 128, bf16: 28 us (parts) + 8 (join) + 74, one CTA of 8 warps an SM, bound by latency.
+// 3 x 5000 tokens, 4 heads of 128, bf16: 154 us with the forward pass's, one CTA of 8 warps an SM, bound by latency.
 template <typename T, int D, bool LOCAL, bool TWO, int MINB>
 __global__ void __launch_bounds__(Shape<T, D>::NT, MINB) k_attn_bwd(const FmeDecayAttn A, const Walkers W) {
     using Z = Shape<T, D>;
@@ -879,7 +888,7 @@ template <typename T, int D> struct Plan {
         W.per = W.chunks;
         W.parts = (float*)a.ws;
         // Segments where half the GPU or more would idle: as many as make one wave, of four chunks at least. 3 x 5000 tokens, 4 heads
-        // of 128: 168 us with 12 segments (144 CTAs on 148 SMs), 250 us with 16 (192 CTAs). Splitting costs a second read of k and v
+        // of 128: 168 us with 12 segments (144 CTAs on 148 SMs; now 154), 250 us with 16 (192 CTAs). Splitting costs a second read of k and v
         // (q and do), so a GPU that is more than half full is left as it is.
         const int64_t slots = (int64_t)SMS * ctas;
         if (pairs > 0 && 2 * pairs <= slots && W.chunks >= 2 * SEG_CHUNKS) {

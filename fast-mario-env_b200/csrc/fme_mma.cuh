@@ -146,10 +146,20 @@ template <> struct Frag<bf16> {
         }
         return a;
     }
-    static __device__ __forceinline__ void mma2(float (&d)[4], const A2& a, const B& b, bool fine) {
-        if (fine) mma(d, a.rest, b);
-        mma(d, a.lo, b);
-        mma(d, a.hi, b);
+    // FINE: with 24 bits, and through a sum of its own. The tensor core cuts a sum off at the accumulator's last bit, always
+    // towards zero, which adds up over many chunks, where an addition rounds to nearest. 16384 tokens: 49 and not 47 us.
+    template <bool FINE> static __device__ __forceinline__ void add(float (&d)[4], const A2& a, const B& b) {
+        if constexpr (FINE) {
+            float t[4];
+            begin<true>(t, a.rest, b);
+            mma(t, a.lo, b);
+            mma(t, a.hi, b);
+#pragma unroll
+            for (int i = 0; i < 4; i++) d[i] += t[i];
+        } else {
+            mma(d, a.lo, b);
+            mma(d, a.hi, b);
+        }
     }
     // The accumulators of 16 columns as an operand whose k runs over them
     static __device__ __forceinline__ A chain(const float (*acc)[4], int ks) {
@@ -230,7 +240,13 @@ template <> struct Frag<float> {
         }
         return a;
     }
-    static __device__ __forceinline__ void mma2(float (&d)[4], const A2& a, const B& b, bool) { mma(d, a, b); }
+    // through a sum of its own, as bf16's; at 2 x 4729 tokens the error falls from 2.7e-6 to 8e-7 for 1 % of the time
+    template <bool> static __device__ __forceinline__ void add(float (&d)[4], const A2& a, const B& b) {
+        float t[4] = {0.f, 0.f, 0.f, 0.f};
+        mma(t, a, b);
+#pragma unroll
+        for (int i = 0; i < 4; i++) d[i] += t[i];
+    }
     static __device__ __forceinline__ A chain(const float (*acc)[4], int ks) {
         const float* u = acc[ks];
         A a;
