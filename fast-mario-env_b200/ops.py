@@ -13,9 +13,11 @@ same inputs give the same bits. There is no CPU path. The reference has no count
 from __future__ import annotations
 
 import ctypes
+import sys
 from functools import lru_cache
 
 import torch
+import torch.autograd.forward_ad as _fw
 from torch.autograd.function import once_differentiable
 from torch.autograd.graph import increment_version
 
@@ -28,6 +30,19 @@ MAX_CHANNELS = 4096
 _fns = {}
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _current = torch._C._cuda_getDevice
+_traced = torch._C._get_tracing_state
+_modes = torch._C._len_torch_dispatch_stack
+
+
+def _followed(*tensors):
+    """Whether forward-mode differentiation or torch.jit.trace follows this call. To both, an output that a kernel writes is
+    an empty tensor without a history; the autograd function refuses the one and stands in the other's record as a call.
+    make_fx looks inside that function too, so it is refused here."""
+    if _modes():
+        proxies = sys.modules.get("torch.fx.experimental.proxy_tensor")
+        if proxies is not None and proxies.get_proxy_mode() is not None:
+            raise RuntimeError("make_fx cannot record this operator: it would replay its outputs empty")
+    return _traced() is not None or _fw._current_level >= 0 and any(t is not None and _fw.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def _call(name, args, index):
@@ -183,11 +198,12 @@ def decay_attention(q, k, v, log_decay, *, reset=None, state=None, scale=None, r
     before the first token, default zeros. scale: default D ** -0.5. Returns (o, state after the last token), the state
     None unless return_state. Gradients for q, k, v and state."""
     _check_qkv(q, k, v, log_decay, reset, state, 2)
-    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
+    scale = float(q.shape[-1] ** -0.5 if scale is None else scale)
+    follow = _followed(q, k, v, log_decay, state)
     q, k, v, log_decay = _rows(q), _rows(k), _rows(v), log_decay.contiguous()
     if state is not None:
         state = state.contiguous()
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (state is not None and state.requires_grad)):
+    if follow or torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (state is not None and state.requires_grad)):
         return _DecayAttention.apply(q, k, v, log_decay, reset, state, scale, return_state)
     o, last, _ = _attn_forward(q, k, v, log_decay, reset, state, scale, return_state, False)
     return o, last
@@ -199,6 +215,8 @@ def decay_attention_step(q, k, v, log_decay, state, *, reset=None, scale=None, o
     _check_qkv(q, k, v, log_decay, reset, state, 1)
     if state is None or not state.is_contiguous() or state.requires_grad:
         raise ValueError("state must be contiguous and without a gradient: it is updated in place")
+    if _followed(q, k, v, log_decay, state):
+        raise RuntimeError("a step has no forward-mode derivative and leaves no trace: it updates its state in place")
     n, h, d = q.shape
     if out is None:
         out = torch.empty((n, h, d), dtype=q.dtype, device=q.device)
@@ -353,6 +371,6 @@ def group_norm_act(x, groups, weight=None, bias=None, *, eps=1e-5, act="silu", c
             if t.shape != (c,) or t.dtype != torch.float32 or t.get_device() != x.get_device() or not t.is_contiguous():
                 raise ValueError(f"{name} must be a contiguous float32 ({c},) tensor on x's device")
             grad = grad or t.requires_grad
-    if grad and torch.is_grad_enabled():
+    if _followed(x, weight, bias) or grad and torch.is_grad_enabled():
         return _GroupNormAct.apply(x, weight, bias, groups, eps, _ACTS[act], checkpoint == "u8")
     return _norm_forward(x, groups, weight, bias, eps, _ACTS[act], False, False)[0]

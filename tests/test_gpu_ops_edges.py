@@ -1,0 +1,59 @@
+"""The memory policy's operators where a call is easily answered wrongly: derivatives and traces that pass a kernel by, outputs
+that overlap themselves, tensors off their boundary or of another layout, and values at the ends of the range."""
+import pytest
+import torch
+from conftest import fme  # noqa: F401  (loads the package)
+from test_gpu_ops import DEV, make
+
+from fast_mario_env_b200 import ops
+
+pytestmark = pytest.mark.gpu
+
+
+def seq(t=5, d=64, dtype=torch.float32, seed=40):
+    c = make(2, t, 2, d, dtype, None, True, seed=seed)
+    return [c[x].to(DEV) for x in ("q", "k", "v")], c["g"].to(DEV), c["state"].to(DEV)
+
+
+# ---------------------------------------------------------------------------------------------- derivatives and traces
+@pytest.mark.parametrize("which", ["q", "v", "state", "log_decay"])
+def test_forward_mode_is_refused(which):
+    """A dual tensor wants a tangent of the output, which no kernel computes."""
+    fw = torch.autograd.forward_ad
+    (q, k, v), g, s = seq()
+    with fw.dual_level():
+        kw = dict(q=q, k=k, v=v, log_decay=g, state=s)
+        assert ops.decay_attention(**kw)[0].isfinite().all()        # no tangent: nothing to refuse
+        kw[which] = fw.make_dual(kw[which], torch.ones_like(kw[which]))
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            ops.decay_attention(**kw)
+        one = {**kw, **{x: kw[x][:, 0] for x in ("q", "k", "v")}}
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            ops.decay_attention_step(**one)
+        x, w = torch.randn(4, 16, device=DEV), torch.ones(16, device=DEV)
+        assert ops.group_norm_act(x, 2, w).isfinite().all()
+        for a in ((fw.make_dual(x, x), 2, w), (x, 2, fw.make_dual(w, w)), (x, 2, w, fw.make_dual(w, w))):
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                ops.group_norm_act(*a)
+
+
+@pytest.mark.filterwarnings("ignore")
+def test_a_trace_computes_and_does_not_replay_empty_outputs():
+    (q, k, v), g, s = seq()
+    f = torch.jit.trace(lambda q, k, v: ops.decay_attention(q, k, v, g, state=s)[0], (q, k, v), check_trace=False)
+    assert torch.equal(f(2 * q, k, v), ops.decay_attention(2 * q, k, v, g, state=s)[0])
+    x = torch.randn(4, 16, device=DEV)
+    f = torch.jit.trace(lambda x: ops.group_norm_act(x, 2), (x,), check_trace=False)
+    y = torch.randn(4, 16, device=DEV)
+    assert torch.equal(f(y), ops.group_norm_act(y, 2))
+    with pytest.raises(RuntimeError, match="trace"):
+        torch.jit.trace(lambda q: ops.decay_attention_step(q[:, 0], k[:, 0], v[:, 0], g, s), (q,), check_trace=False)
+
+
+def test_make_fx_is_refused():
+    from torch.fx.experimental.proxy_tensor import make_fx
+    (q, k, v), g, s = seq()
+    for f in (lambda q: ops.decay_attention(q, k, v, g)[0], lambda q: ops.decay_attention_step(q[:, 0], k[:, 0], v[:, 0], g, s),
+              lambda q: ops.group_norm_act(q[:, 0, 0], 2)):
+        with pytest.raises(RuntimeError, match="make_fx"):
+            make_fx(f)(q)
