@@ -152,6 +152,7 @@ def _attn_forward(q, k, v, log_decay, reset, state, scale, return_state, keep):
 
 def _attn_backward(ctx, do, dlast):
     q, k, v, log_decay, reset, state, saved = ctx.saved_tensors
+    q, k, v = _rows(q), _rows(k), _rows(v)   # a hook on saved tensors may hand them back in another layout
     n, t, h, d = q.shape
     dev, dtype = q.device, _DTYPES[q.dtype]
     do = torch.zeros_like(q) if do is None else _rows(do)
@@ -251,6 +252,11 @@ def _channels_last(x):
     return True
 
 
+def _relaid(x):
+    """x itself if it has channels-last memory, else a copy that does."""
+    return x if _channels_last(x) else x.movedim(1, -1).contiguous().movedim(-1, 1)
+
+
 def _like(x):
     """A dense channels-last tensor of x's shape and dtype."""
     if x.dim() == 4:
@@ -300,8 +306,9 @@ def _norm_forward(x, groups, weight, bias, eps, act, keep, u8):
 def _norm_backward(ctx, dy):
     kept, weight, bias, stats = ctx.saved_tensors
     groups, eps, act, u8 = ctx.how
-    if not _channels_last(dy):
-        dy = dy.movedim(1, -1).contiguous().movedim(-1, 1)
+    dy = _relaid(dy)
+    if not u8:
+        kept = _relaid(kept)   # a hook on saved tensors (pinned offloading) may hand it back in another layout
     shape = dy.shape
     n, c, p = shape[0], shape[1], _pixels(shape)
     dtype, dev, dyp, dy_sn, mean = _DTYPES[dy.dtype], dy.device, dy.data_ptr(), dy.stride(0), stats.data_ptr()

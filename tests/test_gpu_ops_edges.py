@@ -3,7 +3,7 @@ that overlap themselves, tensors off their boundary or of another layout, and va
 import pytest
 import torch
 from conftest import fme  # noqa: F401  (loads the package)
-from test_gpu_ops import DEV, make
+from test_gpu_ops import DEV, last_dense, make, norm_case
 
 from fast_mario_env_b200 import ops
 
@@ -57,3 +57,24 @@ def test_make_fx_is_refused():
               lambda q: ops.group_norm_act(q[:, 0, 0], 2)):
         with pytest.raises(RuntimeError, match="make_fx"):
             make_fx(f)(q)
+
+
+# ---------------------------------------------------------------------------------------------- layouts
+def test_saved_tensors_that_come_back_in_another_layout():
+    """Hooks may hand back what was saved with other strides, as torch's own pinned offloading does."""
+    x, w, b, dy = norm_case((3, 16, 5, 4), 4, torch.float32, seed=41)
+    (q, k, v), g, s = seq(t=70)
+    r = (torch.rand(2, 70, device=DEV) < 0.1).t().contiguous().t()
+    qs = [i.transpose(1, 2).contiguous().transpose(1, 2).requires_grad_() for i in (q, k, v)]
+    gx, gw, gb = last_dense(x.to(DEV)).requires_grad_(), w.to(DEV).requires_grad_(), b.to(DEV).requires_grad_()
+
+    def grads():
+        y = ops.group_norm_act(gx, 4, gw, gb)
+        o, _ = ops.decay_attention(*qs, g, reset=r, state=s)
+        return lambda: (*torch.autograd.grad(y, (gx, gw, gb), last_dense(dy.to(DEV))), *torch.autograd.grad(o, qs, torch.ones_like(o)))
+
+    want = grads()()
+    with torch.autograd.graph.save_on_cpu(pin_memory=True):
+        later = grads()
+    for a, c in zip(want, later()):
+        assert torch.equal(a, c)
