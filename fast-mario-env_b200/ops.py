@@ -85,6 +85,11 @@ def _rows(x):
     return x.clone(memory_format=torch.contiguous_format)
 
 
+def _matrices(x):
+    """x itself if it is contiguous on a 16-byte boundary, else a copy (a state, or its gradient)."""
+    return x if x.is_contiguous() and x.data_ptr() & 15 == 0 else x.clone(memory_format=torch.contiguous_format)
+
+
 def _t4(x):
     """(pointer, strides) of an (N, T, H, D) tensor; the stride of an axis of one element is not used and given as 0."""
     n, t, h, _ = x.shape
@@ -156,7 +161,8 @@ def _attn_backward(ctx, do, dlast):
     n, t, h, d = q.shape
     dev, dtype = q.device, _DTYPES[q.dtype]
     do = torch.zeros_like(q) if do is None else _rows(do)
-    dlast = None if dlast is None else dlast.contiguous()
+    dlast = None if dlast is None else _matrices(dlast)
+    state = None if state is None else _matrices(state)
     if q.is_contiguous():
         dq, dk, dv = torch.empty_like(q), torch.empty_like(q), torch.empty_like(q)
     else:
@@ -203,7 +209,7 @@ def decay_attention(q, k, v, log_decay, *, reset=None, state=None, scale=None, r
     follow = _followed(q, k, v, log_decay, state)
     q, k, v, log_decay = _rows(q), _rows(k), _rows(v), log_decay.contiguous()
     if state is not None:
-        state = state.contiguous()
+        state = _matrices(state)
     if follow or torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (state is not None and state.requires_grad)):
         return _DecayAttention.apply(q, k, v, log_decay, reset, state, scale, return_state)
     o, last, _ = _attn_forward(q, k, v, log_decay, reset, state, scale, return_state, False)
@@ -216,6 +222,8 @@ def decay_attention_step(q, k, v, log_decay, state, *, reset=None, scale=None, o
     _check_qkv(q, k, v, log_decay, reset, state, 1)
     if state is None or not state.is_contiguous() or state.requires_grad:
         raise ValueError("state must be contiguous and without a gradient: it is updated in place")
+    if state.data_ptr() & 15:
+        raise ValueError("state must start on a 16-byte boundary: it is updated in place")
     if _followed(q, k, v, log_decay, state):
         raise RuntimeError("a step has no forward-mode derivative and leaves no trace: it updates its state in place")
     n, h, d = q.shape

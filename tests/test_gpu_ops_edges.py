@@ -60,6 +60,25 @@ def test_make_fx_is_refused():
 
 
 # ---------------------------------------------------------------------------------------------- layouts
+def off_by_one(x):
+    return torch.empty(x.numel() + 1, dtype=x.dtype, device=x.device)[1:].view(x.shape).copy_(x)
+
+
+def test_states_and_their_gradients_off_a_boundary():
+    (q, k, v), g, s = seq()
+    q.requires_grad_()
+    want_o, want = ops.decay_attention(q, k, v, g, state=s)
+    o, last = ops.decay_attention(q, k, v, g, state=off_by_one(s))
+    assert torch.equal(o, want_o) and torch.equal(last, want)
+    dl = torch.randn_like(last)
+    a = torch.autograd.grad(want, q, dl, retain_graph=True)[0]
+    assert torch.equal(torch.autograd.grad(last, q, off_by_one(dl))[0], a)
+    b = torch.autograd.grad(torch.cat([torch.ones(1, device=DEV), want.flatten()]), q, torch.cat([torch.ones(1, device=DEV), dl.flatten()]))[0]
+    assert torch.equal(b, a)
+    with pytest.raises(ValueError, match="16-byte"):   # updated in place: a copy would not do
+        ops.decay_attention_step(q[:, 0].detach(), k[:, 0], v[:, 0], g, off_by_one(s))
+
+
 def test_saved_tensors_that_come_back_in_another_layout():
     """Hooks may hand back what was saved with other strides, as torch's own pinned offloading does."""
     x, w, b, dy = norm_case((3, 16, 5, 4), 4, torch.float32, seed=41)
