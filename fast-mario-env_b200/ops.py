@@ -218,7 +218,8 @@ def decay_attention(q, k, v, log_decay, *, reset=None, state=None, scale=None, r
 
 def decay_attention_step(q, k, v, log_decay, state, *, reset=None, scale=None, out=None):
     """One token of `decay_attention` for each of N envs, for acting: q, k, v (N, H, D), reset (N,), and state
-    (N, H, D, D) float32 contiguous, which is updated in place. Returns o (N, H, D), in `out` where given. No gradient."""
+    (N, H, D, D) float32 contiguous, which is updated in place. Returns o (N, H, D), in `out` where given
+    (which may be q, k or v itself, but may not overlap them or the state otherwise). No gradient."""
     _check_qkv(q, k, v, log_decay, reset, state, 1)
     if state is None or not state.is_contiguous() or state.requires_grad:
         raise ValueError("state must be contiguous and without a gradient: it is updated in place")
@@ -231,6 +232,8 @@ def decay_attention_step(q, k, v, log_decay, state, *, reset=None, scale=None, o
         out = torch.empty((n, h, d), dtype=q.dtype, device=q.device)
     elif out.shape != q.shape or out.dtype != q.dtype or out.get_device() != q.get_device() or _rows(out) is not out:
         raise ValueError("out must have q's shape, dtype and device, with 16-byte aligned rows")
+    elif _shares_memory(out):
+        raise ValueError("rows of out must not overlap")
     q, k, v = _rows(q), _rows(k), _rows(v)
     log_decay = log_decay.contiguous()
     s = state.data_ptr()
@@ -239,6 +242,18 @@ def decay_attention_step(q, k, v, log_decay, state, *, reset=None, scale=None, o
                       _ptr(reset), 0 if reset is None else reset.stride(0), 0, s, s, *_NO4, *_NO4, *_NO4, *_NO4, 0, 0, 0, 0, 0), q.get_device())
     increment_version((state, out))   # a backward pass that kept either notices
     return out
+
+
+def _shares_memory(x):
+    """Whether two rows of an (n, h, d) tensor overlap: n CTAs would write one place in no order."""
+    n, h, d = x.shape
+    sn, sh = (x.stride(0) if n > 1 else 0), (x.stride(1) if h > 1 else 0)
+    if (n == 1 or sn >= (h - 1) * sh + d) and (h == 1 or sh >= d) or (h == 1 or sh >= (n - 1) * sn + d) and (n == 1 or sn >= d):
+        return False
+    if n > 1 and sn == 0:
+        return True
+    # rows i sn + j sh: some difference of two, j heads and as many sequences as come nearest, is less than a row
+    return any(abs(i * sn - j * sh) < d for j in range(h) for i in ((j * sh // sn, j * sh // sn + 1) if n > 1 else (0,)) if (i or j) and i < n)
 
 
 def _t3(x):

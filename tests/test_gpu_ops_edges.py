@@ -97,3 +97,16 @@ def test_saved_tensors_that_come_back_in_another_layout():
         later = grads()
     for a, c in zip(want, later()):
         assert torch.equal(a, c)
+
+
+def test_an_output_whose_rows_overlap_is_refused():
+    (q, k, v), g, s = seq()
+    q, k, v = q[:, 0], k[:, 0], v[:, 0]
+    keep = s.clone()
+    for out in (torch.zeros(1, 2, 64, device=DEV).expand(2, 2, 64), torch.zeros(2, 1, 64, device=DEV).expand(2, 2, 64),
+                torch.zeros(256, device=DEV).as_strided((2, 2, 64), (32, 64, 1))):
+        with pytest.raises(ValueError, match="overlap"):
+            ops.decay_attention_step(q, k, v, g, s, out=out)
+    assert torch.equal(s, keep)
+    want = ops.decay_attention_step(q, k, v, g, keep)
+    assert torch.equal(ops.decay_attention_step(q, k, v, g, s, out=v), want) and torch.equal(s, keep)

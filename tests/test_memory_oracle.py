@@ -60,6 +60,22 @@ def test_operators_refuse_cpu_tensors():
         ops.group_norm_act(torch.zeros(2, 8), 2)
 
 
+def test_rows_of_an_output_that_overlap_are_found():
+    """Against counting: (n, h, d) views of a buffer, shared axes, interleaved rows and rows that run into each other."""
+    flat = torch.arange(4096)
+    seen = set()
+    for n in (1, 2, 3, 5):
+        for h in (1, 2, 4):
+            for sn in (0, 4, 8, 12, 16, 24, 32, 36, 64):
+                for sh in (0, 4, 8, 12, 16, 20, 24, 40, 64):
+                    x = flat.as_strided((n, h, 8), (sn, sh, 1))
+                    shared = x.unique().numel() < x.numel()
+                    assert ops._shares_memory(x) == shared, (n, h, sn, sh)
+                    seen.add(shared)
+    assert seen == {True, False}
+    assert ops._shares_memory(torch.empty(1, 2, 64).expand(5, 2, 64)) and not ops._shares_memory(torch.empty(5, 4, 64)[:, ::2])
+
+
 def _attn(**kw):
     a = N.FmeDecayAttn(n=1, t=1, h=1, d=64, dtype=N.FME_F32, scale=1.0, log_decay=256)
     for k, v in kw.items():
