@@ -21,8 +21,9 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float
 
 namespace cg = cooperative_groups;
 
-// 1 / (1 + 2^(-z log2 e)) by the approximate exponential and reciprocal: each is off by a few units of 2^-23, as the sums around
-// it. Both of +-inf come out as limits (2^inf = inf, 1 / inf = 0).
+// 1 / (1 + 2^(-z log2 e)) by the approximate exponential and reciprocal, each off by a few units of 2^-23. The product with log2 e is
+// rounded before it is an exponent, so the result's relative error grows for negative z, as |z| 2^-24 (of z times it: less than
+// 2^-24 in all, since z^2 e^z < 0.6). Both of +-inf come out as limits (2^inf = inf, 1 / inf = 0).
 __device__ __forceinline__ float sigmoid(float z) {
     float e, r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z * -1.44269504088896340736f));
@@ -33,7 +34,8 @@ __device__ __forceinline__ float act_fwd(int act, float z) {
     return act == FME_ACT_SILU ? z * sigmoid(z) : act == FME_ACT_RELU ? (z < 0.f ? 0.f : z) : z;
 }
 __device__ __forceinline__ float act_bwd(int act, float z, float dy) {
-    if (act == FME_ACT_SILU) { const float s = sigmoid(z); return dy * (s * fmaf(-z, s, 1.f + z)); }   // s (1 + z (1 - s))
+    // s (1 + z (1 - s)). The form s ((1 + z) - z s) loses the 1 from z = 2^24 on, and digits of it before
+    if (act == FME_ACT_SILU) { const float s = sigmoid(z); return dy * (s * fmaf(z, 1.f - s, 1.f)); }
     return act == FME_ACT_RELU ? (z <= 0.f ? 0.f : dy) : dy;
 }
 

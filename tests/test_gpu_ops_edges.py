@@ -3,7 +3,7 @@ that overlap themselves, tensors off their boundary or of another layout, and va
 import pytest
 import torch
 from conftest import fme  # noqa: F401  (loads the package)
-from test_gpu_ops import DEV, last_dense, make, norm_case
+from test_gpu_ops import DEV, U, last_dense, make, norm_case
 
 from fast_mario_env_b200 import ops
 
@@ -110,3 +110,17 @@ def test_an_output_whose_rows_overlap_is_refused():
     assert torch.equal(s, keep)
     want = ops.decay_attention_step(q, k, v, g, keep)
     assert torch.equal(ops.decay_attention_step(q, k, v, g, s, out=v), want) and torch.equal(s, keep)
+
+
+# ---------------------------------------------------------------------------------------------- values
+def test_silu_slope_of_large_values():
+    """silu'(z) is 1 for large z and 0 for very negative ones, however large |z| is; one value a group keeps x^ at 1 and -1."""
+    x = torch.tensor([[1.0, -1.0, 3.0, -3.0]], device=DEV).repeat(6, 1)
+    for shape, p in (((6, 4), 1), ((6, 4, 8), 8)):
+        gx = (x if p == 1 else last_dense(x[:, :, None].repeat(1, 1, p))).requires_grad_()
+        for scale in (30.0, 1e4, 2.0 ** 25, 1e12):
+            w, b = torch.full((4,), scale, device=DEV), torch.zeros(4, device=DEV, requires_grad=True)
+            y = ops.group_norm_act(gx, 2, w, b)
+            db = torch.autograd.grad(y, b, torch.ones_like(y))[0]
+            want = 6 * p * torch.tensor([1.0, 0.0, 1.0, 0.0], device=DEV)   # silu' - (1 or 0) is below 30 e^-30 = 3e-12
+            assert ((db - want).abs() <= 6 * p * 16 * U).all(), (shape, scale, db)
