@@ -845,30 +845,51 @@ __global__ void __launch_bounds__(NT, KV == 4 ? 1 : 2) k_norm_rows_bwd(const Fme
     }
 }
 
-// ---------------------------------------------------------------- many channels of an odd number
-// Channel counts whose vectors repeat only after more than MAX_THREADS (odd ones above 512, mostly): one thread a channel,
-// x read three times. One CTA walks samples blockIdx.x, + gridDim.x, ...; per-channel sums in shared memory, one thread a channel.
+// ---------------------------------------------------------------- calls without a plan
+// What make_plan refuses: vectors whose channels repeat only after more than MAX_THREADS of them (odd channel counts above 512,
+// fp32 ones above 2048, and with c > 512 whatever cannot be read in 16-byte pieces), and more groups than shared memory has
+// room for the sums of. One thread a channel, x read three times. One CTA walks samples blockIdx.x, + gridDim.x, ...;
+// per-channel sums in shared memory, one thread a channel, joined by one warp a group.
+
+// A sum that carries what each addition rounds off (Kahan): a thread adds up all pixels of a channel, and without it the mean of a
+// constant group of 4096 pixels came out 737 units of 2^-24 away from the constant.
+struct Sum {
+    float s = 0.f, c = 0.f;
+    __device__ __forceinline__ void take(float y) { const float t = s + y; c = (t - s) - y; s = t; }
+    __device__ __forceinline__ void add(float x) { take(x - c); }
+    __device__ __forceinline__ void add(float x, float y) { take(fmaf(x, y, -c)); }
+};
+
 template <typename T> __global__ void __launch_bounds__(NT) k_norm_wide_fwd(const FmeGroupNorm A) {
     extern __shared__ float wide[];
-    float *s0 = wide, *s1 = wide + A.c, *s2 = wide + 2 * A.c;
-    const int cg = A.c / A.g;
+    float *s0 = wide, *s1 = wide + A.c, *s2 = wide + 2 * A.c, *s3 = wide + 3 * A.c;
+    const int cg = A.c / A.g, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const float m = (float)((int64_t)A.p * cg);
     for (int64_t n = blockIdx.x; n < A.n; n += gridDim.x) {
         const T* x = (const T*)A.x + n * A.x_sn;
         const int64_t base = n * (int64_t)A.p * A.c;
         for (int c = threadIdx.x; c < A.c; c += NT) {
-            float s = 0.f, lo = INFINITY, hi = -INFINITY;
-            for (int64_t p = 0; p < A.p; p++) { const float v = to_f(x[p * A.c + c]); s += v; lo = fminf(lo, v); hi = fmaxf(hi, v); }
-            s0[c] = s; s1[c] = lo; s2[c] = hi;
+            Sum s;
+            float lo = INFINITY, hi = -INFINITY;
+            for (int64_t p = 0; p < A.p; p++) { const float v = to_f(x[p * A.c + c]); s.add(v); lo = fminf(lo, v); hi = fmaxf(hi, v); }
+            s0[c] = s.s; s3[c] = s.c; s1[c] = lo; s2[c] = hi;
         }
         __syncthreads();
-        for (int g = threadIdx.x; g < A.g; g += NT) {
-            float s = 0.f, lo = INFINITY, hi = -INFINITY;
-            for (int c = g * cg; c < (g + 1) * cg; c++) { s += s0[c]; lo = fminf(lo, s1[c]); hi = fmaxf(hi, s2[c]); }
-            s /= m;
-            for (int c = g * cg; c < (g + 1) * cg; c++) { s0[c] = s; s1[c] = lo; s2[c] = hi; }
-            if (A.codes) { A.lo[n * A.g + g] = lo; A.hi[n * A.g + g] = hi; }
-            if (A.mean) A.mean[n * A.g + g] = s;
+        for (int g = warp; g < A.g; g += NT / 32) {
+            double s = 0.;   // so that the mean is rounded once: of a constant group it is the constant
+            float lo = INFINITY, hi = -INFINITY;
+            for (int c = g * cg + lane; c < (g + 1) * cg; c += 32) { s += (double)s0[c] - (double)s3[c]; lo = fminf(lo, s1[c]); hi = fmaxf(hi, s2[c]); }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) {
+                s += __shfl_xor_sync(0xffffffffu, s, o);
+                lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o)); hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+            }
+            const float mean = (float)(s / ((double)A.p * cg));
+            for (int c = g * cg + lane; c < (g + 1) * cg; c += 32) { s0[c] = mean; s1[c] = lo; s2[c] = hi; }
+            if (lane == 0) {
+                if (A.codes) { A.lo[n * A.g + g] = lo; A.hi[n * A.g + g] = hi; }
+                if (A.mean) A.mean[n * A.g + g] = mean;
+            }
         }
         __syncthreads();
         if (A.codes) {
@@ -880,17 +901,17 @@ template <typename T> __global__ void __launch_bounds__(NT) k_norm_wide_fwd(cons
         }
         __syncthreads();
         for (int c = threadIdx.x; c < A.c; c += NT) {
-            float q = 0.f;
-            for (int64_t p = 0; p < A.p; p++) { const float d = to_f(x[p * A.c + c]) - s0[c]; q = fmaf(d, d, q); }
-            s1[c] = q;
+            Sum q;
+            for (int64_t p = 0; p < A.p; p++) { const float d = to_f(x[p * A.c + c]) - s0[c]; q.add(d, d); }
+            s1[c] = q.s;
         }
         __syncthreads();
-        for (int g = threadIdx.x; g < A.g; g += NT) {
-            float q = 0.f;
-            for (int c = g * cg; c < (g + 1) * cg; c++) q += s1[c];
-            const float r = rsqrtf(q / m + A.eps);
-            for (int c = g * cg; c < (g + 1) * cg; c++) s2[c] = r;
-            if (A.rstd) A.rstd[n * A.g + g] = r;
+        for (int g = warp; g < A.g; g += NT / 32) {
+            Sum q;
+            for (int c = g * cg + lane; c < (g + 1) * cg; c += 32) q.add(s1[c]);
+            const float r = rsqrtf(lanes_sum<32>(q.s) / m + A.eps);
+            for (int c = g * cg + lane; c < (g + 1) * cg; c += 32) s2[c] = r;
+            if (A.rstd && lane == 0) A.rstd[n * A.g + g] = r;
         }
         __syncthreads();
         for (int c = threadIdx.x; c < A.c; c += NT) {
@@ -911,7 +932,7 @@ template <typename T> __device__ __forceinline__ float x_of(const FmeGroupNorm& 
 template <typename T> __global__ void __launch_bounds__(NT) k_norm_wide_bwd(const FmeGroupNorm A) {
     extern __shared__ float wide[];
     float *s0 = wide, *s1 = wide + A.c, *tw = wide + 2 * A.c, *tb = wide + 3 * A.c;
-    const int cg = A.c / A.g;
+    const int cg = A.c / A.g, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const float m = (float)((int64_t)A.p * cg);
     for (int c = threadIdx.x; c < A.c; c += NT) tw[c] = tb[c] = 0.f;
     __syncthreads();
@@ -922,22 +943,23 @@ template <typename T> __global__ void __launch_bounds__(NT) k_norm_wide_bwd(cons
                 const int64_t ng = n * A.g + c / cg;
                 const float mean = A.mean[ng], rstd = A.rstd[ng], w = A.w ? A.w[c] : 1.f, b = A.b ? A.b[c] : 0.f;
                 const float lo = A.codes ? A.lo[ng] : 0.f, step = A.codes ? __fdiv_rn(__fsub_rn(A.hi[ng], lo), 255.f) : 0.f;
-                float a1 = 0.f, a2 = 0.f;
+                Sum a1, a2;
                 for (int64_t p = 0; p < A.p; p++) {
                     const int64_t i = p * A.c + c;
                     const float xh = (x_of<T>(A, n, i, lo, step) - mean) * rstd;
                     const float dz = act_bwd(A.act, fmaf(xh, w, b), to_f(dy[i]));
-                    if (pass == 0) { a1 += dz; a2 = fmaf(dz, xh, a2); }
+                    if (pass == 0) { a1.add(dz); a2.add(dz, xh); }
                     else ((T*)A.dx)[n * (int64_t)A.p * A.c + i] = from_f<T>(rstd * (dz * w - s0[c] - xh * s1[c]));
                 }
-                if (pass == 0) { s0[c] = a1; s1[c] = a2; tb[c] += a1; tw[c] += a2; }
+                if (pass == 0) { s0[c] = a1.s; s1[c] = a2.s; tb[c] += a1.s; tw[c] += a2.s; }
             }
             __syncthreads();
             if (pass == 0) {
-                for (int g = threadIdx.x; g < A.g; g += NT) {
-                    float a1 = 0.f, a2 = 0.f;
-                    for (int c = g * cg; c < (g + 1) * cg; c++) { const float w = A.w ? A.w[c] : 1.f; a1 = fmaf(s0[c], w, a1); a2 = fmaf(s1[c], w, a2); }
-                    for (int c = g * cg; c < (g + 1) * cg; c++) { s0[c] = a1 / m; s1[c] = a2 / m; }
+                for (int g = warp; g < A.g; g += NT / 32) {
+                    Sum a1, a2;
+                    for (int c = g * cg + lane; c < (g + 1) * cg; c += 32) { const float w = A.w ? A.w[c] : 1.f; a1.add(s0[c], w); a2.add(s1[c], w); }
+                    const float m1 = lanes_sum<32>(a1.s) / m, m2 = lanes_sum<32>(a2.s) / m;
+                    for (int c = g * cg + lane; c < (g + 1) * cg; c += 32) { s0[c] = m1; s1[c] = m2; }
                 }
                 __syncthreads();
             }
@@ -1023,7 +1045,7 @@ bool make_rows(const FmeGroupNorm& a, bool bwd, Rows* W, int* kv) {
     return true;
 }
 
-// How a call is laid out. false: the kernels for many channels of an odd number.
+// How a call is laid out. false: the kernels for calls without a plan (k_norm_wide_*).
 bool make_plan(const FmeGroupNorm& a, bool bwd, Plan* P) {
     const int e = a.dtype == FME_F32 ? 4 : 2;
     const int vec = vec_of(a, bwd);
@@ -1199,10 +1221,11 @@ int fme_group_norm_fwd(const FmeGroupNorm* a, void* stream) {
     int kv;
     if (make_rows(*a, false, &W, &kv)) return run_rows<false>(*a, W, kv, st);
     if (!make_plan(*a, false, &P)) {
-        const size_t smem = (size_t)3 * a->c * 4;
+        const size_t smem = (size_t)4 * a->c * 4;
         const int grid = a->n < WIDE_GRID ? a->n : WIDE_GRID;
-        if (a->dtype == FME_F32) k_norm_wide_fwd<float><<<grid, NT, smem, st>>>(*a);
-        else k_norm_wide_fwd<__nv_bfloat16><<<grid, NT, smem, st>>>(*a);
+        auto kernel = a->dtype == FME_F32 ? k_norm_wide_fwd<float> : k_norm_wide_fwd<__nv_bfloat16>;
+        if (smem > 48 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        kernel<<<grid, NT, smem, st>>>(*a);
         return launch_status("fme_group_norm_fwd");
     }
     return a->dtype == FME_F32 ? run_fwd<float>(*a, P, st) : run_fwd<__nv_bfloat16>(*a, P, st);

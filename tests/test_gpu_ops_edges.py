@@ -3,7 +3,7 @@ that overlap themselves, tensors off their boundary or of another layout, and va
 import pytest
 import torch
 from conftest import fme  # noqa: F401  (loads the package)
-from test_gpu_ops import DEV, U, last_dense, make, norm_case
+from test_gpu_ops import DEV, U, check_norm, last_dense, make, norm_case
 
 from fast_mario_env_b200 import ops
 
@@ -124,3 +124,14 @@ def test_silu_slope_of_large_values():
             db = torch.autograd.grad(y, b, torch.ones_like(y))[0]
             want = 6 * p * torch.tensor([1.0, 0.0, 1.0, 0.0], device=DEV)   # silu' - (1 or 0) is below 30 e^-30 = 3e-12
             assert ((db - want).abs() <= 6 * p * 16 * U).all(), (shape, scale, db)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("u8", [False, True])
+@pytest.mark.parametrize("shape, groups", [((2, 515, 64, 64), 5), ((2, 2052, 2), 1), ((3, 2055, 1, 2), 3)])
+def test_constant_groups_of_many_channels(shape, groups, u8, dtype):
+    """A constant group: each rounding of a long sum in the same direction moves the mean off it."""
+    x, w, b, dy = norm_case(shape, groups, dtype, seed=42)
+    x[0] = 1000.1
+    x[1, : shape[1] // groups] = -7.3
+    check_norm(x, groups, w, b, dy, "none", u8)
