@@ -1015,6 +1015,7 @@ bool split_parts(const Plan& P) { return P.parts > 1 && !P.cluster; }
 int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
 
 Div divisor(int d) { return Div{(uint32_t)d, d <= 1 ? 0u : (uint32_t)((0x100000000ull + d - 1) / d)}; }
+int64_t round_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 int pow2_up(int x) { int p = 1; while (p < x) p *= 2; return p; }
 
 int vec_of(const FmeGroupNorm& a, bool bwd) {
@@ -1045,28 +1046,13 @@ bool make_rows(const FmeGroupNorm& a, bool bwd, Rows* W, int* kv) {
     return true;
 }
 
-// How a call is laid out. false: the kernels for calls without a plan (k_norm_wide_*).
-bool make_plan(const FmeGroupNorm& a, bool bwd, Plan* P) {
-    const int e = a.dtype == FME_F32 ? 4 : 2;
-    const int vec = vec_of(a, bwd);
-    P->vec = vec;
-    const int per = a.c / gcd(a.c, vec);               // threads after which a vector's channels repeat
-    if (per > MAX_THREADS) return false;
+// The layout with this many parts of `chunk` vectors. false: more shared memory, or more CTAs, than there are.
+bool lay_out(const FmeGroupNorm& a, bool bwd, int parts, bool cluster, int64_t chunk, int per, Plan* P) {
+    const int e = a.dtype == FME_F32 ? 4 : 2, vec = P->vec;
     const int64_t nvec = (int64_t)a.p * a.c / vec;
     const int bpv = vec * (bwd ? e + (a.codes ? 1 : e) : e);
-    auto up = [](int64_t x, int64_t to) { return (x + to - 1) / to * to; };
-    // Parts of some 50 KB: four CTAs an SM. With few samples, more and smaller parts.
-    const int64_t most = 50 * 1024 / bpv, bound = 200 * 1024 / bpv;
-    int parts = 1;
-    while (parts < 16 && (nvec > parts * most || (a.n * (int64_t)parts < 2 * SMS && nvec >= parts * 2048))) parts *= 2;
-    int64_t chunk = up((nvec + parts - 1) / parts, per);
-    P->cluster = parts > 1;
-    if (chunk > bound) {
-        P->cluster = false;
-        parts = (int)((nvec + most - 1) / most);
-        chunk = up((nvec + parts - 1) / parts, per);
-    }
     P->parts = parts;
+    P->cluster = cluster;
     P->chunk = (int)(chunk < per ? per : chunk);
     P->nvec = (int)nvec;
     const bool gr = (a.c / a.g) % vec == 0, whole = a.c % vec == 0;
@@ -1081,10 +1067,10 @@ bool make_plan(const FmeGroupNorm& a, bool bwd, Plan* P) {
     // (64 registers a thread: four CTAs of 256, five of 192; where clusters have to fit beside each other, five)
     const int unit = P->how == WARP ? 32 : per, top = busy ? (parts > 1 ? 192 : 256) : MAX_THREADS;
     if (r > top) r = top;
-    P->R = (int)up(r, unit);
+    P->R = (int)round_up(r, unit);
     if (P->R > top) P->R = top / unit > 0 ? top / unit * unit : unit;
     P->M = 1;
-    P->tile = (int)up((int64_t)P->chunk * bpv, 16);
+    P->tile = (int)round_up((int64_t)P->chunk * bpv, 16);
     if (parts == 1 && P->R <= 128) {
         P->M = 256 / P->R;
         while (P->M > 1 && (int64_t)P->M * P->tile > 50 * 1024) P->M--;
@@ -1112,6 +1098,28 @@ bool make_plan(const FmeGroupNorm& a, bool bwd, Plan* P) {
         P->grid = (int)(groups * parts);
     }
     return groups * parts <= 0x7fffffff && P->smem <= 220 * 1024;
+}
+
+// How a call is laid out. false: the kernels for calls without a plan (k_norm_wide_*).
+bool make_plan(const FmeGroupNorm& a, bool bwd, Plan* P) {
+    const int e = a.dtype == FME_F32 ? 4 : 2;
+    const int vec = vec_of(a, bwd);
+    P->vec = vec;
+    const int per = a.c / gcd(a.c, vec);               // threads after which a vector's channels repeat
+    if (per > MAX_THREADS) return false;
+    const int64_t nvec = (int64_t)a.p * a.c / vec;
+    const int bpv = vec * (bwd ? e + (a.codes ? 1 : e) : e);
+    // Parts of some 50 KB: four CTAs an SM. With few samples, more and smaller parts.
+    const int64_t most = 50 * 1024 / bpv, bound = 200 * 1024 / bpv;
+    int parts = 1;
+    while (parts < 16 && (nvec > parts * most || (a.n * (int64_t)parts < 2 * SMS && nvec >= parts * 2048))) parts *= 2;
+    // What a cluster cannot hold is split: parts that are too large by themselves, and parts that leave no room for the sums
+    // (16 parts of up to 200 KB with 24 to 48 KB of sums beside them: bf16, 112 x 112 x 64 in 32 groups, backward)
+    const int64_t part = round_up((nvec + parts - 1) / parts, per);
+    if (part <= bound && lay_out(a, bwd, parts, parts > 1, part, per, P)) return true;
+    if (parts == 1) return false;
+    parts = (int)((nvec + most - 1) / most);
+    return lay_out(a, bwd, parts, false, round_up((nvec + parts - 1) / parts, per), per, P);
 }
 
 template <typename... Args>

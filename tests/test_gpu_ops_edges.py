@@ -135,3 +135,11 @@ def test_constant_groups_of_many_channels(shape, groups, u8, dtype):
     x[0] = 1000.1
     x[1, : shape[1] // groups] = -7.3
     check_norm(x, groups, w, b, dy, "none", u8)
+
+
+@pytest.mark.parametrize("shape, groups, u8", [((2, 64, 112, 112), 32, False), ((1, 192, 64, 64), 16, False), ((2, 110, 84, 84), 10, False),
+                                               ((2, 128, 112, 112), 32, False), ((1, 192, 74, 74), 16, True), ((1, 192, 75, 75), 16, True)])
+def test_samples_that_a_cluster_just_holds(shape, groups, u8):
+    """bfloat16 samples that 16 CTAs hold without the sums and not with them."""
+    x, w, b, dy = norm_case(shape, groups, torch.bfloat16, seed=43)
+    check_norm(x, groups, w, b, dy, "silu", u8)

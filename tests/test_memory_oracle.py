@@ -138,3 +138,19 @@ def test_empty_calls_need_no_buffers():
     assert N.lib().fme_decay_attn_fwd(ctypes.byref(_attn(n=0)), None) == 0
     a = N.FmeGroupNorm(n=0, p=1, c=8, g=2, dtype=N.FME_F32, act=0, eps=1e-5)
     assert N.lib().fme_group_norm_fwd(ctypes.byref(a), None) == 0
+
+
+LARGE_SAMPLES = [((8, 64, 112, 112), 32, False, 1), ((8, 192, 64, 64), 16, False, 1), ((8, 192, 64, 64), 32, False, 1), ((8, 110, 84, 84), 10, False, 1),
+                 ((8, 128, 112, 112), 32, False, 0), ((8, 192, 74, 74), 16, True, 1), ((4, 192, 75, 75), 16, True, 1), ((36, 192, 65, 65), 16, False, 1)]
+
+
+@pytest.mark.parametrize("shape, groups, u8, which", LARGE_SAMPLES)
+def test_samples_that_a_cluster_just_holds_leave_room_for_their_sums(shape, groups, u8, which):
+    """bfloat16 samples between what 16 CTAs hold with the sums and without them are split into parts, whose sums a workspace
+    holds; they used to be left to one thread a channel (no workspace forward, 592 rows of dw and db backward)."""
+    n, c = shape[:2]
+    p = shape[2] * shape[3]
+    got = ops._norm_size(n, p, c, groups, N.FME_BF16, u8, True, p * c, True, p * c, which)
+    each, row = (16, 0) if which == 0 else (8, 8 * c)   # bytes of a (sample, part, group), and a part's dw and db
+    parts, rest = divmod(got - n * groups * each, n * (groups * each + row))
+    assert rest == 0 and parts > 16
