@@ -12,14 +12,18 @@
 // Where there are too few sequences and heads to fill the GPU, the chunks are split into segments: first every segment's own
 // part of the state, then these joined in order, then all segments at once with the state that they begin with.
 //
-// What it has to move: forward 4 tensors, backward 7. At 64 features that is 1 KB and 1.8 KB a token and head in bf16 for 25 and 55
-// thousand flops, so HBM is the floor and warp-level mma is enough for it: the tensor pipe is busy for 38 % of the time. What bounds the
-// kernels now is the rest of the instruction stream (issue slots 45 to 50 % used by 12 to 16 warps an SM, shared memory 52 to 65 %):
-// masks, rounding to operands, stores. Measured on a B200 (HBM copy 6441 GB/s), 1024 x 128 tokens of 8 heads of 64, restarts at 2 %:
-// bf16 forward 133 us (4.0 TB/s of the tensors above), backward 263 us (3.6 TB/s); fp32, 257 x 127 with states in and out: 650 us
-// both, backward 70 % of it, bound by its three tf32 products and the splitting of their operands (ALU 46 %, tensor 39 %).
+// What it has to move: forward 4 tensors, backward 7, and between them the kept states (D / C tensors written and read). At 64
+// features the tensors are 1 KB and 1.8 KB a token and head in bf16 for 25 and 55 thousand flops, so HBM is the floor. Products are
+// warp-level mma: every warp fetches its operands from shared memory by itself, and do v^T is found twice. The tensor pipe is busy
+// for 35 % of the time; what bounds the kernels now is the rest of the instruction stream (issue slots 45 to 49 % used by 12 to 16
+// warps an SM, shared memory 55 to 68 %): those fetches, masks, rounding to operands, stores. tcgen05 products, which read shared
+// memory by themselves and accumulate outside the registers, would spare the fetches; they are not built.
+// Measured on a B200 (HBM copy 6441 GB/s), 1024 x 128 tokens of 8 heads of 64, restarts at 2 %: bf16 forward 128 us (4.2 TB/s of the
+// tensors above), backward 268 us (3.5 TB/s); fp32, 257 x 127 with states in and out: 647 us both, backward 70 % of it, bound by
+// its three tf32 products and the splitting of their operands at every read (issue slots 51 %, ALU 45 %, tensor 39 %).
 // Chunks of 64: with 128 (no state between two chunks of a 128-token rollout, more products within one) the same pass took 486
-// against 441 us. One CTA for each sequence and head: CTAs that walk several with the powers kept took 171 against 153 us forward.
+// us where it took 441 then. One CTA for each sequence and head: CTAs that walk several with the powers kept took 171 us forward
+// where it took 153 then.
 #include <math.h>
 
 #include <type_traits>
@@ -373,7 +377,7 @@ __device__ __forceinline__ void block_apply(float (&acc)[NB][4], const float (&p
 
 // state (rows m0..m0+15 of the D x D matrix) += (w a)^T b over the chunk's tokens. The scaled rows of bf16 are taken in 16 bits,
 // fine: in 24, where the state itself is asked for, in fp32. Two loops, the choice outside: with it at each product 3 x 5000 tokens
-// of 4 heads of 128 took 168 and not 153 us, forward and backward, and 1024 x 128 of 8 heads of 64 425 and not 411 us.
+// of 4 heads of 128 took 168 and not 153 us, forward and backward, and 1024 x 128 of 8 heads of 64 425 and not 411 us (then).
 template <typename T, int D, int C, int UNROLL>
 __device__ __forceinline__ void outer(float (&s)[D / 8][4], const Tile<T, D>& a, int m0, const float* w, const Tile<T, D>& b, bool fine) {
     using F = Frag<T>;
@@ -615,7 +619,7 @@ __global__ void __launch_bounds__(Shape<T, D>::NT, MINB) k_attn_fwd(const FmeDec
 // The backward pass of a segment, from its last chunk to its first (state rows: features of k). LOCAL: only its part of the
 // state's gradient, from zero (the last: from ds_out); segments then count from the end. TWO: ds_in is wanted.
 // A warp finds do v^T twice, once by rows and once by columns: two products more, no exchange through shared memory and no barrier.
-// 3 x 5000 tokens, 4 heads of 128, bf16: 154 us with the forward pass's, one CTA of 8 warps an SM, bound by latency.
+// 3 x 5000 tokens, 4 heads of 128, bf16: 153 us with the forward pass's, one CTA of 8 warps an SM, bound by latency.
 template <typename T, int D, bool LOCAL, bool TWO, int MINB>
 __global__ void __launch_bounds__(Shape<T, D>::NT, MINB) k_attn_bwd(const FmeDecayAttn A, const Walkers W) {
     using Z = Shape<T, D>;
@@ -806,7 +810,7 @@ __global__ void k_attn_pass(const float* from, float* to, int64_t n) {
 // One CTA a (sequence, head): a thread holds D * D / 256 values of the state in pieces of four columns, all loaded before the
 // first is used. Bound by HBM: the state is read and written once, 8 D * D bytes, against 4 D values of q, k, v and o. Whole rows of
 // CTAs, not split ones: a sequence and head is 16 KB at 64 features, and 128 of them (16 envs) take 4 us.
-// 4096 envs x 8 heads of 64, bf16: 158 us, 6.9 TB/s; 1003 x 4 heads of 128, fp32: 82 us, 6.5 TB/s (copy: 6441 GB/s).
+// 4096 envs x 8 heads of 64, bf16: 156 us, 7.0 TB/s; 1003 x 4 heads of 128, fp32: 82 us, 6.5 TB/s (copy: 6441 GB/s).
 constexpr int STEP_THREADS = 256;
 template <typename T, int D> __global__ void __launch_bounds__(STEP_THREADS) k_attn_step(const FmeDecayAttn A) {
     constexpr int LANES = D / 4, R = STEP_THREADS / LANES, PER = D / R;
@@ -888,7 +892,7 @@ template <typename T, int D> struct Plan {
         W.per = W.chunks;
         W.parts = (float*)a.ws;
         // Segments where half the GPU or more would idle: as many as make one wave, of four chunks at least. 3 x 5000 tokens, 4 heads
-        // of 128: 168 us with 12 segments (144 CTAs on 148 SMs; now 154), 250 us with 16 (192 CTAs). Splitting costs a second read of k and v
+        // of 128: 168 us with 12 segments (144 CTAs on 148 SMs; now 153), 250 us with 16 (192 CTAs). Splitting costs a second read of k and v
         // (q and do), so a GPU that is more than half full is left as it is.
         const int64_t slots = (int64_t)SMS * ctas;
         if (pairs > 0 && 2 * pairs <= slots && W.chunks >= 2 * SEG_CHUNKS) {
@@ -917,7 +921,7 @@ template <typename K> int go(const char* what, K kernel, int64_t grid, int threa
 }
 int join(const char* what, const Walkers& W, int64_t pairs, int dd, cudaStream_t st) {
     if (W.segs == 2) return FME_OK;   // one part: nothing to add
-    auto kernel = W.segs > 17 ? k_attn_join<32> : k_attn_join<16>;   // 63 parts: 8.2 against 9.7 us; 11 parts: 11.8 against 7.5 us
+    auto kernel = W.segs > 17 ? k_attn_join<32> : k_attn_join<16>;   // 63 parts: 8.1 against 9.7 us; 11 parts: 11.8 against 8.4 us
     return launch_behind(what, kernel, dim3((unsigned)((pairs * dd + 127) / 128)), dim3(128), 0, st, W.parts, pairs, W.segs - 1, dd);
 }
 bool has_ws(const FmeDecayAttn& a, int64_t need) { return need == 0 || (a.ws && !((uintptr_t)a.ws & 255) && a.ws_bytes >= need); }

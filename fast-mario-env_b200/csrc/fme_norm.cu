@@ -117,9 +117,9 @@ template <typename T, int VEC> __device__ __forceinline__ Pack<T, VEC> packed(co
 // some load while others compute. Small samples: M teams in a CTA, a sample each. Large ones: the CTAs of a cluster share a
 // sample and add up their sums through distributed shared memory. Where no cluster can hold a sample its pieces are separate
 // CTAs, and the kernel runs twice, for the sums (STATS) and, after k_norm_join*, for the values (APPLY), with a second read.
-// Measured on a B200 (HBM copy 6441 GB/s), forward + backward + sums of dw and db: 1024 x 20 x 20 x 32 fp32 20 + 33 + 6 us (5.2 and
-// 4.7 TB/s); 8192 x 9 x 9 x 64 fp32 with codes 66 + 78 + 8 us (5.8 and 4.9 TB/s), bound by issue slots (80 % used: 50 instructions a
-// value); 37 x 84 x 84 x 48 bf16 with codes, clusters of 16: 29 + 48 + 5 us, of it 10 + 10 for HBM, bound by the sigmoid (two
+// Measured on a B200 (HBM copy 6441 GB/s), forward + backward + sums of dw and db: 1024 x 20 x 20 x 32 fp32 21 + 35 + 8 us (4.9 and
+// 4.5 TB/s); 8192 x 9 x 9 x 64 fp32 with codes 67 + 80 + 10 us (5.7 and 4.8 TB/s), bound by issue slots (65 to 72 % used: 50
+// instructions a value); 37 x 84 x 84 x 48 bf16 with codes, clusters of 16: 31 + 50 + 7 us, of it 10 + 10 for HBM, bound by the sigmoid (two
 // exponentials and two reciprocals a value backward) and by clusters waiting for their last CTA.
 // How a group's sums are found: EACH: a vector's values may belong to several groups (VEC does not divide c / g); ONE: to one
 // group; WARP: to one, and the c / VEC vectors of a pixel are a power of two up to 32, so that shuffles do most of it.
@@ -618,7 +618,7 @@ __global__ void __launch_bounds__(NT) k_norm_join_bwd(const FmeGroupNorm A, cons
 // p = 1 (tokens, heads): a (sample, group) is c / g values in a row, KV vectors for each of LG lanes of a warp. No shared
 // memory and no barrier: shuffles. A lane keeps its channels over the samples that it walks, U of them on their way at a time, the
 // next ones while these are computed; as many CTAs as the GPU holds (one more would run alone after them).
-// 131072 rows of 8 heads of 64, bf16: forward 55 us (4.9 TB/s), backward 71 us (5.7 TB/s); through shared memory 113 + 282 us.
+// 131072 rows of 8 heads of 64, bf16: forward 55 us (4.9 TB/s), backward 72 us (5.6 TB/s); through shared memory 113 + 282 us.
 struct Rows {
     int LG, segs, tall;   // lanes of a group; groups of a CTA at once; samples of a CTA at once (0: the groups take grid.y)
     Div by_g;
@@ -1059,8 +1059,8 @@ bool lay_out(const FmeGroupNorm& a, bool bwd, int parts, bool cluster, int64_t c
     const int cv = whole ? a.c / vec : 0;
     const bool pow2 = gr && cv <= 32 && (cv & (cv - 1)) == 0 && ((cv / a.g) & (cv / a.g - 1)) == 0;
     P->how = !gr ? EACH : pow2 ? WARP : ONE;
-    // Twelve vectors a thread when there is much to do (8192 x 9 x 9 x 64 fp32 with codes: 66 + 78 us, with eight 78 + 88 us, with sixteen
-    // 62 + 77 us, but 1024 x 20 x 20 x 32 then 22 + 36 against 20 + 33 us); two when not: then the call takes as long as one CTA
+    // Twelve vectors a thread when there is much to do (8192 x 9 x 9 x 64 fp32 with codes: 66 + 78 us then, with eight 78 + 88 us, with
+    // sixteen 62 + 77 us, but 1024 x 20 x 20 x 32 22 + 36 against 20 + 33 us); two when not: then the call takes as long as one CTA
     const bool busy = (int64_t)a.n * parts >= 4 * SMS;
     int64_t r = (P->chunk + (busy ? 12 : 2) - 1) / (busy ? 12 : 2);
     if (r < 32) r = P->chunk < 32 ? P->chunk : 32;

@@ -94,7 +94,10 @@ class MemoryAC(nn.Module):
 class MemoryTrainer:
     """PPO with whole rollouts of some envs as minibatches (GAE, advantage normalisation, clipping and the losses as in
     `ppo.py`; src/fast_mario_env/ppo/train.py:112-247 in the reference). cfg.batch counts samples, so a minibatch holds
-    cfg.batch // cfg.n_steps envs."""
+    cfg.batch // cfg.n_steps envs.
+
+    Every step runs eagerly: cfg.graph is not used. Nor is cfg.trunc_budget (all envs that a time limit cuts are bootstrapped, at
+    one look from the host a step) or cfg.channels_last (the norms need that layout). Gradients are not averaged over ranks."""
 
     def __init__(self, env, cfg: PPOConfig, dev, seed: int = 0, net: MemoryAC | None = None):
         torch.manual_seed(seed)

@@ -256,8 +256,8 @@ typedef struct FmeDecayAttn {
     FmeAttnTensor d_o, dq, dk, dv;   /* backward: gradient of o in, gradients of q, k, v out */
     const float* ds_out;        /* gradient of s_out; NULL: zeros */
     float* ds_in;               /* gradient of s_in; NULL: not wanted */
-    float* saved;               /* forward writes, backward reads; see fme_decay_attn_bytes. NULL in a forward pass
-                                   that no backward pass follows */
+    void* saved;                /* states between chunks of tokens, in `dtype`, 16-byte aligned: forward writes, backward
+                                   reads; see fme_decay_attn_bytes. NULL in a forward pass that no backward pass follows */
     void* ws;                   /* workspace, 256-byte aligned */
     int64_t ws_bytes;
 } FmeDecayAttn;
@@ -296,10 +296,12 @@ typedef struct FmeGroupNorm {
     const void* dy;
     void* dx;
     float *dw, *db;             /* (c,) fp32, both or neither */
-    void* ws;                   /* backward workspace, 256-byte aligned */
+    void* ws;                   /* workspace, 16-byte aligned: always in a backward pass, in a forward pass where
+                                   fme_group_norm_bytes asks for one (samples that are split into parts) */
     int64_t ws_bytes;
 } FmeGroupNorm;
-/* Workspace bytes of a call: which = 0 forward, 1 backward. Negative on bad sizes. */
+/* Workspace bytes of a call: which = 0 forward, 1 backward. They depend on the sizes and on whether x, y, dy, dx (with x_sn,
+ * dy_sn) and codes can be read in whole pieces, so those fields are to be filled in as for the call. Negative on bad sizes. */
 int64_t fme_group_norm_bytes(const FmeGroupNorm* a, int32_t which);
 int fme_group_norm_fwd(const FmeGroupNorm* a, void* stream);
 /* dx, dw and db; sums in a fixed order. Async; allocates nothing. */
