@@ -7,7 +7,8 @@ import os
 
 import numpy as np
 
-from ref import gray_lut, rng_state  # noqa: F401  (same seeding / LUT helpers)
+import ref
+from ref import rng_state  # noqa: F401  (same seeding)
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "_ref", "libfme_oracle.so")
@@ -17,6 +18,17 @@ _lib = None
 
 def available() -> bool:
     return os.path.isfile(LIB_PATH)
+
+
+def gray_lut() -> np.ndarray:
+    """The reference's table, or without its build the same arithmetic on the library's palette (the fixtures pin both)."""
+    if ref.available():
+        return ref.gray_lut()
+    from fast_mario_env_b200 import _native
+    p = np.zeros(64, np.uint32)
+    _native.lib().fme_palette(_ptr(p))
+    g = (((p >> 16) & 255) * 4899 + ((p >> 8) & 255) * 9617 + (p & 255) * 1868 + (1 << 13)) >> 14
+    return np.ascontiguousarray(g[np.arange(256) & 63], np.uint8)
 
 
 def lib():
