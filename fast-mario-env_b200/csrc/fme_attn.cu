@@ -204,7 +204,30 @@ template <typename T, int D> struct Left {
     }
 };
 
-// acc (16 x 8 NB) = A B, B the rows of a D x D tile as columns or, TR, its columns as columns
+// Two steps of an fp32 product, 8 NB columns from n on: acc += a0 b(0) + a1 b(1), each 16 x 8 piece through a sum of its own that an
+// addition rounds. In one accumulator each of the 3 K / 8 products cuts off at its last bit, towards zero: with heads of 128
+// the error against 64 bits was 1.2e-6 (now 3.7e-7) and with heads of 64 5.7e-7 to 8.9e-7 (now 3.7e-7 to 5.3e-7), 2e-7 to 3e-7
+// being that of sums in fp32. load(step, i, b0, b1) gives the columns.
+template <int NB, typename F, typename L>
+__device__ __forceinline__ void two_steps(float (&acc)[NB][4], const typename F::A& a0, const typename F::A& a1, L load) {
+#pragma unroll
+    for (int i = 0; i < NB; i += 2) {
+        float t[2][4];
+        typename F::B b0, b1;
+        load(0, i, b0, b1);
+        F::fresh(t[0], a0, b0);
+        F::fresh(t[1], a0, b1);
+        load(1, i, b0, b1);
+        F::mma(t[0], a1, b0);
+        F::mma(t[1], a1, b1);
+#pragma unroll
+        for (int j = 0; j < 4; j++) { acc[i][j] += t[0][j]; acc[i + 1][j] += t[1][j]; }
+    }
+}
+
+// acc (16 x 8 NB) = A B, B the rows of a D x D tile as columns or, TR, its columns as columns. fp32 in two steps at a time with heads of
+// 128 (10 x 556 tokens of 12 heads 838 -> 826 us forward and backward); with heads of 64 that needs more registers than there are
+// for three CTAs (257 x 127 tokens of 8 heads 650 -> 716 us), and half as many products are added up.
 template <typename T, int NB, int D, bool TR>
 __device__ __forceinline__ void product(float (&acc)[NB][4], const Left<T, D>& a, const Tile<T, D>& b, int n) {
     using F = Frag<T>;
@@ -219,6 +242,18 @@ __device__ __forceinline__ void product(float (&acc)[NB][4], const Left<T, D>& a
             F::template begin<decltype(first)::value>(acc[i + 1], fa, b1);
         }
     };
+    if constexpr (sizeof(T) == 4 && D == 128) {
+        zero(acc);
+#pragma unroll 1
+        for (int k = 0; k < D; k += 2 * F::KS) {
+            const typename F::A a0 = a.get(k), a1 = a.get(k + F::KS);
+            two_steps<NB, F>(acc, a0, a1, [&](int s, int i, typename F::B& b0, typename F::B& b1) {
+                if (TR) F::template ldBt<true>(b, k + s * F::KS, n + 8 * i, b0, b1);
+                else F::ldB(b, n + 8 * i, k + s * F::KS, b0, b1);
+            });
+        }
+        return;
+    }
     if constexpr (sizeof(T) == 2) step(0, std::true_type{});
     else zero(acc);
 #pragma unroll(Frag<T>::UNROLL)
@@ -362,16 +397,18 @@ __device__ __forceinline__ void block_scores(float (&p)[2][4], const Left<T, D>&
 template <typename T, int D, int NB>
 __device__ __forceinline__ void block_apply(float (&acc)[NB][4], const float (&p)[2][4], const Tile<T, D>& b, int row, int n) {
     using F = Frag<T>;
-#pragma unroll
-    for (int ks = 0; ks < 16 / F::KS; ks++) {
-        const typename F::A fa = F::chain(p, ks);
+    if constexpr (sizeof(T) == 2) {
+        const typename F::A fa = F::chain(p, 0);
 #pragma unroll
         for (int i = 0; i < NB; i += 2) {
             typename F::B b0, b1;
-            F::template ldBt<false>(b, row + ks * F::KS, n + 8 * i, b0, b1);
+            F::template ldBt<false>(b, row, n + 8 * i, b0, b1);
             F::mma(acc[i], fa, b0);
             F::mma(acc[i + 1], fa, b1);
         }
+    } else {
+        const typename F::A a0 = F::chain(p, 0), a1 = F::chain(p, 1);
+        two_steps<NB, F>(acc, a0, a1, [&](int s, int i, typename F::B& b0, typename F::B& b1) { F::template ldBt<false>(b, row + s * F::KS, n + 8 * i, b0, b1); });
     }
 }
 

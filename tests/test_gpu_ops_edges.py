@@ -3,7 +3,7 @@ that overlap themselves, tensors off their boundary or of another layout, and va
 import pytest
 import torch
 from conftest import fme  # noqa: F401  (loads the package)
-from test_gpu_ops import DEV, U, check_norm, last_dense, make, norm_case
+from test_gpu_ops import DEV, U, check_norm, last_dense, make, norm_case, on_gpu, oracle
 
 from fast_mario_env_b200 import ops
 
@@ -143,3 +143,16 @@ def test_samples_that_a_cluster_just_holds(shape, groups, u8):
     """bfloat16 samples that 16 CTAs hold without the sums and not with them."""
     x, w, b, dy = norm_case(shape, groups, torch.bfloat16, seed=43)
     check_norm(x, groups, w, b, dy, "silu", u8)
+
+
+@pytest.mark.parametrize("t, p_reset", [(2, None), (67, 0.02), (799, None), (1500, 0.003)])
+@pytest.mark.parametrize("d", [32, 64, 128])
+def test_float32_products_lose_no_digits_along_their_sums(d, t, p_reset):
+    """Relative to its norm a float32 result is off by 16 * 2^-24 at most: an operand in two tf32 numbers and the dropped product of
+    the remainders are 3 * 2^-24 of a term, through two products in a row 6; each of the three sums (scores, their product, the
+    state's) adds at most 16 partial sums, each addition off by 2^-25 of what there is, together 2 * 2^-24 as they are independent."""
+    c = make(1, t, 2, d, torch.float32, p_reset, True, seed=44)
+    want = oracle(c, d ** -0.5)
+    for name, x in on_gpu(c).items():
+        err = (x.detach().double().cpu() - want[name]).norm() / want[name].norm()
+        assert err <= 16 * U, (name, float(err))
