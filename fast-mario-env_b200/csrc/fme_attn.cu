@@ -19,8 +19,8 @@
 // warps an SM, shared memory 55 to 68 %): those fetches, masks, rounding to operands, stores. tcgen05 products, which read shared
 // memory by themselves and accumulate outside the registers, would spare the fetches; they are not built.
 // Measured on a B200 (HBM copy 6441 GB/s), 1024 x 128 tokens of 8 heads of 64, restarts at 2 %: bf16 forward 128 us (4.2 TB/s of the
-// tensors above), backward 268 us (3.5 TB/s); fp32, 257 x 127 with states in and out: 647 us both, backward 70 % of it, bound by
-// its three tf32 products and the splitting of their operands at every read (issue slots 51 %, ALU 45 %, tensor 39 %).
+// tensors above), backward 268 us (3.5 TB/s); fp32, 257 x 127 with states in and out: 665 us both, backward 70 % of it, bound by
+// its three tf32 products and the splitting of their operands at every read (issue slots 50 %, ALU 45 %, tensor 38 %).
 // Chunks of 64: with 128 (no state between two chunks of a 128-token rollout, more products within one) the same pass took 486
 // us where it took 441 then. One CTA for each sequence and head: CTAs that walk several with the powers kept took 171 us forward
 // where it took 153 then.
@@ -371,7 +371,7 @@ __device__ __forceinline__ void block_scores(float (&p)[2][4], const Left<T, D>&
             F::mma(p[1], fa, b1);
         }
     } else {   // the products with a remainder are summed apart: an accumulator drops bits at its own size with each addition
-               // (error against 64 bits 6.7e-7 and not 8.3e-7, and the sums wait less for one another: 640 against 646 us, 257 x 127)
+               // (error against 64 bits 6.7e-7 and not 8.3e-7 then, and the sums wait less for one another: 640 against 646 us, 257 x 127)
         float r[2][4];
         zero(r);
 #pragma unroll 2
